@@ -1,8 +1,9 @@
-"""Build libkrk_gemm.so (the C-ABI GEMM library) and libkrk_probe.so (the
-pure-read floor probe bench.py measures against) for gfx950 with hipcc.
+"""Build libkrk_gemm.so (the C-ABI GEMM library), libkrk_attn.so (the cache
+operators between the qkv and o projections) and libkrk_probe.so (the pure-read
+floor probe bench.py measures against) for gfx950 with hipcc.
 
 Usage: ``python kernel-rush-kawk_amd/build_lib.py`` (or ``build()`` /
-``build_probe()`` from Python).  The libraries are written next to this file
+``build_attn()`` / ``build_probe()`` from Python).  The libraries are written next to this file
 so they ship with the tree.  hipcc cross-compiles for gfx950 without a GPU
 present.
 """
@@ -19,6 +20,8 @@ ROOT = HERE.parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libkrk_gemm.so"
 SOURCES = [CSRC / "krk_gemm.hip"]
+ATTN_LIB = HERE / "libkrk_attn.so"
+ATTN_SOURCES = [CSRC / "krk_attn.hip"]
 PROBE_LIB = HERE / "libkrk_probe.so"
 PROBE_SOURCES = [CSRC / "krk_probe.hip"]
 HEADERS = sorted(CSRC.glob("*.h")) + [ROOT / "include" / "krk_gemm.h"]
@@ -62,6 +65,11 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None, out: Path
     return out
 
 
+def build_attn(verbose: bool = False) -> Path:
+    """Compile libkrk_attn.so (cache attention, rotary embedding, eviction); always recompiles."""
+    return build(verbose, out=ATTN_LIB, sources=ATTN_SOURCES)
+
+
 def build_probe(verbose: bool = False) -> Path:
     """Compile libkrk_probe.so (bench.py's pure-read floor); always recompiles."""
     return build(verbose, out=PROBE_LIB, sources=PROBE_SOURCES)
@@ -70,5 +78,6 @@ def build_probe(verbose: bool = False) -> Path:
 if __name__ == "__main__":
     path = build(verbose=True)
     print(f"built {path}")
+    print(f"built {build_attn(verbose=True)}")
     print(f"built {build_probe(verbose=True)}")
     sys.exit(0)
