@@ -16,9 +16,10 @@ projection calls of one decode step, on libkrk_gemm.so.
 * :class:`GemmStep` — the projection data flow of ``run_layers``
   (engine/model.py:181-214): per layer qkv (normed), o, gate/up (normed),
   down, then the normed lm_head; 4 · layers + 1 calls, 145 for Qwen3-4B.
-  Attention, q/k norm, RoPE and the KV cache are not part of this library:
-  the o projection reads a caller-filled ``attn_out`` buffer and the qkv
-  output is not consumed.  The residual stream uses the reference's two
+  With a :class:`kernels.cache.DecodeCache` it runs the whole layer: q/k
+  norm, rotary embedding, cache write and attention between qkv and o.
+  Without one the o projection reads a caller-filled ``attn_out`` buffer and
+  the qkv output is not consumed.  The residual stream uses the reference's two
   buffers (qkv reads ``cur`` and writes ``xa``, gate/up reads ``xa`` and
   writes ``xb``, lm reads ``xb`` and writes ``xa``), and :meth:`capture`
   records the whole step in one graph as the engine's ``capture`` does
@@ -85,11 +86,22 @@ def decode_matmuls(m, M: int, log=None, tune: bool = True, select_k: int | None 
 class GemmStep:
     """The projection calls of one decode step over ``M`` rows (see the
     module docstring).  ``run(x)`` returns the logits ([M, vocab] bf16), or
-    the selected indices ([M, k] int64) when built with ``select_k``."""
+    the selected indices ([M, k] int64) when built with ``select_k``.
+
+    ``cache`` (a :class:`kernels.cache.DecodeCache` of B sequences; M = B · R)
+    adds the attention of the R rows of each sequence, sequence after sequence
+    in x; each run or replay moves the cache on by R rows.  ``tree`` (int64
+    ``[B, R]`` on the GPU, read at every run and replay) makes them a draft
+    tree's nodes."""
 
     def __init__(self, m, M: int, mm: dict | None = None, log=None, tune: bool = False,
-                 select_k: int | None = None):
+                 select_k: int | None = None, cache=None, tree: torch.Tensor | None = None):
         self.m, self.M = m, M
+        if cache is not None and M % cache.B:
+            raise ValueError(f"M={M} rows for a cache of {cache.B} sequences")
+        if tree is not None and cache is None:
+            raise ValueError("tree masks need a cache")
+        self.cache, self.tree = cache, tree
         self.mm = mm if mm is not None else decode_matmuls(m, M, log, tune=tune, select_k=select_k)
         if select_k is not None and "lm_select" not in self.mm:
             raise ValueError("select_k needs an mm dict with an 'lm_select' entry")
@@ -108,11 +120,20 @@ class GemmStep:
         return 4 * len(self.m.layers) + 1
 
     def run(self, x: torch.Tensor) -> torch.Tensor:
-        m, mm = self.m, self.mm
+        if self.cache is not None:
+            self.cache.reserve(self.M // self.cache.B)
+        return self._run(x)
+
+    def _run(self, x: torch.Tensor) -> torch.Tensor:
+        m, mm, cache = self.m, self.mm, self.cache
         xa, xb = self.xa, self.xb
         cur, y = x, self.zero
-        for layer in m.layers:
-            mm["qkv"](cur, y, layer.in_norm, xa, layer.wqkv)
+        if cache is not None:
+            cache.begin(self.M // cache.B, self.tree, reserve=False)
+        for i, layer in enumerate(m.layers):
+            qkv = mm["qkv"](cur, y, layer.in_norm, xa, layer.wqkv)
+            if cache is not None:
+                cache.attend(i, qkv, self.attn_out)
             o = mm["o"](self.attn_out, layer.wo)
             act = mm["gu"](xa, o, layer.post_norm, xb, layer.wgu)
             y = mm["d"](act, layer.wd)
@@ -123,23 +144,33 @@ class GemmStep:
     def capture(self, x: torch.Tensor) -> torch.cuda.CUDAGraph:
         """Record run(x) in one graph (after warm-up calls on a side stream);
         replay() then recomputes self.out from the current contents of x and
-        attn_out."""
+        attn_out, or continues the cache by the rows of x.  A cache is left as
+        it was, but for slots behind its lengths."""
+        state = None
+        if self.cache is not None:
+            state = self.cache._state()
+            self.cache.reserve(self.M // self.cache.B)  # ValueError if a step does not fit
+            self.cache._restore(state)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             for _ in range(2):
-                self.run(x)
+                self._run(x)
+                if state is not None:
+                    self.cache._restore(state)
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            self.out = self.run(x)
+            self.out = self._run(x)
         self.graph = g
         return g
 
     def replay(self) -> torch.Tensor:
         if self.graph is None:
             raise RuntimeError("capture() first")
+        if self.cache is not None:
+            self.cache.reserve(self.M // self.cache.B)
         self.graph.replay()
         return self.out
 
@@ -154,11 +185,13 @@ class QwenConfig:
     head_dim: int = 128
     vocab: int = 151936
     eps: float = 1e-6
+    theta: float = 1e6
 
 
 def synthetic_model(device, layers: int | None = None, seed: int = 0, scale: float = 0.02, **cfg_overrides):
     """A Qwen3-4B-shaped model object with seeded N(0, scale) bf16 weights and
-    N(1, 0.1) norm gains (real checkpoints are not loaded by this library)."""
+    N(1, 0.1) norm gains (real checkpoints are not loaded by this library).
+    The q/k gains come from a generator of their own."""
     cfg = QwenConfig(**cfg_overrides)
     if layers is not None:
         cfg.layers = layers
@@ -177,5 +210,9 @@ def synthetic_model(device, layers: int | None = None, seed: int = 0, scale: flo
                           wo=w(cfg.hidden, cfg.heads * cfg.head_dim), post_norm=gain(cfg.hidden),
                           wgu=w(2 * cfg.intermediate, cfg.hidden), wd=w(cfg.hidden, cfg.intermediate))
           for _ in range(cfg.layers)]
-    return SimpleNamespace(cfg=cfg, device=dev, layers=Ls, lm_head=w(cfg.vocab, cfg.hidden),
-                           final_norm=gain(cfg.hidden))
+    m = SimpleNamespace(cfg=cfg, device=dev, layers=Ls, lm_head=w(cfg.vocab, cfg.hidden), final_norm=gain(cfg.hidden))
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed + 0x51)
+    for l in Ls:
+        l.q_norm, l.k_norm = gain(cfg.head_dim), gain(cfg.head_dim)
+    return m
