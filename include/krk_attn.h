@@ -86,8 +86,8 @@ typedef struct krk_attn_shape {
  * Padding rows, and rows that see nothing, give zeros in out and -infinity in
  * lse.  Keys that a row does not see have no part in its result, whatever they
  * hold (NaN and infinities too).  Sums, maxima and weights are held in 32
- * bits; the weights are rounded to bf16 for the products with v where R * G
- * is large (krk_attn_plan tells), else carried in two bf16 parts.
+ * bits; the weights enter the products with v rounded to bf16 where 128
+ * rows or more share a workgroup (krk_attn_plan tells), else as two bf16 parts.
  */
 typedef struct krk_attn_args {
     const void* q;     /* [B * R, heads * head_dim], row stride q_row (multiple of 8) */
@@ -120,10 +120,12 @@ size_t krk_attn_workspace_bytes(const krk_attn_shape* shape);
 /* KRK_ATTN_OK, or the error that krk_attn_bf16 would report for this shape. */
 int krk_attn_check(const krk_attn_shape* shape);
 
-/* How the work is cut for this shape. */
+/* How the work is cut for this shape.  Rows are pairs of a new row and a query
+ * head of one key/value head.  Up to 64 of them (16 or 32 per workgroup) run on
+ * a kernel whose waves divide the keys, more (128 or 256 per workgroup) on one
+ * whose waves divide the rows and which rounds the weights to bf16. */
 typedef struct krk_attn_plan_t {
-    int kernel;         /* 0: key ranges split over workgroups and joined; 1: one workgroup per tile of rows */
-    int rows;           /* row and query-head pairs of a key/value head in a tile */
+    int rows;           /* of a workgroup: 16, 32, 128, 256 */
     int splits;         /* key ranges of a sequence's own cache */
     int prefix_rows;    /* the same for the prefix (0 without one) */
     int prefix_splits;

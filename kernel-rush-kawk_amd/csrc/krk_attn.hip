@@ -11,6 +11,7 @@
 
 #include "krk_attn.h"
 #include "krk_attn_split.h"
+#include "krk_attn_tile.h"
 #include "krk_evict.h"
 #include "krk_rope.h"
 
@@ -127,43 +128,44 @@ int check_shape(const krk_attn_shape& s) {
 }
 
 // -------------------------------------------------------------------- plan
+// Rows of a workgroup: 16 or 32 on the split kernel (its waves share the rows
+// and divide the keys), 128 or 256 on the tile kernel (the other way round).
+struct Cut {
+    int rows, tiles, splits;
+};
+
 struct Plan {
-    int mt, prefix_mt;  // 16-row tiles of a workgroup
-    int row_tiles, prefix_row_tiles, splits, prefix_splits;
+    Cut own, prefix;
     int64_t all_rows;
     size_t part, ml, stat, bytes;  // workspace: sizes of its parts and their sum
 };
 
-int tiles_of(int64_t rows) { return rows <= 16 ? 1 : 2; }
-
-// Key ranges for `blocks` workgroups and `keys` keys: enough workgroups for
-// the chip (two per CU where 16 rows leave the registers for it), but a step
-// of 32 keys for every wave at least.
-int splits_of(int64_t blocks, int mt, int64_t keys) {
-    const int64_t want = cdiv(kCuCount * (mt == 1 ? 2 : 1), blocks);
-    const int64_t most = cdiv(keys, 32 * krk::kSplitWaves);
-    return (int)(want < most ? want : most);
+// `lists` row lists of `rows` rows each, over at most `keys` keys.  Key ranges:
+// enough workgroups for the chip (two per CU where 16 rows leave the registers
+// for it), but a step for every wave of the split kernel and four steps of the
+// tile kernel at least.
+Cut make_cut(int64_t rows, int64_t lists, int64_t keys) {
+    Cut c;
+    c.rows = rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
+    c.tiles = (int)cdiv(rows, c.rows);
+    const int64_t want = cdiv(kCuCount * (c.rows == 16 ? 2 : 1), lists * c.tiles);
+    const int64_t most = cdiv(keys, c.rows < 128 ? 32 * krk::kSplitWaves : 4 * krk::kTileStep);
+    c.splits = (int)(want < most ? want : most);
+    return c;
 }
 
 Plan make_plan(const krk_attn_shape& s) {
     Plan p{};
     const int64_t RG = (int64_t)s.R * (s.heads / s.kv_heads);
     p.all_rows = RG * s.B * s.kv_heads;
-    p.mt = tiles_of(RG);
-    p.row_tiles = (int)cdiv(RG, 16 * p.mt);
     int64_t keys = s.capacity;
     if (s.window) {
         const int64_t near = (int64_t)s.window + s.sinks + s.R + 64;
         keys = near < keys ? near : keys;
     }
-    p.splits = splits_of((int64_t)s.B * s.kv_heads * p.row_tiles, p.mt, keys);
-    p.prefix_mt = 1;
-    if (s.prefix) {
-        p.prefix_mt = tiles_of(RG * s.B);
-        p.prefix_row_tiles = (int)cdiv(RG * s.B, 16 * p.prefix_mt);
-        p.prefix_splits = splits_of((int64_t)s.kv_heads * p.prefix_row_tiles, p.prefix_mt, s.prefix);
-    }
-    const int n = p.splits + p.prefix_splits;
+    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys);
+    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix);
+    const int n = p.own.splits + p.prefix.splits;
     if (n > 1) {
         p.part = align_up((size_t)n * p.all_rows * s.head_dim * sizeof(float), 256);
         p.ml = align_up((size_t)n * p.all_rows * sizeof(float2), 256);
@@ -184,23 +186,38 @@ int launch_split(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
     return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(krk::kSplitThreads), args, shm, stream), "attn_split_kernel launch");
 }
 
+template <int D, int W>
+int launch_tile(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    const void* fn = reinterpret_cast<const void*>(&krk::attn_tile_kernel<D, W>);
+    const size_t shm = krk::tile_lds_bytes<D>();
+    if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "attn_tile_kernel LDS size");
+    void* args[] = {(void*)&p};
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(64 * W), args, shm, stream), "attn_tile_kernel launch");
+}
+
 template <int D>
-int launch_split_mt(const krk::AttnParams& p, int mt, int64_t blocks, hipStream_t stream) {
-    return mt == 1 ? launch_split<D, 1>(p, blocks, stream) : launch_split<D, 2>(p, blocks, stream);
+int launch_rows(const krk::AttnParams& p, int rows, int64_t blocks, hipStream_t stream) {
+    switch (rows) {
+        case 16: return launch_split<D, 1>(p, blocks, stream);
+        case 32: return launch_split<D, 2>(p, blocks, stream);
+        case 128: return launch_tile<D, 4>(p, blocks, stream);
+        default: return launch_tile<D, 8>(p, blocks, stream);
+    }
 }
 
 template <int D>
 int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
-    if (plan.prefix_splits) {
-        const int64_t blocks = (int64_t)plan.prefix_row_tiles * p.kv_heads * plan.prefix_splits;
-        if (int rc = launch_split_mt<D>(p, plan.prefix_mt, blocks, stream)) return rc;
+    if (plan.prefix.splits) {
+        const int64_t blocks = (int64_t)plan.prefix.tiles * p.kv_heads * plan.prefix.splits;
+        if (int rc = launch_rows<D>(p, plan.prefix.rows, blocks, stream)) return rc;
     }
     krk::AttnParams o = p;
     o.prefix_row_tiles = 0;
-    const int64_t blocks = (int64_t)plan.row_tiles * p.kv_heads * p.B * plan.splits;
-    if (int rc = launch_split_mt<D>(o, plan.mt, blocks, stream)) return rc;
+    const int64_t blocks = (int64_t)plan.own.tiles * p.kv_heads * p.B * plan.own.splits;
+    if (int rc = launch_rows<D>(o, plan.own.rows, blocks, stream)) return rc;
     void* args[] = {(void*)&p};
-    if (plan.splits + plan.prefix_splits > 1) {
+    if (plan.own.splits + plan.prefix.splits > 1) {
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_join_kernel<D>),
                                              dim3((unsigned)cdiv(plan.all_rows, 4)), dim3(256), args, 0, stream);
         if (int rc = hip_status(e, "attn_join_kernel launch")) return rc;
@@ -251,7 +268,7 @@ int krk_attn_plan(const krk_attn_shape* shape, krk_attn_plan_t* out) {
     if (!shape || !out) return fail(KRK_ATTN_ERR_INVALID, "null argument");
     if (int rc = check_shape(*shape)) return rc;
     const Plan p = make_plan(*shape);
-    *out = krk_attn_plan_t{0, 16 * p.mt, p.splits, shape->prefix ? 16 * p.prefix_mt : 0, p.prefix_splits};
+    *out = krk_attn_plan_t{p.own.rows, p.own.splits, p.prefix.rows, p.prefix.splits};
     return KRK_ATTN_OK;
 }
 
@@ -342,10 +359,10 @@ int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* 
     p.window = s.window;
     p.sinks = s.sinks;
     p.prefix = a.prefix;
-    p.splits = plan.splits;
-    p.prefix_splits = plan.prefix_splits;
-    p.row_tiles = plan.row_tiles;
-    p.prefix_row_tiles = plan.prefix_row_tiles;
+    p.splits = plan.own.splits;
+    p.prefix_splits = plan.prefix.splits;
+    p.row_tiles = plan.own.tiles;
+    p.prefix_row_tiles = plan.prefix.tiles;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return s.head_dim == 128 ? launch_attn<128>(p, plan, st) : launch_attn<64>(p, plan, st);
 }

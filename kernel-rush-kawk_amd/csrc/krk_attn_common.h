@@ -89,12 +89,9 @@ __device__ __forceinline__ RowSight row_sight(const AttnParams& p, int b, int r,
 }
 
 __device__ __forceinline__ bool sees(const RowSight& s, int t, int sinks) {
-    bool ok = t <= s.hi && (t >= s.lo || t < sinks);
-    if (s.bits) {
-        const unsigned d = (unsigned)(t - s.first);
-        ok = ok || (d < 64 && ((s.bits >> d) & 1));
-    }
-    return ok;
+    const unsigned d = (unsigned)(t - s.first);
+    const bool node = d < 64 && ((s.bits >> (d & 63)) & 1);
+    return (t <= s.hi && (t >= s.lo || t < sinks)) || node;
 }
 
 // Wait until every load this wave issued has returned.
@@ -105,6 +102,132 @@ __device__ __forceinline__ void drain_loads() {
 }
 
 __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// A workgroup's share: TR rows of a key/value head against one range of the
+// keys of a run (a sequence's own cache, or the shared prefix).
+struct Task {
+    bool shared;
+    int h, b0;          // head; sequence (own cache)
+    int rows, row0;     // rows of the run's row list, and the task's first
+    int sp, nsp, part;  // key range, of how many, and its place among the partial results
+    int seg, limit;     // position of the run's first key; its keys
+    const uint16_t *k, *v;
+    int64_t k_slot, v_slot;
+};
+
+// Heads change fastest: with 8 heads each XCD (workgroups go to them round
+// robin) keeps to one head's keys.  Later row tiles, which see more keys, go
+// first.
+template <int TR>
+__device__ __forceinline__ Task task_of(const AttnParams& p, int id) {
+    Task t;
+    const int nprefix = p.prefix_row_tiles * p.kv_heads * p.prefix_splits;
+    t.shared = id < nprefix;
+    if (!t.shared) id -= nprefix;
+    t.h = id % p.kv_heads;
+    id /= p.kv_heads;
+    t.b0 = 0;
+    int tile;
+    if (t.shared) {
+        tile = id % p.prefix_row_tiles;
+        t.sp = id / p.prefix_row_tiles;
+        t.nsp = p.prefix_splits;
+        t.part = p.splits + t.sp;
+        t.rows = p.B * p.RG;
+        t.seg = 0;
+        t.limit = p.prefix;
+    } else {
+        tile = p.row_tiles - 1 - id % p.row_tiles;
+        id /= p.row_tiles;
+        t.b0 = id % p.B;
+        t.sp = id / p.B;
+        t.nsp = p.splits;
+        t.part = t.sp;
+        t.rows = p.RG;
+        t.seg = p.prefix;
+        t.limit = seq_len(p, t.b0);
+    }
+    t.row0 = tile * TR;
+    const CacheView& k = t.shared ? p.kp : p.k;
+    const CacheView& v = t.shared ? p.vp : p.v;
+    t.k = k.p + (t.shared ? 0 : (int64_t)t.b0 * k.seq) + (int64_t)t.h * k.head;
+    t.v = v.p + (t.shared ? 0 : (int64_t)t.b0 * v.seq) + (int64_t)t.h * v.head;
+    t.k_slot = k.slot;
+    t.v_slot = v.slot;
+    return t;
+}
+
+// Row `row` of a task's list (the last one again behind its end): what it
+// sees, and where its q is.
+struct TaskRow {
+    int b, r, head;
+    RowSight sight;
+};
+__device__ __forceinline__ TaskRow task_row(const AttnParams& p, const Task& t, int row) {
+    TaskRow x;
+    const int j = row < t.rows ? row : t.rows - 1;
+    x.b = t.shared ? j / p.RG : t.b0;
+    const int jj = t.shared ? j - x.b * p.RG : j;
+    x.r = jj / p.G;
+    x.head = t.h * p.G + (jj - x.r * p.G);
+    x.sight = row_sight(p, x.b, x.r, t.shared ? seq_len(p, x.b) : t.limit);
+    return x;
+}
+
+// What a set of rows sees at most (lo_min .. hi_max) and all of them see (from
+// lo_max to hi_min), over the lanes of a wave.
+struct Reach {
+    int lo_min = 0x7fffffff, hi_max = -1, lo_max = 0, hi_min = 0x7fffffff;
+    __device__ __forceinline__ void add(const RowSight& s, bool live) {
+        if (live && s.lo != kPadding) {
+            const int hi = s.bits ? s.first + 63 : s.hi;
+            lo_min = s.lo < lo_min ? s.lo : lo_min;
+            lo_max = s.lo > lo_max ? s.lo : lo_max;
+            hi_max = hi > hi_max ? hi : hi_max;
+            hi_min = s.hi < hi_min ? s.hi : hi_min;
+        }
+    }
+    __device__ __forceinline__ void join_lanes() {
+        lo_min = wave_min_i(lo_min);
+        lo_max = -wave_min_i(-lo_max);
+        hi_max = -wave_min_i(-hi_max);
+        hi_min = wave_min_i(hi_min);
+    }
+    __device__ static __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int o = __shfl_xor(v, s);
+            v = o < v ? o : v;
+        }
+        return __builtin_amdgcn_readfirstlane(v);
+    }
+};
+
+// A task's keys in steps of STEP: those that hold sinks, then from the first
+// key that some row's window holds to the last that some row sees.  The task
+// takes steps t0 .. t1 - 1.
+template <int STEP>
+struct KeySteps {
+    int from, sink_steps, t0, t1;
+    __device__ __forceinline__ KeySteps(const AttnParams& p, const Task& t, const Reach& r) {
+        int end = r.hi_max + 1 - t.seg;
+        end = end < t.limit ? end : t.limit;
+        end = end > 0 ? end : 0;
+        from = r.lo_min - t.seg;
+        from = from > 0 ? (from < end ? from & ~(STEP - 1) : end) : 0;
+        int nsink = p.sinks - t.seg;
+        nsink = nsink > 0 ? (nsink < end ? nsink : end) : 0;
+        sink_steps = (nsink + STEP - 1) / STEP;
+        if (STEP * sink_steps >= from) {
+            from = 0;
+            sink_steps = 0;
+        }
+        const int steps = sink_steps + (end > from ? (end - from + STEP - 1) / STEP : 0);
+        t0 = (int)((int64_t)steps * t.sp / t.nsp);
+        t1 = (int)((int64_t)steps * (t.sp + 1) / t.nsp);
+    }
+    __device__ __forceinline__ int key(int t) const { return t < sink_steps ? STEP * t : from + STEP * (t - sink_steps); }
+};
 
 // Maximum / sum over the four lanes n, n + 16, n + 32, n + 48 that hold a row.
 __device__ __forceinline__ float row_max(float v) {
@@ -119,23 +242,6 @@ __device__ __forceinline__ float row_sum(float v) {
     const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-__device__ __forceinline__ int row_min_i(int v) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int o = __shfl_xor(v, s);
-        v = o < v ? o : v;
-    }
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int row_max_i(int v) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const int o = __shfl_xor(v, s);
-        v = o > v ? o : v;
-    }
-    return __builtin_amdgcn_readfirstlane(v);
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     bf16x2 v;
     v[0] = (__bf16)lo;
@@ -220,51 +326,62 @@ __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// Eight bf16 values with zeros for infinities and NaNs.
+__device__ __forceinline__ u32x4 finite_bf16x8(const u32x4& x) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = x[i];
+        r[i] = ((w & 0x7f80u) != 0x7f80u ? w & 0xffffu : 0u) | ((w & 0x7f800000u) != 0x7f800000u ? w & 0xffff0000u : 0u);
+    }
+    return r;
+}
+// Marks for the infinities and NaNs among them, in bf16: 1 for +infinity, 2^7
+// for -infinity, 2^14 for NaN.  A sum of up to 64 of each says which there are.
+__device__ __forceinline__ uint32_t odd_mark(uint32_t e) {
+    const uint32_t m = e == 0x7f80u ? 0x3f80u : e == 0xff80u ? 0x4300u : 0x4680u;
+    return (e & 0x7f80u) == 0x7f80u ? m : 0u;
+}
+__device__ __forceinline__ u32x4 odd_marks(const u32x4& x) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = x[i];
+        r[i] = odd_mark(w & 0xffffu) | odd_mark(w >> 16) << 16;
+    }
+    return r;
+}
+__device__ __forceinline__ float odd_value(float n) {
+    const uint32_t c = (uint32_t)n;
+    const float inf = __builtin_inff();
+    float v = (c & 0x7fu) ? inf : 0.0f;
+    v = (c >> 7) & 0x7fu ? v - inf : v;  // both signs: NaN
+    return c >> 14 ? __builtin_nanf("") : v;
+}
+
 // O^T += V^T P^T where values among the 32 keys are infinite or NaN; bit i of
 // vis says that the lane's row sees key 8q + i.  A zero weight times an infinity
 // would reach rows that do not see it, so the products run on the finite values
-// alone, and a count of the visible infinities and NaNs of each output (a
-// product of zeros and ones) adds them.
+// alone, and a count of the visible infinities and NaNs of each output (their
+// marks against zeros and ones) adds them.
 template <int D, int MT>
 __device__ __forceinline__ void add_odd_values(f32x4 (&acc)[MT][D / 16], const ValueFrag<D>& v, const bf16x8 (&hi)[MT],
                                                const bf16x8 (&lo)[MT], const uint32_t (&vis)[MT]) {
-    const float special[3] = {__builtin_inff(), -__builtin_inff(), __builtin_nanf("")};
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
         const u32x4 x = __builtin_bit_cast(u32x4, v.operand(j));
-        u32x4 fin, kind[3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t keep = 0, k0 = 0, k1 = 0, k2 = 0;
-#pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-                const uint32_t e = (x[i] >> h) & 0xffffu;
-                const uint32_t one = 0x3f80u << h;
-                const bool f = (e & 0x7f80u) != 0x7f80u;
-                keep |= f ? e << h : 0u;
-                k0 |= e == 0x7f80u ? one : 0u;
-                k1 |= e == 0xff80u ? one : 0u;
-                k2 |= !f && (e & 0x7fu) ? one : 0u;
-            }
-            fin[i] = keep;
-            kind[0][i] = k0;
-            kind[1][i] = k1;
-            kind[2][i] = k2;
-        }
+        const bf16x8 a = __builtin_bit_cast(bf16x8, finite_bf16x8(x));
+        const u32x4 marks = odd_marks(x);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             u32x4 ones;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                ones[e] = ((vis[i] >> (2 * e)) & 1 ? 0x3f80u : 0u) | ((vis[i] >> (2 * e + 1)) & 1 ? 0x3f800000u : 0u);
-            const bf16x8 a = __builtin_bit_cast(bf16x8, fin);
+                ones[e] = ((vis[i] >> (2 * e)) & 1) * 0x3f80u | ((vis[i] >> (2 * e + 1)) & 1) * 0x3f800000u;
             acc[i][j] = mfma16(a, hi[i], mfma16(a, lo[i], acc[i][j]));
+            const f32x4 n = mfma16(marks, ones, f32x4{0, 0, 0, 0});
 #pragma unroll
-            for (int s = 0; s < 3; ++s) {
-                const f32x4 n = mfma16(kind[s], ones, f32x4{0, 0, 0, 0});
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] += n[e] > 0.0f ? special[s] : 0.0f;
-            }
+            for (int e = 0; e < 4; ++e) acc[i][j][e] += odd_value(n[e]);
             __builtin_amdgcn_sched_barrier(0);  // one tile's temporaries at a time
         }
     }

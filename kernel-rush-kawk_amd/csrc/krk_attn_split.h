@@ -42,83 +42,25 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
 
-    // Which rows, which keys.
-    int id = blockIdx.x;
-    const int nprefix = p.prefix_row_tiles * p.kv_heads * p.prefix_splits;
-    const bool shared = id < nprefix;
-    if (!shared) id -= nprefix;
-    const int h = id % p.kv_heads;
-    id /= p.kv_heads;
-    int b0 = 0, tile, sp, nsp, part;
-    if (shared) {
-        tile = id % p.prefix_row_tiles;
-        sp = id / p.prefix_row_tiles;
-        nsp = p.prefix_splits;
-        part = p.splits + sp;
-    } else {
-        tile = id % p.row_tiles;
-        id /= p.row_tiles;
-        b0 = id % p.B;
-        sp = id / p.B;
-        nsp = p.splits;
-        part = sp;
-    }
-    const int rows = shared ? p.B * p.RG : p.RG;
-    const int row0 = tile * TR;
-    const int seg = shared ? 0 : p.prefix;  // position of the run's first key
-    const int limit = shared ? p.prefix : seq_len(p, b0);
-    const CacheView& kc = shared ? p.kp : p.k;
-    const CacheView& vc = shared ? p.vp : p.v;
-    const uint16_t* kbase = kc.p + (int64_t)b0 * (shared ? 0 : kc.seq) + (int64_t)h * kc.head;
-    const uint16_t* vbase = vc.p + (int64_t)b0 * (shared ? 0 : vc.seq) + (int64_t)h * vc.head;
+    const Task task = task_of<TR>(p, blockIdx.x);
+    const int limit = task.limit;
 
     // This lane's rows: what they see, and their q.
     RowSight sight[MT];
     u32x4 qf[MT][KS];
-    int lo_min = 0x7fffffff, hi_max = -1, lo_max = 0, hi_min = 0x7fffffff;
+    Reach reach;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int row = row0 + 16 * i + n16;
-        const int j = row < rows ? row : rows - 1;
-        const int b = shared ? j / p.RG : b0;
-        const int jj = shared ? j - b * p.RG : j;
-        const int r = jj / p.G;
-        sight[i] = row_sight(p, b, r, shared ? seq_len(p, b) : limit);
-        const bool live = row < rows && sight[i].lo != kPadding;
-        if (live) {
-            const int hi = sight[i].bits ? sight[i].first + 63 : sight[i].hi;
-            lo_min = sight[i].lo < lo_min ? sight[i].lo : lo_min;
-            lo_max = sight[i].lo > lo_max ? sight[i].lo : lo_max;
-            hi_max = hi > hi_max ? hi : hi_max;
-            hi_min = sight[i].hi < hi_min ? sight[i].hi : hi_min;
-        }
-        const uint16_t* qr = p.q + ((int64_t)b * p.R + r) * p.q_row + (int64_t)(h * p.G + (jj - r * p.G)) * D + 8 * q4;
+        const int row = task.row0 + 16 * i + n16;
+        const TaskRow x = task_row(p, task, row);
+        sight[i] = x.sight;
+        reach.add(x.sight, row < task.rows);
+        const uint16_t* qr = p.q + ((int64_t)x.b * p.R + x.r) * p.q_row + (int64_t)x.head * D + 8 * q4;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[i][s] = load_cached16(qr + 32 * s);
     }
-    lo_min = row_min_i(lo_min);
-    lo_max = row_max_i(lo_max);
-    hi_max = row_max_i(hi_max);
-    hi_min = row_min_i(hi_min);
-
-    // The run's keys that some row sees, in steps of 32: those below the sinks'
-    // end, then from the window's first key on.
-    int end = hi_max + 1 - seg;
-    end = end < limit ? end : limit;
-    end = end > 0 ? end : 0;
-    int from = lo_min - seg;
-    from = from > 0 ? (from < end ? from & ~31 : end) : 0;
-    int nsink = p.sinks - seg;
-    nsink = nsink > 0 ? (nsink < end ? nsink : end) : 0;
-    int sink_steps = (nsink + 31) >> 5;
-    if (32 * sink_steps >= from) {
-        from = 0;
-        sink_steps = 0;
-    }
-    const int steps = sink_steps + (end > from ? (end - from + 31) >> 5 : 0);
-    const int t0 = (int)((int64_t)steps * sp / nsp);
-    const int t1 = (int)((int64_t)steps * (sp + 1) / nsp);
-    auto step_key = [&](int t) { return t < sink_steps ? 32 * t : from + 32 * (t - sink_steps); };
+    reach.join_lanes();
+    const KeySteps<32> steps(p, task, reach);
 
     f32x4 acc[MT][VD];
     float m[MT], l[MT];
@@ -132,13 +74,14 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
 
     KeyFrag<D> kf;
     ValueFrag<D> vf;
-    int t = t0 + wave;
+    const int t1 = steps.t1;
+    int t = steps.t0 + wave;
     if (t < t1) {
-        kf.load(kbase, kc.slot, step_key(t), limit, lane);
-        vf.load(vbase, vc.slot, step_key(t), limit, lane);
+        kf.load(task.k, task.k_slot, steps.key(t), limit, lane);
+        vf.load(task.v, task.v_slot, steps.key(t), limit, lane);
     }
     for (; t < t1; t += kSplitWaves) {
-        const int kb = step_key(t);
+        const int kb = steps.key(t);
         const int next = t + kSplitWaves;
         f32x4 s[MT][2];
 #pragma unroll
@@ -149,12 +92,12 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) s[i][u] = mfma16(kf.f[u][ks], qf[i][ks], s[i][u]);
             }
-        if (next < t1) kf.load(kbase, kc.slot, step_key(next), limit, lane);
+        if (next < t1) kf.load(task.k, task.k_slot, steps.key(next), limit, lane);
 
         // What each row does not see gets no weight.  Steps that every row
         // sees whole skip this.
-        const int pos = seg + kb;
-        const bool whole = kb + 32 <= limit && pos + 31 <= hi_min && (pos >= lo_max || pos + 32 <= p.sinks);
+        const int pos = task.seg + kb;
+        const bool whole = kb + 32 <= limit && pos + 31 <= reach.hi_min && (pos >= reach.lo_max || pos + 32 <= p.sinks);
         uint32_t vis[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) vis[i] = 0xff;
@@ -165,7 +108,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = kb + 8 * q4 + e;
-                    const bool ok = key < limit && sees(sight[i], seg + key, p.sinks);
+                    const bool ok = key < limit && sees(sight[i], task.seg + key, p.sinks);
                     vis[i] |= ok ? 1u << e : 0u;
                     s[i][e >> 2][e & 3] = ok ? s[i][e >> 2][e & 3] : kNegInf;
                 }
@@ -212,7 +155,7 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
                 for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, lo[i], acc[i][j]));
             }
         }
-        if (next < t1) vf.load(vbase, vc.slot, step_key(next), limit, lane);
+        if (next < t1) vf.load(task.v, task.v_slot, steps.key(next), limit, lane);
     }
 
     // The waves meet: O as [wave][row][D + 4] (rows 4 banks apart), maxima and
@@ -244,8 +187,8 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
     constexpr int PER_ROW = D / 4;
     for (int e = threadIdx.x; e < TR * PER_ROW; e += kSplitThreads) {
         const int n = e / PER_ROW, d = 4 * (e % PER_ROW);
-        const int row = row0 + n;
-        if (row >= rows) break;  // rows grow with e
+        const int row = task.row0 + n;
+        if (row >= task.rows) break;  // rows grow with e
         float mw[kSplitWaves], M = kNegInf, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kSplitWaves; ++w) {
@@ -260,12 +203,12 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
             L += f * lo_ml[w * TR + n].y;
             o += f * *reinterpret_cast<const f32x4*>(lo_o + ((size_t)w * TR + n) * LD + d);
         }
-        const int b = shared ? row / p.RG : b0;
-        const int j = shared ? row - b * p.RG : row;
-        const int64_t g = ((int64_t)b * p.kv_heads + h) * p.RG + j;
+        const int b = task.shared ? row / p.RG : task.b0;
+        const int j = task.shared ? row - b * p.RG : row;
+        const int64_t g = ((int64_t)b * p.kv_heads + task.h) * p.RG + j;
         if (last) {
             const int r = j / p.G;
-            const int head = h * p.G + (j - r * p.G);
+            const int head = task.h * p.G + (j - r * p.G);
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             if (L == 0.0f) o = f32x4{0, 0, 0, 0};
             const int64_t at = (int64_t)b * p.R + r;
@@ -276,8 +219,8 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
                 if (p.stat) p.stat[g] = make_float2(ms, inv);
             }
         } else {
-            *reinterpret_cast<f32x4*>(p.part + ((int64_t)part * all_rows + g) * D + d) = o;
-            if (d == 0) p.ml[(int64_t)part * all_rows + g] = make_float2(M, L);
+            *reinterpret_cast<f32x4*>(p.part + ((int64_t)task.part * all_rows + g) * D + d) = o;
+            if (d == 0) p.ml[(int64_t)task.part * all_rows + g] = make_float2(M, L);
         }
     }
 }

@@ -68,7 +68,7 @@ class EvictArgs(ctypes.Structure):
 class AttnPlan(ctypes.Structure):
     """``krk_attn_plan_t``."""
 
-    _fields_ = [(n, _int) for n in ("kernel", "rows", "splits", "prefix_rows", "prefix_splits")]
+    _fields_ = [(n, _int) for n in ("rows", "splits", "prefix_rows", "prefix_splits")]
 
     def as_dict(self) -> dict:
         return {name: getattr(self, name) for name, _ in self._fields_}
