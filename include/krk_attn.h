@@ -87,7 +87,7 @@ typedef struct krk_attn_shape {
  * lse.  Keys that a row does not see have no part in its result, whatever they
  * hold (NaN and infinities too).  Sums, maxima and weights are held in 32
  * bits; the weights enter the products with v rounded to bf16 where 128
- * rows or more share a workgroup (krk_attn_plan tells), else as two bf16 parts.
+ * rows share a workgroup (krk_attn_plan tells), else as two bf16 parts.
  */
 typedef struct krk_attn_args {
     const void* q;     /* [B * R, heads * head_dim], row stride q_row (multiple of 8) */
@@ -109,8 +109,11 @@ typedef struct krk_attn_args {
 } krk_attn_args;
 
 /* One call.  `workspace`: krk_attn_workspace_bytes(shape) bytes, 16-byte
- * aligned, its contents of no matter (may be NULL when that is 0).  Calls that
- * share a workspace must be ordered on one stream.  Results are deterministic. */
+ * aligned (may be NULL when that is 0).  It must be zero-filled once before its
+ * first use; every call leaves its counters, at the start, zero again and
+ * partial results behind them.  Calls that share one workspace must be ordered
+ * on one stream; for another shape it is zero-filled again first.  Results are
+ * deterministic. */
 int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* workspace, size_t workspace_bytes,
                   void* stream);
 
@@ -122,10 +125,10 @@ int krk_attn_check(const krk_attn_shape* shape);
 
 /* How the work is cut for this shape.  Rows are pairs of a new row and a query
  * head of one key/value head.  Up to 64 of them (16 or 32 per workgroup) run on
- * a kernel whose waves divide the keys, more (128 or 256 per workgroup) on one
- * whose waves divide the rows and which rounds the weights to bf16. */
+ * a kernel whose waves divide the keys, more (128 per workgroup) on one whose
+ * waves divide the rows and which rounds the weights to bf16. */
 typedef struct krk_attn_plan_t {
-    int rows;           /* of a workgroup: 16, 32, 128, 256 */
+    int rows;           /* of a workgroup: 16, 32 or 128 */
     int splits;         /* key ranges of a sequence's own cache */
     int prefix_rows;    /* the same for the prefix (0 without one) */
     int prefix_splits;

@@ -81,7 +81,9 @@ int check_cache(const char* name, krk_cache& c, int64_t seqs, int64_t slots, int
     return KRK_ATTN_OK;
 }
 
-int check_rows(const char* name, const void* p, int64_t row, int64_t rows, int64_t cols, Span* out) {
+// [rows, cols] operand; one row's stride is of no matter and set to its length.
+int check_rows(const char* name, const void* p, int64_t& row, int64_t rows, int64_t cols, Span* out) {
+    if (rows == 1) row = cols;
     if (!p) return fail(KRK_ATTN_ERR_INVALID, "%s: null pointer", name);
     if (row < cols || row > kMaxStride) return fail(KRK_ATTN_ERR_INVALID, "%s: row stride %lld must be >= %lld", name, (long long)row, (long long)cols);
     if (row % 8) return fail(KRK_ATTN_ERR_ALIGN, "%s: the row stride must be a multiple of 8 elements", name);
@@ -129,7 +131,7 @@ int check_shape(const krk_attn_shape& s) {
 
 // -------------------------------------------------------------------- plan
 // Rows of a workgroup: 16 or 32 on the split kernel (its waves share the rows
-// and divide the keys), 128 or 256 on the tile kernel (the other way round).
+// and divide the keys), 128 on the tile kernel (the other way round).
 struct Cut {
     int rows, tiles, splits;
 };
@@ -137,19 +139,25 @@ struct Cut {
 struct Plan {
     Cut own, prefix;
     int64_t all_rows;
-    size_t part, ml, stat, bytes;  // workspace: sizes of its parts and their sum
+    bool join_in_kernel;
+    bool keep_raw;  // scored: q.k goes through the workspace instead of K being read again
+    int64_t raw_row;
+    size_t ctr, part, ml, stat, raw, bytes;  // workspace: sizes of its parts and their sum
 };
 
 // `lists` row lists of `rows` rows each, over at most `keys` keys.  Key ranges:
-// enough workgroups for the chip (two per CU where 16 rows leave the registers
-// for it), but a step for every wave of the split kernel and four steps of the
-// tile kernel at least.
-Cut make_cut(int64_t rows, int64_t lists, int64_t keys) {
+// one workgroup per CU, which is enough to draw 6 TB/s (32 sequences with
+// windows of 4096 keys: 89 us in one range, 96 in two, 101 in six); two where
+// sequences may differ in length (`ragged`) or several tiles of rows share their
+// keys and the matrix pipe is what counts.  But a step for every wave of the
+// split kernel and four steps of the tile kernel at least.
+Cut make_cut(int64_t rows, int64_t lists, int64_t keys, bool ragged) {
     Cut c;
-    c.rows = rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
+    c.rows = rows <= 16 ? 16 : rows <= 64 ? 32 : krk::kTileRows;
     c.tiles = (int)cdiv(rows, c.rows);
-    const int64_t want = cdiv(kCuCount * (c.rows == 16 ? 2 : 1), lists * c.tiles);
-    const int64_t most = cdiv(keys, c.rows < 128 ? 32 * krk::kSplitWaves : 4 * krk::kTileStep);
+    const bool two = c.rows == 16 ? ragged : c.rows == krk::kTileRows && c.tiles > 1;
+    const int64_t want = cdiv(kCuCount * (two ? 2 : 1), lists * c.tiles);
+    const int64_t most = cdiv(keys, c.rows <= 32 ? 32 * krk::kSplitWaves : 4 * krk::kTileStep);
     c.splits = (int)(want < most ? want : most);
     return c;
 }
@@ -163,66 +171,82 @@ Plan make_plan(const krk_attn_shape& s) {
         const int64_t near = (int64_t)s.window + s.sinks + s.R + 64;
         keys = near < keys ? near : keys;
     }
-    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys);
-    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix);
+    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, keys == s.capacity);
+    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, false);
     const int n = p.own.splits + p.prefix.splits;
     if (n > 1) {
+        // One workgroup joins a sequence's head: up to 96 KB of partial results.
+        p.join_in_kernel = p.own.rows <= 32 && p.prefix.rows <= 32 && RG * n * s.head_dim <= 24 << 10;
+        if (p.join_in_kernel) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
         p.part = align_up((size_t)n * p.all_rows * s.head_dim * sizeof(float), 256);
         p.ml = align_up((size_t)n * p.all_rows * sizeof(float2), 256);
     }
-    if (s.scored) p.stat = align_up((size_t)p.all_rows * sizeof(float2), 256);
-    p.bytes = p.part + p.ml + p.stat;
+    if (s.scored) {
+        p.stat = align_up((size_t)p.all_rows * sizeof(float2), 256);
+        p.keep_raw = p.own.rows == 16 && s.window == 0;
+        p.raw_row = (int64_t)align_up((size_t)s.capacity, 32);
+        if (p.keep_raw) p.raw = align_up((size_t)p.all_rows * p.raw_row * sizeof(float), 256);
+    }
+    p.bytes = p.ctr + p.part + p.ml + p.stat + p.raw;
     return p;
 }
 
 // ---------------------------------------------------------------- launches
-template <int D, int MT>
+template <int D, int MTO, int MTP>
 int launch_split(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    const void* fn = reinterpret_cast<const void*>(&krk::attn_split_kernel<D, MT>);
-    const size_t shm = krk::split_lds_bytes<D, MT>();
+    const void* fn = reinterpret_cast<const void*>(&krk::attn_split_kernel<D, MTO, MTP>);
+    const size_t shm = krk::split_lds_bytes<D, (MTO > MTP ? MTO : MTP)>();
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "attn_split_kernel LDS size");
     void* args[] = {(void*)&p};
     return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(krk::kSplitThreads), args, shm, stream), "attn_split_kernel launch");
 }
 
-template <int D, int W>
+template <int D>
 int launch_tile(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    const void* fn = reinterpret_cast<const void*>(&krk::attn_tile_kernel<D, W>);
+    const void* fn = reinterpret_cast<const void*>(&krk::attn_tile_kernel<D>);
     const size_t shm = krk::tile_lds_bytes<D>();
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "attn_tile_kernel LDS size");
     void* args[] = {(void*)&p};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(64 * W), args, shm, stream), "attn_tile_kernel launch");
-}
-
-template <int D>
-int launch_rows(const krk::AttnParams& p, int rows, int64_t blocks, hipStream_t stream) {
-    switch (rows) {
-        case 16: return launch_split<D, 1>(p, blocks, stream);
-        case 32: return launch_split<D, 2>(p, blocks, stream);
-        case 128: return launch_tile<D, 4>(p, blocks, stream);
-        default: return launch_tile<D, 8>(p, blocks, stream);
-    }
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(krk::kTileThreads), args, shm, stream), "attn_tile_kernel launch");
 }
 
 template <int D>
 int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
-    if (plan.prefix.splits) {
-        const int64_t blocks = (int64_t)plan.prefix.tiles * p.kv_heads * plan.prefix.splits;
-        if (int rc = launch_rows<D>(p, plan.prefix.rows, blocks, stream)) return rc;
-    }
-    krk::AttnParams o = p;
-    o.prefix_row_tiles = 0;
-    const int64_t blocks = (int64_t)plan.own.tiles * p.kv_heads * p.B * plan.own.splits;
-    if (int rc = launch_rows<D>(o, plan.own.rows, blocks, stream)) return rc;
+    const int64_t own = (int64_t)plan.own.tiles * p.kv_heads * p.B * plan.own.splits;
+    const int64_t shared = (int64_t)plan.prefix.tiles * p.kv_heads * plan.prefix.splits;
     void* args[] = {(void*)&p};
-    if (plan.own.splits + plan.prefix.splits > 1) {
+    if (plan.own.rows <= 32 && plan.prefix.rows <= 32) {  // one launch
+        int rc;
+        if (plan.own.rows == 32) rc = launch_split<D, 2, 2>(p, own + shared, stream);
+        else if (plan.prefix.rows == 32) rc = launch_split<D, 1, 2>(p, own + shared, stream);
+        else rc = launch_split<D, 1, 1>(p, own + shared, stream);
+        if (rc) return rc;
+    } else {
+        if (shared) {
+            if (int rc = launch_tile<D>(p, shared, stream)) return rc;
+        }
+        krk::AttnParams o = p;
+        o.prefix_row_tiles = 0;  // the own caches' workgroups alone
+        int rc;
+        switch (plan.own.rows) {
+            case 16: rc = launch_split<D, 1, 1>(o, own, stream); break;
+            case 32: rc = launch_split<D, 2, 2>(o, own, stream); break;
+            default: rc = launch_tile<D>(o, own, stream);
+        }
+        if (rc) return rc;
+    }
+    if (plan.own.splits + plan.prefix.splits > 1 && !plan.join_in_kernel) {
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_join_kernel<D>),
-                                             dim3((unsigned)cdiv(plan.all_rows, 4)), dim3(256), args, 0, stream);
+                                             dim3((unsigned)cdiv(plan.all_rows, 256 / (D / 4) / krk::kGroups)), dim3(256), args, 0, stream);
         if (int rc = hip_status(e, "attn_join_kernel launch")) return rc;
     }
-    if (p.stat) {
+    if (plan.keep_raw) {
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_weights_raw_kernel),
+                                             dim3((unsigned)cdiv(p.capacity, 1024), p.kv_heads, p.B), dim3(256), args, 0, stream);
+        if (int rc = hip_status(e, "attn_weights_raw_kernel launch")) return rc;
+    } else if (p.stat) {
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_weights_kernel<D>),
                                              dim3((unsigned)cdiv(p.capacity, 128), p.kv_heads, p.B), dim3(256), args, 0, stream);
         if (int rc = hip_status(e, "attn_weights_kernel launch")) return rc;
@@ -342,11 +366,17 @@ int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* 
     p.so_seq = a.so_seq;
     p.so_head = a.so_head;
     unsigned char* w = static_cast<unsigned char*>(workspace);
-    if (plan.part) {
-        p.part = reinterpret_cast<float*>(w);
-        p.ml = reinterpret_cast<float2*>(w + plan.part);
-    }
-    if (s.scored) p.stat = reinterpret_cast<float2*>(w + plan.part + plan.ml);
+    auto take = [&](size_t n) {
+        unsigned char* at = n ? w : nullptr;
+        w += n;
+        return at;
+    };
+    p.ctr = reinterpret_cast<uint32_t*>(take(plan.ctr));
+    p.part = reinterpret_cast<float*>(take(plan.part));
+    p.ml = reinterpret_cast<float2*>(take(plan.ml));
+    p.stat = reinterpret_cast<float2*>(take(plan.stat));
+    p.raw = reinterpret_cast<float*>(take(plan.raw));
+    p.raw_row = plan.raw_row;
     p.scale = a.scale;
     p.c = (float)((double)a.scale * 1.4426950408889634);
     p.B = s.B;
@@ -387,7 +417,7 @@ int krk_qk_norm_rope_bf16(const krk_rope_args* args, void* stream) {
         return fail(KRK_ATTN_ERR_ALIGN, "q_norm, k_norm and table must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(a.lens) | reinterpret_cast<uintptr_t>(a.positions)) % 4)
         return fail(KRK_ATTN_ERR_ALIGN, "lens and positions must be 4-byte aligned");
-    const bool in_place = a.q_out == a.qkv && a.q_row == a.qkv_row;
+    const bool in_place = a.q_out == a.qkv && (M == 1 || a.q_row == a.qkv_row);
     const Span ins[5] = {span(a.q_norm, a.head_dim, 2), span(a.k_norm, a.head_dim, 2), span(a.table, (uint64_t)a.table_rows * a.head_dim, 4),
                          span(a.lens, a.B, 4), span(a.positions, M, 4)};
     bool bad = (overlaps(q, qkv) && !in_place) || overlaps(k, qkv) || overlaps(v, qkv) || overlaps(q, k) || overlaps(q, v) || a.k.p == a.v.p;

@@ -44,6 +44,9 @@ struct AttnParams {
     float* part;   // [splits + prefix_splits][rows][D] unnormalised outputs
     float2* ml;    // [splits + prefix_splits][rows] running maximum (of q.k) and sum
     float2* stat;  // [rows] final maximum and 1 / sum (scored calls)
+    float* raw;    // [rows][raw_row] scores q.k of a scored call that keeps them, else null
+    uint32_t* ctr; // [B][kv_heads] finished workgroups, null where the join has a launch of its own
+    int64_t raw_row;
     float scale;   // of q.k
     float c;       // scale * log2(e)
     int B, R, heads, kv_heads, G, RG, capacity, window, sinks, prefix;
@@ -94,6 +97,23 @@ __device__ __forceinline__ bool sees(const RowSight& s, int t, int sinks) {
     return (t <= s.hi && (t >= s.lo || t < sinks)) || node;
 }
 
+// Partial results cross XCDs, whose L2s are not coherent with each other:
+// agent-scope relaxed accesses, ordered by a drain before the counter moves.
+__device__ __forceinline__ void put_agent(float2* p, float2 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_agent(const float2* p) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void put_agent(float* p, const f32x4& v) {
+    put_agent(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
+    put_agent(reinterpret_cast<float2*>(p) + 1, make_float2(v[2], v[3]));
+}
+__device__ __forceinline__ f32x4 get_agent(const float* p) {
+    const float2 a = get_agent(reinterpret_cast<const float2*>(p)), b = get_agent(reinterpret_cast<const float2*>(p) + 1);
+    return f32x4{a.x, a.y, b.x, b.y};
+}
+
 // Wait until every load this wave issued has returned.
 __device__ __forceinline__ void drain_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -103,7 +123,7 @@ __device__ __forceinline__ void drain_loads() {
 
 __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// A workgroup's share: TR rows of a key/value head against one range of the
+// A workgroup's share: a tile of rows of a key/value head against one range of the
 // keys of a run (a sequence's own cache, or the shared prefix).
 struct Task {
     bool shared;
@@ -118,8 +138,7 @@ struct Task {
 // Heads change fastest: with 8 heads each XCD (workgroups go to them round
 // robin) keeps to one head's keys.  Later row tiles, which see more keys, go
 // first.
-template <int TR>
-__device__ __forceinline__ Task task_of(const AttnParams& p, int id) {
+__device__ __forceinline__ Task task_of(const AttnParams& p, int id, int own_rows, int prefix_rows) {
     Task t;
     const int nprefix = p.prefix_row_tiles * p.kv_heads * p.prefix_splits;
     t.shared = id < nprefix;
@@ -147,7 +166,7 @@ __device__ __forceinline__ Task task_of(const AttnParams& p, int id) {
         t.seg = p.prefix;
         t.limit = seq_len(p, t.b0);
     }
-    t.row0 = tile * TR;
+    t.row0 = tile * (t.shared ? prefix_rows : own_rows);
     const CacheView& k = t.shared ? p.kp : p.k;
     const CacheView& v = t.shared ? p.vp : p.v;
     t.k = k.p + (t.shared ? 0 : (int64_t)t.b0 * k.seq) + (int64_t)t.h * k.head;
@@ -193,12 +212,20 @@ struct Reach {
         hi_max = -wave_min_i(-hi_max);
         hi_min = wave_min_i(hi_min);
     }
+    template <int CTRL>
+    __device__ static __forceinline__ int dpp_min(int v) {
+        const int o = __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+        return o < v ? o : v;
+    }
     __device__ static __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int o = __shfl_xor(v, s);
-            v = o < v ? o : v;
-        }
+        v = dpp_min<0xB1>(v);   // lane ^ 1
+        v = dpp_min<0x4E>(v);   // lane ^ 2
+        v = dpp_min<0x141>(v);  // mirrored in 8
+        v = dpp_min<0x140>(v);  // mirrored in 16
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = (int)a[0] < (int)a[1] ? (int)a[0] : (int)a[1];
+        const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = (int)b[0] < (int)b[1] ? (int)b[0] : (int)b[1];
         return __builtin_amdgcn_readfirstlane(v);
     }
 };
@@ -252,6 +279,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // The key of 32 that row r of 16-key tile t holds (see the top).
 __device__ __forceinline__ int tile_key(int t, int r) { return 8 * (r >> 2) + 4 * t + (r & 3); }
 
+// Two bf16 values with zeros for infinities and NaNs.
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
+    return ((w & 0x7f80u) != 0x7f80u ? w & 0xffffu : 0u) | ((w & 0x7f800000u) != 0x7f800000u ? w & 0xffff0000u : 0u);
+}
+// An infinity or NaN given as an fp32's bits, else 0.
+__device__ __forceinline__ float odd_or_zero(uint32_t f32_bits) {
+    return (f32_bits & 0x7f800000u) == 0x7f800000u ? __uint_as_float(f32_bits) : 0.0f;
+}
+
+// Four finished outputs of row j of (b, h), and with d = 0 what else is kept
+// of the row: M the maximum of q.k (-infinity: the row sees nothing), L the sum.
+__device__ __forceinline__ void finish_row(const AttnParams& p, int b, int h, int j, int D, int d, const f32x4& o, float M, float L) {
+    const int r = j / p.G;
+    const int head = h * p.G + (j - r * p.G);
+    const int64_t at = (int64_t)b * p.R + r;
+    const bool none = L == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / L;
+    *reinterpret_cast<uint2*>(p.out + at * p.out_row + (int64_t)head * D + d) =
+        none ? make_uint2(0u, 0u) : make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+    if (d == 0) {
+        if (p.lse) p.lse[at * p.heads + head] = none ? kNegInf : M * p.scale + logf(L);
+        if (p.stat) p.stat[((int64_t)b * p.kv_heads + h) * p.RG + j] = make_float2(M == kNegInf ? 0.0f : M, inv);
+    }
+}
+
 // 32 keys as operands of S^T = K Q^T: two 16-key tiles of D / 32 k-steps.
 template <int D>
 struct KeyFrag {
@@ -279,23 +331,15 @@ template <int D>
 struct ValueFrag {
     static constexpr int VD = D / 16;
     static constexpr int W = VD / 2;  // dwords of a key in a lane
-    uint32_t f[8][W];
+    typedef __attribute__((ext_vector_type(W))) uint32_t vec;
+    vec f[8];
     __device__ __forceinline__ void load(const uint16_t* base, int64_t slot, int kb, int limit, int lane) {
         const int r = lane & 15, q = lane >> 4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             int key = kb + 8 * q + i;
             key = key < limit ? key : limit - 1;
-            const uint16_t* row = base + (int64_t)key * slot + VD * r;
-            if constexpr (VD == 8) {
-                const u32x4 x = load_cached16(row);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) f[i][w] = x[w];
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(row);
-                f[i][0] = x.x;
-                f[i][1] = x.y;
-            }
+            f[i] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(base + (int64_t)key * slot + VD * r));
         }
     }
     // Operand of outputs d = VD r + j.
@@ -305,6 +349,18 @@ struct ValueFrag {
         for (int i = 0; i < 4; ++i)
             x[i] = __builtin_amdgcn_perm(f[2 * i + 1][j >> 1], f[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
         return __builtin_bit_cast(bf16x8, x);
+    }
+    // Infinities and NaNs to zero.
+    __device__ __forceinline__ void tame() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const vec e = f[i] & 0x7f807f80u;
+            vec keep;
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                keep[w] = ((e[w] & 0xffffu) != 0x7f80u ? 0xffffu : 0u) | ((e[w] >> 16) != 0x7f80u ? 0xffff0000u : 0u);
+            f[i] &= keep;
+        }
     }
     // Whether this lane holds an infinity or a NaN.
     __device__ __forceinline__ bool odd() const {
@@ -326,65 +382,11 @@ __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, const 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight bf16 values with zeros for infinities and NaNs.
 __device__ __forceinline__ u32x4 finite_bf16x8(const u32x4& x) {
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = x[i];
-        r[i] = ((w & 0x7f80u) != 0x7f80u ? w & 0xffffu : 0u) | ((w & 0x7f800000u) != 0x7f800000u ? w & 0xffff0000u : 0u);
-    }
+    for (int i = 0; i < 4; ++i) r[i] = finite_bf16x2(x[i]);
     return r;
-}
-// Marks for the infinities and NaNs among them, in bf16: 1 for +infinity, 2^7
-// for -infinity, 2^14 for NaN.  A sum of up to 64 of each says which there are.
-__device__ __forceinline__ uint32_t odd_mark(uint32_t e) {
-    const uint32_t m = e == 0x7f80u ? 0x3f80u : e == 0xff80u ? 0x4300u : 0x4680u;
-    return (e & 0x7f80u) == 0x7f80u ? m : 0u;
-}
-__device__ __forceinline__ u32x4 odd_marks(const u32x4& x) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = x[i];
-        r[i] = odd_mark(w & 0xffffu) | odd_mark(w >> 16) << 16;
-    }
-    return r;
-}
-__device__ __forceinline__ float odd_value(float n) {
-    const uint32_t c = (uint32_t)n;
-    const float inf = __builtin_inff();
-    float v = (c & 0x7fu) ? inf : 0.0f;
-    v = (c >> 7) & 0x7fu ? v - inf : v;  // both signs: NaN
-    return c >> 14 ? __builtin_nanf("") : v;
-}
-
-// O^T += V^T P^T where values among the 32 keys are infinite or NaN; bit i of
-// vis says that the lane's row sees key 8q + i.  A zero weight times an infinity
-// would reach rows that do not see it, so the products run on the finite values
-// alone, and a count of the visible infinities and NaNs of each output (their
-// marks against zeros and ones) adds them.
-template <int D, int MT>
-__device__ __forceinline__ void add_odd_values(f32x4 (&acc)[MT][D / 16], const ValueFrag<D>& v, const bf16x8 (&hi)[MT],
-                                               const bf16x8 (&lo)[MT], const uint32_t (&vis)[MT]) {
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-        const u32x4 x = __builtin_bit_cast(u32x4, v.operand(j));
-        const bf16x8 a = __builtin_bit_cast(bf16x8, finite_bf16x8(x));
-        const u32x4 marks = odd_marks(x);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            u32x4 ones;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                ones[e] = ((vis[i] >> (2 * e)) & 1) * 0x3f80u | ((vis[i] >> (2 * e + 1)) & 1) * 0x3f800000u;
-            acc[i][j] = mfma16(a, hi[i], mfma16(a, lo[i], acc[i][j]));
-            const f32x4 n = mfma16(marks, ones, f32x4{0, 0, 0, 0});
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] += odd_value(n[e]);
-            __builtin_amdgcn_sched_barrier(0);  // one tile's temporaries at a time
-        }
-    }
 }
 
 }  // namespace krk

@@ -21,6 +21,7 @@
 #pragma once
 
 #include "krk_attn_common.h"
+#include "krk_epilogue.h"
 
 namespace krk {
 
@@ -33,16 +34,14 @@ constexpr size_t split_lds_bytes() {
 }
 
 template <int D, int MT>
-__global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_kernel(AttnParams p) {
+__device__ __forceinline__ void split_task(const AttnParams& p, const Task& task, unsigned char* lds) {
     constexpr int TR = 16 * MT;
     constexpr int KS = D / 32;
     constexpr int VD = D / 16;
-    extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
 
-    const Task task = task_of<TR>(p, blockIdx.x);
     const int limit = task.limit;
 
     // This lane's rows: what they see, and their q.
@@ -72,6 +71,10 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
         for (int j = 0; j < VD; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     }
 
+    // An infinity or a NaN times a zero weight would reach rows that do not see
+    // it: the products run on zeros in their place, and the rows that see them
+    // get them behind the last step.
+    bool any_odd = false;
     KeyFrag<D> kf;
     ValueFrag<D> vf;
     const int t1 = steps.t1;
@@ -98,19 +101,25 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
         // sees whole skip this.
         const int pos = task.seg + kb;
         const bool whole = kb + 32 <= limit && pos + 31 <= reach.hi_min && (pos >= reach.lo_max || pos + 32 <= p.sinks);
-        uint32_t vis[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) vis[i] = 0xff;
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                vis[i] = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = kb + 8 * q4 + e;
                     const bool ok = key < limit && sees(sight[i], task.seg + key, p.sinks);
-                    vis[i] |= ok ? 1u << e : 0u;
                     s[i][e >> 2][e & 3] = ok ? s[i][e >> 2][e & 3] : kNegInf;
+                }
+            }
+        }
+        if (p.raw) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int row = task.row0 + 16 * i + n16;
+                if (row < task.rows) {
+                    float* to = p.raw + (((int64_t)task.b0 * p.kv_heads + task.h) * p.RG + row) * p.raw_row + kb + 8 * q4;
+                    *reinterpret_cast<f32x4*>(to) = s[i][0];
+                    *reinterpret_cast<f32x4*>(to + 4) = s[i][1];
                 }
             }
         }
@@ -146,16 +155,38 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
             }
         }
         if (__any(vf.odd())) {
-            add_odd_values<D, MT>(acc, vf, hi, lo, vis);
-        } else {
+            vf.tame();
+            any_odd = true;
+        }
 #pragma unroll
-            for (int j = 0; j < VD; ++j) {
-                const bf16x8 a = vf.operand(j);
+        for (int j = 0; j < VD; ++j) {
+            const bf16x8 a = vf.operand(j);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, lo[i], acc[i][j]));
-            }
+            for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, lo[i], acc[i][j]));
         }
         if (next < t1) vf.load(task.v, task.v_slot, steps.key(next), limit, lane);
+    }
+
+    if (any_odd) {  // rare, so key by key
+#pragma unroll 1
+        for (t = steps.t0 + wave; t < t1; t += kSplitWaves) {
+#pragma unroll 1
+            for (int key = steps.key(t); key < steps.key(t) + 32 && key < limit; ++key) {
+                const uint16_t* vr = task.v + (int64_t)key * task.v_slot + 4 * q4 * VD;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < VD; j += 2) {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(vr + e * VD + j);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            const bool ok = sees(sight[i], task.seg + key, p.sinks);
+                            acc[i][j][e] += ok ? odd_or_zero(x << 16) : 0.0f;
+                            acc[i][j + 1][e] += ok ? odd_or_zero(x & 0xffff0000u) : 0.0f;
+                        }
+                    }
+            }
+        }
     }
 
     // The waves meet: O as [wave][row][D + 4] (rows 4 banks apart), maxima and
@@ -205,82 +236,178 @@ __global__ void __launch_bounds__(kSplitThreads, MT == 1 ? 2 : 1) attn_split_ker
         }
         const int b = task.shared ? row / p.RG : task.b0;
         const int j = task.shared ? row - b * p.RG : row;
-        const int64_t g = ((int64_t)b * p.kv_heads + task.h) * p.RG + j;
         if (last) {
-            const int r = j / p.G;
-            const int head = task.h * p.G + (j - r * p.G);
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            if (L == 0.0f) o = f32x4{0, 0, 0, 0};
-            const int64_t at = (int64_t)b * p.R + r;
-            *reinterpret_cast<uint2*>(p.out + at * p.out_row + (int64_t)head * D + d) =
-                make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-            if (d == 0) {
-                if (p.lse) p.lse[at * p.heads + head] = L == 0.0f ? kNegInf : M * p.scale + logf(L);
-                if (p.stat) p.stat[g] = make_float2(ms, inv);
-            }
+            finish_row(p, b, task.h, j, D, d, o, M, L);
         } else {
-            *reinterpret_cast<f32x4*>(p.part + ((int64_t)task.part * all_rows + g) * D + d) = o;
-            if (d == 0) p.ml[(int64_t)task.part * all_rows + g] = make_float2(M, L);
+            const int64_t g = (int64_t)task.part * all_rows + ((int64_t)b * p.kv_heads + task.h) * p.RG + j;
+            put_agent(p.part + g * D + d, o);
+            if (d == 0) put_agent(p.ml + g, make_float2(M, L));
         }
     }
 }
 
-// Joins the key ranges: a wave per row.  Ranges in order, so the result does
-// not depend on which finished first.
+// Four outputs of a row over some of its key ranges, and their maximum and sum.
+struct Joined {
+    float M = kNegInf, L = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    __device__ __forceinline__ void add(const AttnParams& p, float m, float l, const f32x4& x) {
+        const float mn = fmaxf(M, m);
+        const float ms = mn == kNegInf ? 0.0f : mn;
+        const float f0 = exp2_raw((M - ms) * p.c), f1 = exp2_raw((m - ms) * p.c);
+        L = L * f0 + f1 * l;
+        o = o * f0 + f1 * x;
+        M = mn;
+    }
+};
+
+// Joins key ranges from, from + step, ... of row `row` (of all rows); kJoin
+// loads are in flight at a time.  AGENT: they were written by this launch, so
+// each is a round trip beyond this XCD's L2.
+constexpr int kJoin = 8;
+template <int D, bool AGENT>
+__device__ __forceinline__ Joined join_ranges(const AttnParams& p, int64_t row, int d, int from, int step) {
+    const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
+    const int n = p.splits + p.prefix_splits;
+    Joined y;
+    for (int s0 = from; s0 < n; s0 += kJoin * step) {
+        float2 ml[kJoin];
+        f32x4 x[kJoin];
+#pragma unroll
+        for (int s = 0; s < kJoin; ++s) {
+            const int at = s0 + s * step;
+            const int64_t g = (at < n ? at : s0) * all_rows + row;
+            ml[s] = AGENT ? get_agent(p.ml + g) : p.ml[g];
+            x[s] = AGENT ? get_agent(p.part + g * D + d) : *reinterpret_cast<const f32x4*>(p.part + g * D + d);
+        }
+#pragma unroll
+        for (int s = 0; s < kJoin; ++s)
+            if (s0 + s * step < n) y.add(p, ml[s].x, ml[s].y, x[s]);
+    }
+    return y;
+}
+
+// Joins all rows of (b, h) with the whole workgroup: every four outputs of a
+// row are one thread's, or (few rows) several threads', each with every
+// groups-th range, which then meet in LDS in order.  The ranges a thread takes
+// and the order they are added in follow from the shape alone, so the result
+// does not depend on which range finished first.
+template <int D>
+__device__ __forceinline__ void join_rows(const AttnParams& p, int b, int h, unsigned char* lds) {
+    const int64_t first = ((int64_t)b * p.kv_heads + h) * p.RG;
+    const int units = p.RG * (D / 4);
+    int groups = 1;
+    while (2 * groups * units <= kSplitThreads && groups < 8) groups *= 2;
+    const int g = groups > 1 ? threadIdx.x / units : 0;
+    if (groups > 1) {
+        const int e = threadIdx.x - g * units;
+        const int j = e / (D / 4), d = 4 * (e % (D / 4));
+        Joined y;
+        if (g < groups) y = join_ranges<D, true>(p, first + j, d, g, groups);
+        f32x4* lo = reinterpret_cast<f32x4*>(lds);
+        float2* lml = reinterpret_cast<float2*>(lds + kSplitThreads * sizeof(f32x4));
+        __syncthreads();
+        lo[threadIdx.x] = y.o;
+        lml[threadIdx.x] = make_float2(y.M, y.L);
+        __syncthreads();
+        if (g == 0) {
+            for (int k = 1; k < groups; ++k) y.add(p, lml[e + k * units].x, lml[e + k * units].y, lo[e + k * units]);
+            finish_row(p, b, h, j, D, d, y.o, y.M, y.L);
+        }
+        return;
+    }
+    for (int e = threadIdx.x; e < units; e += kSplitThreads) {
+        const int j = e / (D / 4), d = 4 * (e % (D / 4));
+        const Joined y = join_ranges<D, true>(p, first + j, d, 0, 1);
+        finish_row(p, b, h, j, D, d, y.o, y.M, y.L);
+    }
+}
+
+// MTO 16-row tiles of a sequence's own rows per workgroup, MTP of the rows over
+// a shared prefix, in one launch.  Where partial results are joined here, the
+// workgroup that finishes last for a sequence and head does it: no second
+// launch (3 us and more between dependent kernels, and 2 us of host time).
+template <int D, int MTO, int MTP>
+__global__ void __launch_bounds__(kSplitThreads, 2) attn_split_kernel(AttnParams p) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ int done[16 * (MTO > MTP ? MTO : MTP)];
+    const Task task = task_of(p, blockIdx.x, 16 * MTO, 16 * MTP);
+    if (MTO == MTP || !task.shared) split_task<D, MTO>(p, task, lds);
+    else split_task<D, MTP>(p, task, lds);
+    if (!p.ctr) return;
+    const int TR = 16 * (task.shared ? MTP : MTO);
+    const int end = task.row0 + TR < task.rows ? task.row0 + TR : task.rows;
+    const int b_lo = task.shared ? task.row0 / p.RG : task.b0;
+    const int nb = task.shared ? (end - 1) / p.RG - b_lo + 1 : 1;
+    drain_memory();
+    __syncthreads();
+    if ((int)threadIdx.x < nb) {
+        const int b = b_lo + threadIdx.x;
+        uint32_t all = (uint32_t)(p.row_tiles * p.splits);
+        if (p.prefix_splits) {
+            const int t0 = b * p.RG / (16 * MTP), t1 = ((b + 1) * p.RG - 1) / (16 * MTP);
+            all += (uint32_t)((t1 - t0 + 1) * p.prefix_splits);
+        }
+        const uint32_t before = __hip_atomic_fetch_add(p.ctr + (int64_t)b * p.kv_heads + task.h, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        done[threadIdx.x] = before == all - 1;
+    }
+    __syncthreads();
+    for (int i = 0; i < nb; ++i) {
+        if (!done[i]) continue;
+        join_rows<D>(p, b_lo + i, task.h, lds);
+        if (threadIdx.x == 0)
+            __hip_atomic_store(p.ctr + (int64_t)(b_lo + i) * p.kv_heads + task.h, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+// Joins the key ranges in a launch of its own: D / 4 threads a row and group
+// of ranges, kGroups groups that meet in LDS in order.
+constexpr int kGroups = 4;
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnParams p) {
-    const int lane = threadIdx.x & 63;
+    constexpr int T = D / 4;                      // threads of a row and group
+    constexpr int ROWS = 256 / T / kGroups;       // of a workgroup
+    __shared__ f32x4 lo[256];
+    __shared__ float2 lml[256];
     const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
-    const int64_t g = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (g >= all_rows) return;
-    const int n = p.splits + p.prefix_splits;
-    float M = kNegInf;
-    for (int s = lane; s < n; s += 64) M = fmaxf(M, p.ml[s * all_rows + g].x);
+    const int t = threadIdx.x % T, g = threadIdx.x / T % kGroups;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / (T * kGroups);
+    const bool live = row < all_rows;
+    Joined y;
+    if (live) y = join_ranges<D, false>(p, row, 4 * t, g, kGroups);
+    lo[threadIdx.x] = y.o;
+    lml[threadIdx.x] = make_float2(y.M, y.L);
+    __syncthreads();
+    if (!live || g) return;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) M = fmaxf(M, __shfl_xor(M, s));
-    const float ms = M == kNegInf ? 0.0f : M;
-    float L = 0.0f, o[D / 64];
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-    for (int s0 = 0; s0 < n; s0 += 64) {
-        float f = 0.0f, part_l = 0.0f;
-        if (s0 + lane < n) {
-            const float2 ml = p.ml[(s0 + lane) * all_rows + g];
-            f = exp2_raw((ml.x - ms) * p.c);
-            part_l = f * ml.y;
-        }
-        const int cnt = n - s0 < 64 ? n - s0 : 64;
+    for (int k = 1; k < kGroups; ++k) y.add(p, lml[threadIdx.x + k * T].x, lml[threadIdx.x + k * T].y, lo[threadIdx.x + k * T]);
+    const int64_t bh = row / p.RG;
+    finish_row(p, (int)(bh / p.kv_heads), (int)(bh % p.kv_heads), (int)(row - bh * p.RG), D, 4 * t, y.o, y.M, y.L);
+}
+
+// Adds the keys' weights to their scores from the kept q.k: 4 keys a thread.
+// 8 bytes a key and row (write, read) against a second read of K at 2 * D.
+__global__ void __launch_bounds__(256) attn_weights_raw_kernel(AttnParams p) {
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int len = seq_len(p, b);
+    const int key = 4 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
+    if (key >= len) return;
+    const int64_t first = ((int64_t)b * p.kv_heads + h) * p.RG;
+    f32x4 w = {0, 0, 0, 0};
 #pragma unroll 4
-        for (int s = 0; s < cnt; ++s) {
-            const float fs = __shfl(f, s);
-            L += __shfl(part_l, s);
-            const float* q = p.part + ((int64_t)(s0 + s) * all_rows + g) * D + lane * (D / 64);
-            if constexpr (D == 128) {
-                const float2 x = *reinterpret_cast<const float2*>(q);
-                o[0] = __builtin_fmaf(fs, x.x, o[0]);
-                o[1] = __builtin_fmaf(fs, x.y, o[1]);
-            } else {
-                o[0] = __builtin_fmaf(fs, *q, o[0]);
-            }
+    for (int j = 0; j < p.RG; ++j) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(p.raw + (first + j) * p.raw_row + key);
+        const float2 st = p.stat[first + j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = exp2_raw((s[e] - st.x) * p.c) * st.y;
+            w[e] += s[e] == kNegInf || st.y == 0.0f ? 0.0f : x;  // hidden, or the row sees nothing
         }
     }
-    const int64_t bh = g / p.RG;
-    const int j = (int)(g - bh * p.RG);
-    const int b = (int)(bh / p.kv_heads), h = (int)(bh - (int64_t)b * p.kv_heads);
-    const int r = j / p.G;
-    const int head = h * p.G + (j - r * p.G);
-    const int64_t at = (int64_t)b * p.R + r;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (L == 0.0f) o[0] = o[D / 64 - 1] = 0.0f;
-    uint16_t* y = p.out + at * p.out_row + (int64_t)head * D + lane * (D / 64);
-    if constexpr (D == 128)
-        *reinterpret_cast<uint32_t*>(y) = pack_bf16(o[0] * inv, o[1] * inv);
-    else
-        *y = (uint16_t)f32_to_bf16(o[0] * inv);
-    if (lane == 0) {
-        if (p.lse) p.lse[at * p.heads + head] = L == 0.0f ? kNegInf : M * p.scale + logf(L);
-        if (p.stat) p.stat[g] = make_float2(ms, inv);
-    }
+    const float* was = p.scores + (int64_t)b * p.sc_seq + (int64_t)h * p.sc_head + key;
+    float* to = p.scores_out + (int64_t)b * p.so_seq + (int64_t)h * p.so_head + key;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (key + e < len) to[e] = was[e] + w[e];
 }
 
 // Adds the keys' weights to their scores: a wave per 32 keys of a sequence

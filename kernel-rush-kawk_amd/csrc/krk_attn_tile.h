@@ -1,29 +1,28 @@
-// Cache attention for many rows of a head (prompts, large batches over a
-// shared prefix): one workgroup per tile of 32 * W rows, K and V through LDS.
+// Cache attention for many rows of a head (prompts, batches over a shared
+// prefix): one workgroup per tile of 128 rows, K and V through LDS.
 //
 // Bound by the matrix pipe, the exponentials and LDS alike: 64 keys of a wave's
 // 32 rows are 1.05 MFLOP (1030 cycles of a SIMD's MFMA at head size 128), 32 KB
 // of LDS reads (a quarter of 1030 cycles of what a CU's LDS delivers), and 2048
-// weights at about 30 VALU cycles per 64 of them.
+// weights at about 25 VALU cycles per 64 of them.
 //
-// Work split.  W waves (4 or 8), each with 32 rows of its own, all reading the
-// same 64-key steps of K and V from LDS; two waves per SIMD, so that one's
-// softmax runs under the other's products.  S^T = K Q^T and O^T = V^T P^T on
+// Work split.  Four waves, each with 32 rows of its own, all reading the same
+// 64-key steps of K and V from LDS.  S^T = K Q^T and O^T = V^T P^T on
 // v_mfma_f32_32x32x16_bf16, the row in the column (lane & 31) of either; the key
 // order of a step's second product is the one the first leaves in its lanes, so
 // weights stay in their lane.  V's operand comes transposed out of LDS
-// (ds_read_b64_tr_b16).
+// (ds_read_b64_tr_b16).  Two workgroups share a CU (80 KB of LDS and up to 256
+// registers a lane each) and run apart, so that one's exponentials run under the
+// other's products: 8 waves in one workgroup, in step or half a step apart,
+// were 8% slower at 8192 rows.
 //
-// Steps are pipelined: the scores of step j + 1 (MFMA) run with the weights of
-// step j (VALU), then step j's products with V with the maxima of step j + 1.
 // The running maximum moves only when a row's grows by more than 2^8 (the
 // weights stay below 2^8 then, which costs no precision), so O is rescaled a
 // few times a row instead of every step.
 //
-// LDS: rings of three 64-key steps of K and two of V (80 KB at head size 128:
-// two workgroups a CU), filled by DMA, one barrier a step.  16-byte chunks of a
-// row are permuted with the row's low bits, so that neither kind of read meets
-// bank conflicts.
+// LDS: rings of three 64-key steps of K and two of V, filled by DMA, one
+// barrier a step.  16-byte chunks of a row are permuted with the row's low
+// bits, so that neither kind of read meets bank conflicts.
 //
 // Weights are rounded to bf16 for the product with V (their sum is not): with
 // 8 bits of mantissa each, the error of a weighted mean of many values is that
@@ -39,24 +38,35 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kTileStep = 64;
-constexpr int kTileKRing = 3, kTileVRing = 2;
+constexpr int kTileWaves = 4;
+constexpr int kTileThreads = 64 * kTileWaves;
+constexpr int kTileRows = 32 * kTileWaves;
+constexpr int kTileKRing = 3, kTileVRing = 2;  // steps in LDS
 
 template <int D>
 constexpr size_t tile_lds_bytes() {
     return (size_t)(kTileKRing + kTileVRing) * kTileStep * D * 2;
 }
 
+// One 1 KB DMA into LDS, lane l's 16 bytes from src to dst + 16 l (as dma_row).
+// In assembly, because around the builtin the compiler waits for every DMA in
+// flight before a transposed LDS read, and a step then lasts as long as the
+// fetch that it started; the waits here are vm_wait_stages' alone.
+__device__ __forceinline__ void dma_row_quiet(const uint16_t* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(dst) : "memory", "m0");
+}
+
 __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-template <int D, int W>
+template <int D>
 struct TileKernel {
     static constexpr int KS = D / 16;  // k-steps of S^T
     static constexpr int DT = D / 32;  // 32-wide tiles of O^T
     static constexpr int CH = D / 8;   // 16-byte chunks of a row
     static constexpr int ROWS_PER_DMA = 64 / CH;
-    static constexpr int DMAS = kTileStep / ROWS_PER_DMA / W;  // of K, or of V, per wave and step
+    static constexpr int DMAS = kTileStep / ROWS_PER_DMA / kTileWaves;  // of K, or of V, per wave and step
     static constexpr int STEP_BYTES = kTileStep * D * 2;
 
     // Chunk permutations: K reads take 16 (8) rows of one chunk at a time, V
@@ -64,27 +74,28 @@ struct TileKernel {
     static __device__ __forceinline__ int k_swizzle(int row) { return row & (CH - 1); }
     static __device__ __forceinline__ int v_swizzle(int row) { return 4 * (row & (CH / 4 - 1)); }
 
-    // This wave's share of keys kb .. kb + 63 into `to`: off[i] is the lane's
-    // place from the step's first key; keys from `limit` on read the last one
-    // again.
+    // This wave's share of keys kb .. kb + 63 into `to`: lane offsets from the
+    // step's first key; keys from `limit` on read the last one again.
     template <bool V>
-    static __device__ __forceinline__ int chunk_of(int i, int wave, int lane) {
-        const int row = (wave + W * i) * ROWS_PER_DMA + lane / CH;
-        return (lane % CH) ^ (V ? v_swizzle(row) : k_swizzle(row));
-    }
-    template <bool V>
-    static __device__ __forceinline__ void fetch(const uint16_t* base, int64_t slot, const int64_t (&off)[DMAS], int kb,
-                                                 int limit, unsigned char* to, int wave, int lane) {
-        const uint16_t* step = base + (int64_t)kb * slot;
+    static __device__ __forceinline__ void offsets(int64_t slot, int wave, int lane, int64_t (&off)[DMAS]) {
 #pragma unroll
         for (int i = 0; i < DMAS; ++i) {
-            const int idx = wave + W * i;
-            const uint16_t* from = step + off[i];
-            if (kb + kTileStep > limit) {
-                const int key = kb + idx * ROWS_PER_DMA + lane / CH;
-                from = base + (int64_t)(key < limit ? key : limit - 1) * slot + 8 * chunk_of<V>(i, wave, lane);
+            const int row = (wave + kTileWaves * i) * ROWS_PER_DMA + lane / CH;
+            off[i] = row * slot + 8 * ((lane % CH) ^ (V ? v_swizzle(row) : k_swizzle(row)));
+        }
+    }
+    static __device__ __forceinline__ void fetch(const uint16_t* base, int64_t slot, const int64_t (&off)[DMAS], int kb,
+                                                 int limit, uint32_t to, int wave, int lane) {
+        const uint16_t* step = base + (int64_t)kb * slot;
+        if (kb + kTileStep <= limit) {
+#pragma unroll
+            for (int i = 0; i < DMAS; ++i) dma_row_quiet(step + off[i], to + (wave + kTileWaves * i) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < DMAS; ++i) {
+                const int over = kb + (wave + kTileWaves * i) * ROWS_PER_DMA + lane / CH - (limit - 1);
+                dma_row_quiet(step + off[i] - (over > 0 ? over : 0) * slot, to + (wave + kTileWaves * i) * 1024);
             }
-            dma_row(from, to + idx * 1024);
         }
     }
 
@@ -112,16 +123,28 @@ __device__ __forceinline__ bool odd_bf16x8(const bf16x8& v) {
     return odd;
 }
 
-template <int D, int W>
-__global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) {
-    using T = TileKernel<D, W>;
+// Issue order of N MFMAs and their operands' LDS reads (EACH an MFMA): AHEAD
+// reads first, then they alternate.  Left alone the compiler reads each operand
+// right before its MFMA and waits.
+template <int N, int AHEAD, int EACH>
+__device__ __forceinline__ void read_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p) {
+    using T = TileKernel<D>;
     constexpr int KS = T::KS, DT = T::DT;
-    constexpr int TR = 32 * W;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, g2 = lane >> 5;
-    const Task task = task_of<TR>(p, blockIdx.x);
+    const Task task = task_of(p, blockIdx.x, kTileRows, kTileRows);
     const int limit = task.limit;
 
     const int my_row = task.row0 + wave * 32 + n32;
@@ -147,7 +170,7 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
         }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < kTileWaves; ++w) {
             block.lo_min = x[4 * w] < block.lo_min ? x[4 * w] : block.lo_min;
             block.hi_max = x[4 * w + 1] > block.hi_max ? x[4 * w + 1] : block.hi_max;
             block.lo_max = x[4 * w + 2] > block.lo_max ? x[4 * w + 2] : block.lo_max;
@@ -164,17 +187,23 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
 
     unsigned char* kring = lds;
     unsigned char* vring = lds + kTileKRing * T::STEP_BYTES;
-    auto k_at = [&](int t) { return kring + (unsigned)t % kTileKRing * T::STEP_BYTES; };
-    auto v_at = [&](int t) { return vring + (unsigned)t % kTileVRing * T::STEP_BYTES; };
-    int64_t k_off[T::DMAS], v_off_in[T::DMAS];
-#pragma unroll
-    for (int i = 0; i < T::DMAS; ++i) {
-        const int row = (wave + W * i) * T::ROWS_PER_DMA + lane / T::CH;
-        k_off[i] = row * task.k_slot + 8 * T::template chunk_of<false>(i, wave, lane);
-        v_off_in[i] = row * task.v_slot + 8 * T::template chunk_of<true>(i, wave, lane);
-    }
-    auto fetch_k = [&](int t) { T::template fetch<false>(task.k, task.k_slot, k_off, steps.key(t), limit, k_at(t), wave, lane); };
-    auto fetch_v = [&](int t) { T::template fetch<true>(task.v, task.v_slot, v_off_in, steps.key(t), limit, v_at(t), wave, lane); };
+    const uint32_t lds_base = (uint32_t)(uintptr_t)(lds_s16x4*)lds;
+    auto k_slot_at = [&](int t) { return (unsigned)t % kTileKRing * T::STEP_BYTES; };
+    auto v_slot_at = [&](int t) { return (unsigned)t % kTileVRing * T::STEP_BYTES; };
+
+    // Steps past the last fetch the last one again, into slots that nothing
+    // reads any more: every step then has the same number of DMAs in flight.
+    int64_t k_off[T::DMAS], v_from[T::DMAS];
+    T::template offsets<false>(task.k_slot, wave, lane, k_off);
+    T::template offsets<true>(task.v_slot, wave, lane, v_from);
+    auto fetch_k = [&](int t) {
+        T::fetch(task.k, task.k_slot, k_off, steps.key(t < t1 ? t : t1 - 1), limit,
+                 lds_base + k_slot_at(t), wave, lane);
+    };
+    auto fetch_v = [&](int t) {
+        T::fetch(task.v, task.v_slot, v_from, steps.key(t < t1 ? t : t1 - 1), limit,
+                 lds_base + kTileKRing * T::STEP_BYTES + v_slot_at(t), wave, lane);
+    };
 
     // This lane's places in a step's K and V.
     const int k_row = n32 * D * 2;
@@ -195,62 +224,53 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
-    // Scores of a step into x.
-    auto scores = [&](int t, f32x16 (&x)[2]) {
-        const unsigned char* kb = k_at(t) + k_row;
+    // Scores of a step.
+    auto scores = [&](int t) {
+        const unsigned char* kb = kring + k_slot_at(t) + k_row;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[kt][e] = 0.0f;
-        // Two k-steps' operands are read ahead, no more: the compiler would
-        // read all of them at once and spill q.
-        bf16x8 a[2][2];
-        auto read = [&](int ks) {
+            for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) a[ks & 1][kt] = T::k_operand(kb, 32 * kt * D * 2 + ((2 * ks) ^ k_xor) * 16);
-        };
-        read(0);
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if (ks + 1 < KS) read(ks + 1);
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) x[kt] = mfma32(a[ks & 1][kt], qf[ks], x[kt]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int kt = 0; kt < 2; ++kt)
+                s[kt] = mfma32(T::k_operand(kb, 32 * kt * D * 2 + ((2 * ks) ^ k_xor) * 16), qf[ks], s[kt]);
+        read_ahead<2 * KS, 6, 1>();
     };
-    // No weight for what the row does not see.  Steps that every row of the
-    // wave sees whole skip this.
+    // No weight for what the row does not see (not called for steps that every
+    // row of the wave sees whole).
     const int hi = sight.hi < task.seg + limit - 1 ? sight.hi : task.seg + limit - 1;
     auto seen_whole = [&](const Reach& r, int kb) {
         const int pos = task.seg + kb;
         return kb + kTileStep <= limit && pos + kTileStep - 1 <= r.hi_min && (pos >= r.lo_max || pos + kTileStep <= p.sinks);
     };
-    auto hide = [&](int t, f32x16 (&x)[2]) {
+    auto hide = [&](int t) {
         const int kb = steps.key(t);
-        if (seen_whole(reach, kb)) return;
-        uint32_t vis = 0;  // bit e: the key of register e
-        if (p.tree) {
-#pragma unroll 1
-            for (int e = 0; e < 32; ++e) {
-                const int key = kb + tile32_key(e >> 4, e & 15, g2);
-                vis |= (key < limit && sees(sight, task.seg + key, p.sinks)) ? 1u << e : 0u;
-            }
-        } else {
-            const int from = task.seg + kb + 4 * g2;
+        const int from = task.seg + kb + 4 * g2;
+        if (!p.tree) {
+            const int top = hi - from, low = sight.lo - from, sink = p.sinks - from;
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-                const int t_e = from + tile32_key(e >> 4, e & 15, 0);
-                const bool ok = (t_e <= hi) & ((t_e >= sight.lo) | (t_e < p.sinks));
-                vis |= ok ? 1u << e : 0u;
+                const int k = tile32_key(e >> 4, e & 15, 0);
+                const bool ok = (k <= top) & ((k >= low) | (k < sink));
+                s[e >> 4][e & 15] = ok ? s[e >> 4][e & 15] : kNegInf;
             }
+            return;
+        }
+        uint32_t vis = 0;  // bit e: the key of register e
+#pragma unroll 1
+        for (int e = 0; e < 32; ++e) {
+            const int k = tile32_key(e >> 4, e & 15, 0) + 4 * g2;
+            vis |= (kb + k < limit && sees(sight, task.seg + kb + k, p.sinks)) ? 1u << e : 0u;
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e >> 4][e & 15] = (vis >> e) & 1 ? x[e >> 4][e & 15] : kNegInf;
+        for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = (vis >> e) & 1 ? s[e >> 4][e & 15] : kNegInf;
     };
-    auto maximum = [&](const f32x16 (&x)[2]) {
-        float v = fmaxf(x[0][0], x[1][0]);
+    auto maximum = [&]() {
+        float v = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) v = fmaxf(fmaxf(v, x[0][e]), x[1][e]);
+        for (int e = 1; e < 16; ++e) v = fmaxf(fmaxf(v, s[0][e]), s[1][e]);
         const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
         return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
     };
@@ -267,36 +287,38 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
     };
-    // Weights of a step, rounded to bf16 as the operand of the second product.
-    auto weigh = [&](const f32x16 (&x)[2], u32x4 (&w)[4]) {
+    // Its weights, rounded to bf16 as the operand of the second product.
+    u32x4 w[4];
+    auto weigh = [&]() {
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-            const float a = exp2_raw(__builtin_fmaf(x[e >> 4][e & 15], p.c, -mc));
-            const float b = exp2_raw(__builtin_fmaf(x[e >> 4][(e & 15) + 1], p.c, -mc));
+            const float a = exp2_raw(__builtin_fmaf(s[e >> 4][e & 15], p.c, -mc));
+            const float b = exp2_raw(__builtin_fmaf(s[e >> 4][(e & 15) + 1], p.c, -mc));
             sum[0] += a;
             sum[1] += b;
             w[e >> 3][(e & 7) >> 1] = pack_bf16(a, b);
         }
         l += sum[0] + sum[1];
     };
-    auto products = [&](int t, const u32x4 (&w)[4]) {
-        const unsigned char* vb = v_at(t);
+    auto products = [&](int t) {
+        const unsigned char* vb = vring + v_slot_at(t);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int d = 0; d < DT; ++d)
                 o[d] = mfma32(T::v_operand(vb + v_off[d] + 16 * ks * D * 2), __builtin_bit_cast(bf16x8, w[ks]), o[d]);
+        read_ahead<4 * DT, 8, 2>();
     };
     // A step that some row of the workgroup does not see whole may hold
     // infinities or NaNs that only some rows see.  Each wave then zeroes those
     // among the values it fetched; they are added behind the last step.
     bool any_odd = false;
     auto tame = [&](int t) {
-        unsigned char* at = v_at(t);
-#pragma unroll
+        unsigned char* at = vring + v_slot_at(t);
+#pragma unroll 1
         for (int i = 0; i < T::DMAS; ++i) {
-            u32x4* x = reinterpret_cast<u32x4*>(at + (wave + W * i) * 1024 + lane * 16);
+            u32x4* x = reinterpret_cast<u32x4*>(at + (wave + kTileWaves * i) * 1024 + lane * 16);
             const u32x4 v = *x;
             if (__any(odd_bf16x8(__builtin_bit_cast(bf16x8, v)))) {
                 *x = finite_bf16x8(v);
@@ -307,46 +329,47 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
 
     if (t0 < t1) {
         // K two steps ahead of the scores, V one ahead of its products.
-        const int two = t0 + 1 < t1, three = t0 + 2 < t1;
         fetch_k(t0);
-        if (two) fetch_k(t0 + 1);
+        fetch_k(t0 + 1);
         fetch_v(t0);
-        if (three) fetch_k(t0 + 2);
-        vm_wait_stages<T::DMAS>(1 + two + three);  // K of the first step has landed
+        fetch_k(t0 + 2);
+        vm_wait_stages<T::DMAS>(3);  // K of the first step has landed
+        // q has landed as well; said here, or the compiler waits for it in the
+        // loop, and with it for the DMAs just issued.
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
         bare_barrier();
-        scores(t0, s);
-        hide(t0, s);
-        raise(maximum(s));
+        auto next_scores = [&](int t) {
+            scores(t);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!seen_whole(reach, steps.key(t))) hide(t);
+            raise(maximum());
+        };
+        next_scores(t0);
         for (int t = t0; t < t1; ++t) {
             // K of step t + 1 and V of step t have landed (K of step t + 2,
-            // issued after them, may not have), and every wave is through with
-            // the slots that the next DMAs fill.
-            vm_wait_stages<T::DMAS>(t + 2 < t1);
+            // fetched behind them, may not have), and every wave is through
+            // with the slots that the next DMAs fill.
+            vm_wait_stages<T::DMAS>(1);
             if (!seen_whole(block, steps.key(t))) tame(t);
             lds_wait();
             bare_barrier();
-            if (t + 1 < t1) fetch_v(t + 1);
-            if (t + 3 < t1) fetch_k(t + 3);
-            f32x16 nx[2];
-            const bool more = t + 1 < t1;
-            if (more) scores(t + 1, nx);
-            u32x4 w[4];
-            weigh(s, w);
+            fetch_v(t + 1);
+            fetch_k(t + 3);
+            weigh();
             __builtin_amdgcn_sched_barrier(0);
-            products(t, w);
-            if (more) {
-                s[0] = nx[0];
-                s[1] = nx[1];
-                hide(t + 1, s);
-                raise(maximum(s));
-            }
+            products(t);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < t1) next_scores(t + 1);
         }
-        int* flags = reinterpret_cast<int*>(lds);
+        vm_wait_stages<T::DMAS>(0);
+        // Behind the wave's output rows below.
+        int* flags = reinterpret_cast<int*>(lds + tile_lds_bytes<D>() - 64);
         __syncthreads();
         if (lane == 0) flags[wave] = any_odd;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) any_odd = any_odd || flags[w];
+        for (int w = 0; w < kTileWaves; ++w) any_odd = any_odd || flags[w];
         if (any_odd) {  // the infinities and NaNs left out above: rare, so key by key
 #pragma unroll 1
             for (int t = t0; t < t1; ++t) {
@@ -364,7 +387,7 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
                             const uint32_t y[4] = {x.x << 16, x.x & 0xffff0000u, x.y << 16, x.y & 0xffff0000u};
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                o[d][e + k] += ok && (y[k] & 0x7f800000u) == 0x7f800000u ? __uint_as_float(y[k]) : 0.0f;
+                                o[d][e + k] += ok ? odd_or_zero(y[k]) : 0.0f;
                         }
                 }
             }
@@ -380,29 +403,48 @@ __global__ void __launch_bounds__(64 * W, 8 / W) attn_tile_kernel(AttnParams p) 
         L = 0.0f;
         m = kNegInf;
     }
-    if (my_row >= task.rows) return;
+    const bool live = my_row < task.rows;
     const int64_t at = (int64_t)mine.b * p.R + mine.r;
     const int64_t g = ((int64_t)mine.b * p.kv_heads + task.h) * p.RG + (int64_t)mine.r * p.G + (mine.head - task.h * p.G);
-    const float inv = L == 0.0f ? 0.0f : last ? 1.0f / L : 1.0f;
-    if (g2 == 0) {
+    const bool none = L == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / L;
+    if (live && g2 == 0) {
         if (!last) p.ml[(int64_t)task.part * all_rows + g] = make_float2(m, L);
-        if (last && p.lse) p.lse[at * p.heads + mine.head] = L == 0.0f ? kNegInf : m * p.scale + logf(L);
+        if (last && p.lse) p.lse[at * p.heads + mine.head] = none ? kNegInf : m * p.scale + logf(L);
         if (last && p.stat) p.stat[g] = make_float2(m == kNegInf ? 0.0f : m, inv);
     }
+    if (!last) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                if (live)
+                    *reinterpret_cast<f32x4*>(p.part + ((int64_t)task.part * all_rows + g) * D + 32 * d + 2 * e + 4 * g2) =
+                        none ? f32x4{0, 0, 0, 0} : f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+        return;
+    }
+    // Through LDS, so that a store covers whole rows of a head instead of 16
+    // bytes of 32 rows.
+    constexpr int ROW = D * 2 + 16;
+    unsigned char* mine_lds = lds + wave * 32 * ROW;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            f32x4 y;
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<uint2*>(mine_lds + n32 * ROW + (32 * d + 2 * e + 4 * g2) * 2) =
+                none ? make_uint2(0u, 0u)
+                     : make_uint2(pack_bf16(o[d][e] * inv, o[d][e + 1] * inv), pack_bf16(o[d][e + 2] * inv, o[d][e + 3] * inv));
+    lds_wait();
+    const int64_t to = live ? at * p.out_row + (int64_t)mine.head * D : -1;
+    constexpr int CH = T::CH;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = L == 0.0f ? 0.0f : o[d][e + k] * inv;
-            const int col = 32 * d + 2 * e + 4 * g2;
-            if (last)
-                *reinterpret_cast<uint2*>(p.out + at * p.out_row + (int64_t)mine.head * D + col) =
-                    make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-            else
-                *reinterpret_cast<f32x4*>(p.part + ((int64_t)task.part * all_rows + g) * D + col) = y;
-        }
+    for (int i = 0; i < 32 * CH / 64; ++i) {
+        const int row = i * (64 / CH) + lane / CH;
+        const int lo = __shfl((int)to, row), up = __shfl((int)(to >> 32), row);
+        const int64_t off = ((int64_t)up << 32) | (uint32_t)lo;
+        const u32x4 y = *reinterpret_cast<const u32x4*>(mine_lds + row * ROW + (lane % CH) * 16);
+        if (off >= 0) *reinterpret_cast<u32x4*>(p.out + off + 8 * (lane % CH)) = y;
+    }
 }
 
 }  // namespace krk

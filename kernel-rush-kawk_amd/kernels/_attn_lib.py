@@ -7,6 +7,7 @@ struct layouts, and has no fallback: a missing library is an ImportError.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -76,14 +77,15 @@ class AttnPlan(ctypes.Structure):
 
 _ptr = ctypes.POINTER
 
-#: Every function the header declares, with (restype, argtypes).
+#: Every function the header declares, with (restype, argtypes).  The calls of
+#: a step take their structs as packed bytes (:data:`PACK`) or by reference.
 SIGNATURES = {
-    "krk_attn_bf16": (_int, [_ptr(AttnShape), _ptr(AttnArgs), _p, _size, _p]),
+    "krk_attn_bf16": (_int, [_p, _p, _p, _size, _p]),
     "krk_attn_workspace_bytes": (_size, [_ptr(AttnShape)]),
     "krk_attn_check": (_int, [_ptr(AttnShape)]),
     "krk_attn_plan": (_int, [_ptr(AttnShape), _ptr(AttnPlan)]),
-    "krk_qk_norm_rope_bf16": (_int, [_ptr(RopeArgs), _p]),
-    "krk_cache_evict_bf16": (_int, [_ptr(EvictArgs), _p]),
+    "krk_qk_norm_rope_bf16": (_int, [_p, _p]),
+    "krk_cache_evict_bf16": (_int, [_p, _p]),
     "krk_attn_abi_version": (_int, []),
     "krk_attn_struct_size": (_size, [_int]),
     "krk_attn_last_error": (ctypes.c_char_p, []),
@@ -92,6 +94,24 @@ SIGNATURES = {
 #: The ABI this binding was written against (KRK_ATTN_ABI_VERSION) and its structs, in the header's order.
 ABI_VERSION = 1
 STRUCTS = (AttnShape, AttnArgs, RopeArgs, EvictArgs, AttnPlan)
+
+_CODES = {_p: "P", _i64: "q", _int: "i", _f: "f"}
+
+
+def _packer(cls) -> struct.Struct:
+    """The struct's layout for ``pack``: its fields in order, nested caches
+    flattened.  One call fills it, where setting a ctypes field costs as much
+    as reading a tensor's pointer."""
+    fmt = ""
+    for _, t in cls._fields_:
+        fmt += "".join(_CODES[u] for _, u in t._fields_) if t is Cache else _CODES[t]
+    s = struct.Struct("@" + fmt + "0P")
+    if s.size != ctypes.sizeof(cls):
+        raise ImportError(f"{cls.__name__}: packed {s.size} bytes, laid out {ctypes.sizeof(cls)}")
+    return s
+
+
+PACK = {cls: _packer(cls).pack for cls in (AttnArgs, RopeArgs, EvictArgs)}
 
 _lib = None
 _lock = threading.Lock()

@@ -31,18 +31,28 @@ import ctypes
 import torch
 
 from . import _attn_lib as _lib
-from ._attn_lib import AttnArgs, AttnPlan, AttnShape, Cache, EvictArgs, RopeArgs
+from ._attn_lib import AttnArgs, AttnPlan, AttnShape, EvictArgs, RopeArgs
 
 __all__ = ["CacheAttention", "CacheEviction", "qk_norm_rope", "rope_table"]
 
 _BF16 = torch.bfloat16
 _byref = ctypes.byref
+_PACK_ATTN, _PACK_ROPE, _PACK_EVICT = (_lib.PACK[t] for t in (AttnArgs, RopeArgs, EvictArgs))
+
+
+# One eager call of a decode step's operators is bound by the host (their
+# kernels take 3-10 us at one row): each property of an operand is read once,
+# in one expression that a good operand passes, and only one that fails it is
+# looked at again for the message.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
+_NO_CACHE = (0, 0, 0, 0)
 
 
 def _launch(fn, index: int, *args) -> None:
     """``fn(*args, stream)`` on GPU ``index`` and torch's current stream there."""
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
+    stream = _raw_stream(index)
+    if _current() == index:
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
@@ -51,62 +61,69 @@ def _launch(fn, index: int, *args) -> None:
         _lib.check(rc)
 
 
-def _on(index: int, name: str, t: torch.Tensor) -> None:
+def _index(name: str, t: torch.Tensor) -> int:
+    """The GPU that a call's first operand is on."""
+    if isinstance(t, torch.Tensor):
+        index = t.get_device()
+        if index >= 0 and t.is_cuda:
+            return index
+        raise ValueError(f"{name} must be a GPU tensor, got device {t.device}")
+    raise ValueError(f"{name} must be a torch.Tensor")
+
+
+def _refuse(name: str, t, index: int, dtype: torch.dtype, shape: tuple, layout: str):
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a torch.Tensor")
     if t.get_device() != index or not t.is_cuda:
         raise ValueError(f"{name} must be on the operands' GPU, got {t.device}")
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    raise ValueError(f"{name}: {layout}, got strides {t.stride()}")
 
 
-def _index(name: str, t: torch.Tensor) -> int:
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a GPU tensor, got device {t.device}")
-    return t.get_device()
+def _cache(name: str, t: torch.Tensor, index: int, shape: tuple) -> tuple:
+    """The fields of ``krk_cache`` for a [sequences, slots, kv_heads, head_dim] tensor."""
+    if isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.shape == shape and t.get_device() == index:
+        seq, slot, head, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), seq, slot, head
+    _refuse(name, t, index, _BF16, shape, "the elements of a head must be contiguous")
 
 
-def _cache(name: str, t: torch.Tensor, index: int, B: int | None, slots: int | None, kv_heads: int, dim: int) -> tuple:
-    """The fields of ``krk_cache`` for a [B, slots, kv_heads, dim] tensor (B
-    None: a [slots, kv_heads, dim] one), checked."""
-    _on(index, name, t)
-    want = (slots, kv_heads, dim) if B is None else (B, slots, kv_heads, dim)
-    if t.dtype is not _BF16 or t.dim() != len(want) or any(w is not None and s != w for s, w in zip(t.shape, want)):
-        raise ValueError(f"{name} must be bfloat16 of shape {want}, got {t.dtype} {tuple(t.shape)}")
-    st = t.stride()
-    if st[-1] != 1:
-        raise ValueError(f"{name}: the elements of a head must be contiguous, got strides {st}")
-    return (t.data_ptr(), 0, *st[:2]) if B is None else (t.data_ptr(), *st[:3])
+def _prefix(name: str, t: torch.Tensor, index: int, shape: tuple) -> tuple:
+    """The same for a [keys, kv_heads, head_dim] tensor."""
+    if isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.shape == shape and t.get_device() == index:
+        slot, head, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), 0, slot, head
+    _refuse(name, t, index, _BF16, shape, "the elements of a head must be contiguous")
 
 
-def _rows(name: str, t: torch.Tensor, index: int, rows: int, cols: int) -> tuple:
-    _on(index, name, t)
-    if t.dtype is not _BF16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name} must be bfloat16 of shape ({rows}, {cols}), got {t.dtype} {tuple(t.shape)}")
-    row, one = t.stride()
-    if one != 1 and cols > 1:
-        raise ValueError(f"{name} rows must be contiguous (stride(1) == 1), got strides {t.stride()}")
-    return t.data_ptr(), row if rows > 1 else max(row, cols)
+def _rows(name: str, t: torch.Tensor, index: int, shape: tuple) -> tuple:
+    """Address and row stride of a [rows, columns] bf16 tensor."""
+    if isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.shape == shape and t.get_device() == index:
+        row, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), row
+    _refuse(name, t, index, _BF16, shape, "rows must be contiguous")
 
 
 def _plain(name: str, t: torch.Tensor, index: int, dtype: torch.dtype, shape: tuple) -> int:
     """The address of a contiguous tensor of this type and shape."""
-    _on(index, name, t)
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.data_ptr()
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == index
+            and t.is_contiguous()):
+        return t.data_ptr()
+    _refuse(name, t, index, dtype, shape, "it must be contiguous")
 
 
-def _scores(name: str, t: torch.Tensor, index: int, B: int, kv_heads: int, slots: int, more: bool = False) -> tuple:
-    _on(index, name, t)
-    if (t.dtype is not torch.float32 or t.dim() != 3 or t.shape[:2] != (B, kv_heads)
-            or not (t.shape[2] == slots or more and t.shape[2] > slots)):
-        raise ValueError(f"{name} must be float32 of shape ({B}, {kv_heads}, {slots}), got {t.dtype} {tuple(t.shape)}")
-    seq, head, one = t.stride()
-    if one != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name}: the scores of a head must be contiguous, got strides {t.stride()}")
-    return t.data_ptr(), seq, head
+def _scores(name: str, t: torch.Tensor, index: int, shape: tuple, more: bool = False) -> tuple:
+    """Address and strides of [sequences, heads, slots] scores (``more``: or more slots)."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == index and t.dim() == 3:
+        if t.shape == shape or more and t.shape[:2] == shape[:2] and t.shape[2] > shape[2]:
+            seq, head, one = t.stride()
+            if one == 1 or t.shape[2] == 1:
+                return t.data_ptr(), seq, head
+    _refuse(name, t, index, torch.float32, shape, "the scores of a head must be contiguous")
 
 
 def rope_table(positions: int, head_dim: int, theta: float, device) -> torch.Tensor:
@@ -141,36 +158,31 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.T
     index = _index("qkv", qkv)
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a [B, capacity, kv_heads, head_dim] tensor")
-    B, cap, KV, D = k.shape
+    if not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise ValueError("table must be a [positions, head_dim] tensor")
+    shape = k.shape
+    B, cap, KV, D = shape
     if qkv.dim() != 2 or B < 1 or D < 1 or qkv.shape[0] < 1 or qkv.shape[0] % B or qkv.shape[1] % D:
-        raise ValueError(f"qkv must be [B * R, (heads + 2 * kv_heads) * head_dim] for a cache of shape {tuple(k.shape)}, "
+        raise ValueError(f"qkv must be [B * R, (heads + 2 * kv_heads) * head_dim] for a cache of shape {tuple(shape)}, "
                          f"got {tuple(qkv.shape)}")
     M, cols = qkv.shape
     heads = cols // D - 2 * KV
     if heads < 1:
         raise ValueError(f"qkv of {cols} columns has no q heads beside {KV} k and {KV} v heads of {D}")
-    a = RopeArgs()
-    a.qkv, a.qkv_row = _rows("qkv", qkv, index, M, cols)
-    a.k = _cache("k", k, index, B, cap, KV, D)
-    a.v = _cache("v", v, index, B, cap, KV, D)
-    if q_norm is not None:
-        a.q_norm = _plain("q_norm", q_norm, index, _BF16, (D,))
-    if k_norm is not None:
-        a.k_norm = _plain("k_norm", k_norm, index, _BF16, (D,))
-    a.eps = eps
-    if not isinstance(table, torch.Tensor) or table.dim() != 2:
-        raise ValueError("table must be a [positions, head_dim] tensor")
-    a.table, a.table_rows = _plain("table", table, index, torch.float32, (table.shape[0], D)), table.shape[0]
-    a.lens = _plain("lens", lens, index, torch.int32, (B,))
-    if positions is not None:
-        a.positions = _plain("positions", positions, index, torch.int32, (M,))
     if q_out is None:
-        q_out = torch.empty((M, heads * D), dtype=_BF16, device=qkv.device)
-    a.q_out, a.q_row = _rows("q_out", q_out, index, M, heads * D)
-    if M == 1 and a.q_out == a.qkv:
-        a.q_row = a.qkv_row  # one row in place: its stride is of no matter
-    a.B, a.R, a.heads, a.kv_heads, a.head_dim, a.capacity = B, M // B, heads, KV, D, cap
-    _launch(_lib.load().krk_qk_norm_rope_bf16, index, _byref(a))
+        q_out = qkv.new_empty((M, heads * D))
+    x, x_row = _rows("qkv", qkv, index, (M, cols))
+    q, q_row = _rows("q_out", q_out, index, (M, heads * D))
+    n = table.shape[0]
+    args = _PACK_ROPE(
+        x, x_row,
+        0 if q_norm is None else _plain("q_norm", q_norm, index, _BF16, (D,)),
+        0 if k_norm is None else _plain("k_norm", k_norm, index, _BF16, (D,)),
+        eps, _plain("table", table, index, torch.float32, (n, D)), n,
+        0 if positions is None else _plain("positions", positions, index, torch.int32, (M,)),
+        _plain("lens", lens, index, torch.int32, (B,)), q, q_row,
+        *_cache("k", k, index, shape), *_cache("v", v, index, shape), B, M // B, heads, KV, D, cap)
+    _launch(_lib.load().krk_qk_norm_rope_bf16, index, args)
     return q_out
 
 
@@ -198,7 +210,9 @@ class CacheAttention:
         lib = _lib.load()
         _lib.check(lib.krk_attn_check(_byref(self._shape)))
         nbytes = int(lib.krk_attn_workspace_bytes(_byref(self._shape)))
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        self._q_shape = (B * R, heads * head_dim)
+        self._cache_shape = (B, capacity, kv_heads, head_dim)
+        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
 
     @property
     def plan(self) -> dict:
@@ -213,15 +227,10 @@ class CacheAttention:
         """Allocation-free form: write into ``out`` (``[B * R, heads *
         head_dim]``), and with ``lse`` (``[B * R, heads]`` fp32) the log of each
         softmax's sum."""
-        B, M, KV, D, cap = self.B, self.B * self.R, self.kv_heads, self.head_dim, self.capacity
         index = _index("q", q)
-        a = AttnArgs()
-        a.q, a.q_row = _rows("q", q, index, M, self.heads * D)
-        a.out, a.out_row = _rows("out", out, index, M, self.heads * D)
-        a.k = _cache("k", k, index, B, cap, KV, D)
-        a.v = _cache("v", v, index, B, cap, KV, D)
-        a.lens = _plain("lens", lens, index, torch.int32, (B,))
-        a.scale = self.scale
+        B, shape = self.B, self._cache_shape
+        kp = vp = _NO_CACHE
+        n = 0
         if prefix is not None:
             kp, vp = prefix
             if not isinstance(kp, torch.Tensor) or kp.dim() != 3:
@@ -229,33 +238,31 @@ class CacheAttention:
             n = kp.shape[0]
             if n > self.prefix:
                 raise ValueError(f"a prefix of {n} keys; this object was built for up to {self.prefix}")
-            if n:
-                a.kp = _cache("prefix k", kp, index, None, n, KV, D)
-            _on(index, "prefix v", vp)
-            if n or vp.shape != kp.shape:
-                a.vp = _cache("prefix v", vp, index, None, n, KV, D)
-            a.prefix = n
-        if tree is not None:
-            a.tree = _plain("tree", tree, index, torch.int64, (B, self.R))
-        if lse is not None:
-            a.lse = _plain("lse", lse, index, torch.float32, (M, self.heads))
+            run = (n, self.kv_heads, self.head_dim)
+            kp, vp = _prefix("prefix k", kp, index, run), _prefix("prefix v", vp, index, run)
+        sc = so = (0, 0, 0)
         if self.scored:
             if scores is None:
                 raise ValueError("this object updates scores: give scores=")
-            a.scores, a.sc_seq, a.sc_head = _scores("scores", scores, index, B, KV, cap)
-            if scores_out is None:
-                a.scores_out, a.so_seq, a.so_head = a.scores, a.sc_seq, a.sc_head
-            else:
-                a.scores_out, a.so_seq, a.so_head = _scores("scores_out", scores_out, index, B, KV, cap)
+            run = (B, self.kv_heads, self.capacity)
+            sc = so = _scores("scores", scores, index, run)
+            if scores_out is not None:
+                so = _scores("scores_out", scores_out, index, run)
         elif scores is not None or scores_out is not None:
             raise ValueError("scores are kept by objects built with scored=True")
+        args = _PACK_ATTN(
+            *_rows("q", q, index, self._q_shape), *_cache("k", k, index, shape), *_cache("v", v, index, shape),
+            *kp, *vp, n, self.scale, _plain("lens", lens, index, torch.int32, (B,)),
+            0 if tree is None else _plain("tree", tree, index, torch.int64, (B, self.R)),
+            *_rows("out", out, index, self._q_shape),
+            0 if lse is None else _plain("lse", lse, index, torch.float32, (B * self.R, self.heads)), *sc, *so)
         ws = self.workspace
         if ws is None:
-            _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), _byref(a), 0, 0)
+            _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), args, 0, 0)
+        elif ws.get_device() == index:
+            _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), args, ws.data_ptr(), ws.numel())
         else:
-            if ws.get_device() != index:
-                raise ValueError(f"operands on {q.device}; this object was built on {self.device}")
-            _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), _byref(a), ws.data_ptr(), ws.numel())
+            raise ValueError(f"operands on {q.device}; this object was built on {self.device}")
         return out
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, *,
@@ -273,7 +280,7 @@ class CacheAttention:
         rows and the query heads of its group, is added; into ``scores_out``
         where given (slots below ``lens``)."""
         _index("q", q)
-        out = torch.empty((self.B * self.R, self.heads * self.head_dim), dtype=_BF16, device=q.device)
+        out = torch.empty(self._q_shape, dtype=_BF16, device=q.device)
         return self.run(q, k, v, lens, out, prefix=prefix, tree=tree, scores=scores, scores_out=scores_out, lse=lse)
 
 
@@ -306,36 +313,31 @@ class CacheEviction:
         ``lens_out`` (which may be ``lens``).  ``out=(k, v, scores)`` receives the
         kept rows (at least ``budget`` slots each; what lies behind them is left
         as it was); without it the cache is compacted in place."""
-        B, KV, D, cap = self.B, self.kv_heads, self.head_dim, self.capacity
         index = _index("k", k)
-        a = EvictArgs()
-        a.k = _cache("k", k, index, B, cap, KV, D)
-        a.v = _cache("v", v, index, B, cap, KV, D)
-        a.scores, a.sc_seq, a.sc_head = _scores("scores", scores, index, B, KV, cap)
+        B, KV, D, cap, n = self.B, self.kv_heads, self.head_dim, self.capacity, self.budget
+        shape, run = (B, cap, KV, D), (B, KV, cap)
+        kc, vc, sc = _cache("k", k, index, shape), _cache("v", v, index, shape), _scores("scores", scores, index, run)
         if out is None:
-            a.k_out, a.v_out = a.k, a.v
-            a.scores_out, a.so_seq, a.so_head = a.scores, a.sc_seq, a.sc_head
+            ko, vo, so = kc, vc, sc
         else:
             ko, vo, so = out
-            a.k_out = _cache("out k", ko, index, B, None, KV, D)
-            a.v_out = _cache("out v", vo, index, B, None, KV, D)
-            if min(ko.shape[1], vo.shape[1]) < self.budget:
-                raise ValueError(f"out k and v must have at least {self.budget} slots, got {ko.shape[1]} and {vo.shape[1]}")
-            a.scores_out, a.so_seq, a.so_head = _scores("out scores", so, index, B, KV, self.budget, more=True)
-        a.lens = _plain("lens", lens, index, torch.int32, (B,))
-        a.lens_out = _plain("lens_out", lens_out, index, torch.int32, (B,))
-        a.keep = _plain("keep", keep, index, torch.int32, (B, KV, self.budget))
-        a.B, a.kv_heads, a.head_dim, a.capacity = B, KV, D, cap
-        a.budget, a.sinks, a.recent = self.budget, self.sinks, self.recent
-        _launch(_lib.load().krk_cache_evict_bf16, index, _byref(a))
+            for name, t in (("out k", ko), ("out v", vo)):
+                if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[1] < n:
+                    raise ValueError(f"{name} must be a [{B}, {n} or more, {KV}, {D}] tensor")
+            ko = _cache("out k", ko, index, (B, ko.shape[1], KV, D))
+            vo = _cache("out v", vo, index, (B, vo.shape[1], KV, D))
+            so = _scores("out scores", so, index, (B, KV, n), more=True)
+        args = _PACK_EVICT(
+            *kc, *vc, *ko, *vo, *sc, *so, _plain("lens", lens, index, torch.int32, (B,)),
+            _plain("lens_out", lens_out, index, torch.int32, (B,)), _plain("keep", keep, index, torch.int32, (B, KV, n)),
+            B, KV, D, cap, n, self.sinks, self.recent)
+        _launch(_lib.load().krk_cache_evict_bf16, index, args)
         return keep
 
     def __call__(self, k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor, lens: torch.Tensor,
                  out: tuple | None = None) -> tuple:
         """``(keep, new lens)`` as new tensors (:meth:`run`)."""
-        _index("k", k)
-        dev = k.device
-        keep = torch.empty((self.B, self.kv_heads, self.budget), dtype=torch.int32, device=dev)
-        lens_out = torch.empty((self.B,), dtype=torch.int32, device=dev)
+        _index("lens", lens)
+        keep, lens_out = lens.new_empty((self.B, self.kv_heads, self.budget)), lens.new_empty((self.B,))
         self.run(k, v, scores, lens, keep, lens_out, out)
         return keep, lens_out

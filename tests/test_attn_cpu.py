@@ -158,8 +158,10 @@ def test_plans_cover_the_rows_and_fit_the_workspace(lib, R):
                     rows = B * R * heads
                     n = p.splits + p.prefix_splits
                     need = (n * rows * (4 * D + 8) if n > 1 else 0) + (8 * rows if s.scored else 0)
+                    if s.scored and p.rows == 16 and not s.window:
+                        need += 4 * rows * (-(-cap // 32) * 32)  # kept q.k
                     got = lib.krk_attn_workspace_bytes(ctypes.byref(s))
-                    assert need <= got <= need + 4096
+                    assert need <= got <= need + 4 * B * kv + 8192
 
 
 def _t(*s, dtype=BF):

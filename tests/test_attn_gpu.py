@@ -64,7 +64,7 @@ def close(got, ref, tol, what):
 
 
 def weight_half(op):
-    """Relative rounding of the weights: one bf16 part in workgroups of 128 rows or more, else two."""
+    """Relative rounding of the weights: one bf16 part in workgroups of 128 rows, else two."""
     return 2.0 ** -8 if max(op.plan["rows"], op.plan["prefix_rows"]) >= 128 else 2.0 ** -16
 
 
