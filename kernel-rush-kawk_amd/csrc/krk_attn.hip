@@ -171,12 +171,17 @@ Plan make_plan(const krk_attn_shape& s) {
         const int64_t near = (int64_t)s.window + s.sinks + s.R + 64;
         keys = near < keys ? near : keys;
     }
-    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, keys == s.capacity);
     if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, false);
+    // In one launch with the prefix's, the own caches' workgroups have half of
+    // the chip's places.
+    const bool alone = p.prefix.rows == 0 || p.prefix.rows == krk::kTileRows;
+    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, alone && keys == s.capacity);
     const int n = p.own.splits + p.prefix.splits;
     if (n > 1) {
         // One workgroup joins a sequence's head: up to 96 KB of partial results.
-        p.join_in_kernel = p.own.rows <= 32 && p.prefix.rows <= 32 && RG * n * s.head_dim <= 24 << 10;
+        // Not behind a prefix: the workgroup that finishes its last range would
+        // join all sequences of its rows, one after the other (8 of them, 8 us).
+        p.join_in_kernel = p.own.rows <= 32 && !s.prefix && RG * n * s.head_dim <= 24 << 10;
         if (p.join_in_kernel) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
         p.part = align_up((size_t)n * p.all_rows * s.head_dim * sizeof(float), 256);
         p.ml = align_up((size_t)n * p.all_rows * sizeof(float2), 256);
@@ -206,10 +211,10 @@ template <int D>
 int launch_tile(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
     const void* fn = reinterpret_cast<const void*>(&krk::attn_tile_kernel<D>);
-    const size_t shm = krk::tile_lds_bytes<D>();
-    if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "attn_tile_kernel LDS size");
+    const size_t lds = krk::tile_lds_bytes<D>();
+    if (hipError_t e = ensure_lds_limit(fn, lds, done)) return hip_status(e, "attn_tile_kernel LDS size");
     void* args[] = {(void*)&p};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(krk::kTileThreads), args, shm, stream), "attn_tile_kernel launch");
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(krk::kTileThreads), args, lds, stream), "attn_tile_kernel launch");
 }
 
 template <int D>
@@ -217,26 +222,24 @@ int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
     const int64_t own = (int64_t)plan.own.tiles * p.kv_heads * p.B * plan.own.splits;
     const int64_t shared = (int64_t)plan.prefix.tiles * p.kv_heads * plan.prefix.splits;
     void* args[] = {(void*)&p};
-    if (plan.own.rows <= 32 && plan.prefix.rows <= 32) {  // one launch
-        int rc;
-        if (plan.own.rows == 32) rc = launch_split<D, 2, 2>(p, own + shared, stream);
-        else if (plan.prefix.rows == 32) rc = launch_split<D, 1, 2>(p, own + shared, stream);
-        else rc = launch_split<D, 1, 1>(p, own + shared, stream);
-        if (rc) return rc;
-    } else {
-        if (shared) {
-            if (int rc = launch_tile<D>(p, shared, stream)) return rc;
-        }
+    int rc;
+    if (plan.own.rows == krk::kTileRows) {
+        rc = launch_tile<D>(p, own + shared, stream);
+    } else if (plan.prefix.rows == krk::kTileRows) {
+        // Two launches: one of both kinds of workgroups was no faster (they
+        // share CUs at the register and LDS cost of the larger kind).
+        rc = launch_tile<D>(p, shared, stream);
         krk::AttnParams o = p;
-        o.prefix_row_tiles = 0;  // the own caches' workgroups alone
-        int rc;
-        switch (plan.own.rows) {
-            case 16: rc = launch_split<D, 1, 1>(o, own, stream); break;
-            case 32: rc = launch_split<D, 2, 2>(o, own, stream); break;
-            default: rc = launch_tile<D>(o, own, stream);
-        }
-        if (rc) return rc;
+        o.prefix_row_tiles = 0;
+        if (!rc) rc = plan.own.rows == 32 ? launch_split<D, 2, 2>(o, own, stream) : launch_split<D, 1, 1>(o, own, stream);
+    } else if (plan.own.rows == 32) {
+        rc = launch_split<D, 2, 2>(p, own + shared, stream);
+    } else if (plan.prefix.rows == 32) {
+        rc = launch_split<D, 1, 2>(p, own + shared, stream);
+    } else {
+        rc = launch_split<D, 1, 1>(p, own + shared, stream);
     }
+    if (rc) return rc;
     if (plan.own.splits + plan.prefix.splits > 1 && !plan.join_in_kernel) {
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_join_kernel<D>),
                                              dim3((unsigned)cdiv(plan.all_rows, 256 / (D / 4) / krk::kGroups)), dim3(256), args, 0, stream);
@@ -252,6 +255,15 @@ int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
         if (int rc = hip_status(e, "attn_weights_kernel launch")) return rc;
     }
     return KRK_ATTN_OK;
+}
+
+// By how many keys a lane holds: time and code grow with it (1024 slots on the
+// 36-key kernel: 13.7 us, on the 4-key one 7).
+const void* select_kernel(int capacity) {
+    if (capacity <= 4 * krk::kEvictThreads) return reinterpret_cast<const void*>(&krk::evict_select_kernel<4>);
+    if (capacity <= 12 * krk::kEvictThreads) return reinterpret_cast<const void*>(&krk::evict_select_kernel<12>);
+    if (capacity <= 36 * krk::kEvictThreads) return reinterpret_cast<const void*>(&krk::evict_select_kernel<36>);
+    return reinterpret_cast<const void*>(&krk::evict_select_kernel<0>);
 }
 
 krk::CacheView view(const krk_cache& c) { return {static_cast<const uint16_t*>(c.p), c.seq, c.slot, c.head}; }
@@ -481,10 +493,10 @@ int krk_cache_evict_bf16(const krk_evict_args* args, void* stream) {
                        a.B, a.kv_heads, a.capacity, a.budget, a.sinks, a.recent};
     hipStream_t st = static_cast<hipStream_t>(stream);
     void* kargs[] = {(void*)&p};
-    hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::evict_select_kernel), dim3(a.kv_heads, a.B),
-                                   dim3(krk::kEvictThreads), kargs, 0, st);
-    if (int rc = hip_status(e, "evict_select_kernel launch")) return rc;
     const bool wide = a.head_dim == 128;
+    const void* select = select_kernel(a.capacity);
+    hipError_t e = hipLaunchKernel(select, dim3(a.kv_heads, a.B), dim3(krk::kEvictThreads), kargs, 0, st);
+    if (int rc = hip_status(e, "evict_select_kernel launch")) return rc;
     const void* fn;
     dim3 grid;
     if (in_place) {

@@ -323,40 +323,29 @@ __device__ __forceinline__ void join_rows(const AttnParams& p, int b, int h, uns
 }
 
 // MTO 16-row tiles of a sequence's own rows per workgroup, MTP of the rows over
-// a shared prefix, in one launch.  Where partial results are joined here, the
-// workgroup that finishes last for a sequence and head does it: no second
-// launch (3 us and more between dependent kernels, and 2 us of host time).
+// a shared prefix, in one launch.  Where partial results are joined here (no
+// prefix), the workgroup that finishes last for a sequence and head does it: no
+// second launch (one decode row over 1000 keys: 13.3 us a call in two launches,
+// 9.1 in one).
 template <int D, int MTO, int MTP>
 __global__ void __launch_bounds__(kSplitThreads, 2) attn_split_kernel(AttnParams p) {
     extern __shared__ __align__(16) unsigned char lds[];
-    __shared__ int done[16 * (MTO > MTP ? MTO : MTP)];
+    __shared__ int last;
     const Task task = task_of(p, blockIdx.x, 16 * MTO, 16 * MTP);
     if (MTO == MTP || !task.shared) split_task<D, MTO>(p, task, lds);
     else split_task<D, MTP>(p, task, lds);
     if (!p.ctr) return;
-    const int TR = 16 * (task.shared ? MTP : MTO);
-    const int end = task.row0 + TR < task.rows ? task.row0 + TR : task.rows;
-    const int b_lo = task.shared ? task.row0 / p.RG : task.b0;
-    const int nb = task.shared ? (end - 1) / p.RG - b_lo + 1 : 1;
     drain_memory();
     __syncthreads();
-    if ((int)threadIdx.x < nb) {
-        const int b = b_lo + threadIdx.x;
-        uint32_t all = (uint32_t)(p.row_tiles * p.splits);
-        if (p.prefix_splits) {
-            const int t0 = b * p.RG / (16 * MTP), t1 = ((b + 1) * p.RG - 1) / (16 * MTP);
-            all += (uint32_t)((t1 - t0 + 1) * p.prefix_splits);
-        }
-        const uint32_t before = __hip_atomic_fetch_add(p.ctr + (int64_t)b * p.kv_heads + task.h, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        done[threadIdx.x] = before == all - 1;
+    uint32_t* ctr = p.ctr + (int64_t)task.b0 * p.kv_heads + task.h;
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = before == (uint32_t)(p.row_tiles * p.splits) - 1;
     }
     __syncthreads();
-    for (int i = 0; i < nb; ++i) {
-        if (!done[i]) continue;
-        join_rows<D>(p, b_lo + i, task.h, lds);
-        if (threadIdx.x == 0)
-            __hip_atomic_store(p.ctr + (int64_t)(b_lo + i) * p.kv_heads + task.h, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if (!last) return;
+    join_rows<D>(p, task.b0, task.h, lds);
+    if (threadIdx.x == 0) __hip_atomic_store(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Joins the key ranges in a launch of its own: D / 4 threads a row and group
@@ -410,45 +399,93 @@ __global__ void __launch_bounds__(256) attn_weights_raw_kernel(AttnParams p) {
         if (key + e < len) to[e] = was[e] + w[e];
 }
 
-// Adds the keys' weights to their scores: a wave per 32 keys of a sequence
-// and head, over all R * G rows; no atomics, rows in order.
+// Adds the keys' weights to their scores where q.k was not kept: a wave per 32
+// keys of a sequence and head, whose K stays in registers, over all R * G rows
+// in order (no atomics).  The rows come 32 at a time through LDS, shared by the
+// four waves, the next 32 loading meanwhile.  Bound by reading K once more and
+// by the weights themselves (20 VALU cycles a wave and 64 of them).
+constexpr int kWeightRows = 32;
 template <int D>
-__global__ void __launch_bounds__(256) attn_weights_kernel(AttnParams p) {
+__global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
     constexpr int KS = D / 32;
+    constexpr int LDQ = D * 2 + 16;  // bytes of a row in LDS: rows 4 banks apart
+    constexpr int CH = D / 8, PARTS = kWeightRows * CH / 256;
+    __shared__ __align__(16) unsigned char lq[kWeightRows * LDQ];
+    __shared__ float2 lst[kWeightRows];
     const int lane = threadIdx.x & 63;
     const int n16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.y, b = blockIdx.z;
     const int len = seq_len(p, b);
+    if (128 * (int)blockIdx.x >= len) return;  // the whole workgroup
     const int kb = 32 * ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
-    if (kb >= len) return;
+    const uint16_t* base = p.k.p + (int64_t)b * p.k.seq + (int64_t)h * p.k.head;
     KeyFrag<D> kf;
-    kf.load(p.k.p + (int64_t)b * p.k.seq + (int64_t)h * p.k.head, p.k.slot, kb, len, lane);
-    const float2* stat = p.stat + ((int64_t)b * p.kv_heads + h) * p.RG;
+    kf.load(base, p.k.slot, kb, len, lane);
+    // Which rows see what, from the first live row and the last.
+    const int live_from = len - p.R > 0 ? len - p.R : 0;  // position of the first row with a slot
+    const int hi_min = p.tree ? len - p.R - 1 : live_from;
+    const int lo_max = p.window && len > p.window ? len - p.window : 0;
+    const bool whole = kb + 32 <= len && kb + 31 <= hi_min && (kb >= lo_max || kb + 32 <= p.sinks);
+
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = 0.0f;
-    for (int row0 = 0; row0 < p.RG; row0 += 16) {
-        const int row = row0 + n16;
-        const int j = row < p.RG ? row : p.RG - 1;
-        const int r = j / p.G;
-        const RowSight sight = row_sight(p, b, r, len);
-        const uint16_t* qr = p.q + ((int64_t)b * p.R + r) * p.q_row + (int64_t)(h * p.G + (j - r * p.G)) * D + 8 * q4;
-        const float2 st = stat[j];
-        f32x4 s[2];
+    const float2* stat = p.stat + ((int64_t)b * p.kv_heads + h) * p.RG;
+    const uint16_t* qbase = p.q + (int64_t)b * p.R * p.q_row + (int64_t)h * p.G * D;
+    u32x4 part[PARTS];
+    float2 st;
+    auto fetch = [&](int row0) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const u32x4 qf = load_cached16(qr + 32 * ks);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) s[u] = mfma16(kf.f[u][ks], qf, s[u]);
+        for (int i = 0; i < PARTS; ++i) {
+            const int e = i * 256 + threadIdx.x;
+            int j = row0 + e / CH;
+            j = j < p.RG ? j : p.RG - 1;
+            const int r = j / p.G;
+            part[i] = load_cached16(qbase + (int64_t)r * p.q_row + (int64_t)(j - r * p.G) * D + 8 * (e % CH));
         }
-        const bool live = row < p.RG;
+        const int j = row0 + (int)threadIdx.x;  // the first 32 threads
+        // Behind the last row: exp2(-infinity) times 0.
+        st = j < p.RG && threadIdx.x < kWeightRows ? stat[j] : make_float2(__builtin_inff(), 0.0f);
+        st.x *= p.c;
+    };
+    fetch(0);
+    for (int row0 = 0; row0 < p.RG; row0 += kWeightRows) {
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int key = kb + 8 * q4 + e;
-            const float x = exp2_raw((s[e >> 2][e & 3] - st.x) * p.c) * st.y;
-            w[e] += live && key < len && sees(sight, key, p.sinks) ? x : 0.0f;
+        for (int i = 0; i < PARTS; ++i) {
+            const int e = i * 256 + threadIdx.x;
+            *reinterpret_cast<u32x4*>(lq + e / CH * LDQ + e % CH * 16) = part[i];
+        }
+        if (threadIdx.x < kWeightRows) lst[threadIdx.x] = st;
+        __syncthreads();
+        if (row0 + kWeightRows < p.RG) fetch(row0 + kWeightRows);
+        for (int i0 = 0; i0 < kWeightRows && row0 + i0 < p.RG; i0 += 16) {
+            f32x4 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 q = *reinterpret_cast<const u32x4*>(lq + (i0 + n16) * LDQ + 64 * ks + 16 * q4);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[u] = mfma16(kf.f[u][ks], q, s[u]);
+            }
+            const float2 now = lst[i0 + n16];
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    w[e] = __builtin_fmaf(exp2_raw(__builtin_fmaf(s[e >> 2][e & 3], p.c, -now.x)), now.y, w[e]);
+            } else {
+                const int j = row0 + i0 + n16;
+                const RowSight sight = row_sight(p, b, (j < p.RG ? j : p.RG - 1) / p.G, len);
+                // A row that sees nothing (or is none) adds nothing, whatever its q.
+                const bool adds = now.y != 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = kb + 8 * q4 + e;
+                    const float x = exp2_raw(__builtin_fmaf(s[e >> 2][e & 3], p.c, -now.x)) * now.y;
+                    w[e] += adds && key < len && sees(sight, key, p.sinks) ? x : 0.0f;
+                }
+            }
         }
     }
     // Sum over the 16 rows in the lanes; lane n16 = e of each group keeps key e.
@@ -456,8 +493,10 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(AttnParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         float x = w[e];
-#pragma unroll
-        for (int s = 1; s < 16; s <<= 1) x += __shfl_xor(x, s);
+        x += partner<8>(x);
+        x += partner<4>(x);
+        x += partner<2>(x);
+        x += partner<1>(x);
         mine = n16 == e ? x : mine;
     }
     const int key = kb + 8 * q4 + n16;

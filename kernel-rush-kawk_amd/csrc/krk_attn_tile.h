@@ -141,10 +141,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
     using T = TileKernel<D>;
     constexpr int KS = T::KS, DT = T::DT;
     extern __shared__ __align__(16) unsigned char lds[];
+    const Task task = task_of(p, blockIdx.x, kTileRows, kTileRows);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31, g2 = lane >> 5;
-    const Task task = task_of(p, blockIdx.x, kTileRows, kTileRows);
     const int limit = task.limit;
 
     const int my_row = task.row0 + wave * 32 + n32;

@@ -1,14 +1,17 @@
 // Cache eviction by accumulated attention weight (gfx950): which slots stay,
 // then the move.
 //
-// Selection: one workgroup per sequence and head.  The highest scores come
-// from a radix select (11 + 11 + 10 bits of an order-preserving key, a
-// histogram in LDS each), which reads the scores three times from L2, then two
-// passes over contiguous runs of slots per wave: one counts, one writes the
-// kept slots in order.  The histograms' integer atomics commute, so the result
-// does not depend on their order.
+// Selection: one workgroup per sequence and head; each wave has a run of slots
+// next to each other.  The highest scores come from a radix select (11 + 11 + 10
+// bits of an order-preserving key, histograms in LDS), then two passes, one to
+// count, one to write the kept slots in order.  Up to 36864 slots the keys stay
+// in registers and the scores are read once; a longer cache reads them for each
+// of the five passes.  The histograms' integer atomics commute, so the result
+// does not depend on their order.  Bound by latency, the LDS atomics and the
+// vector pipe of the B * kv_heads CUs that have a workgroup.
 //
-// Move: bound by reading and writing the kept rows once.  Slots keep their
+// Move: bound by reading and writing the kept rows once (a launch of its own:
+// copied by the selecting workgroup, 512 rows of 8 heads took 6 us instead of 3).  Slots keep their
 // order, so row i comes from a slot >= i.
 #pragma once
 
@@ -41,11 +44,19 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 
+// PER: keys a lane holds, for caches of up to 1024 * PER slots (code and time
+// grow with it); 0: none, any length.
+template <int PER>
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(EvictParams p) {
-    __shared__ uint32_t hist[2048];
+    // Few keys: one histogram.  Many: each quarter of the waves has its own, as
+    // heavy-tailed scores crowd into some 80 of the first digits.
+    constexpr int COPIES = PER > 0 && PER <= 4 ? 1 : 4;
+    __shared__ uint32_t hist[COPIES][2048];
     __shared__ uint32_t wave_sum[kEvictWaves];
+    __shared__ uint32_t counts[2][kEvictWaves];
     __shared__ uint32_t found[2];  // the digit, and how many are still wanted of it
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int h = blockIdx.x, b = blockIdx.y;
     int len = p.lens[b];
     len = len < 0 ? 0 : len > p.capacity ? p.capacity : len;
@@ -54,97 +65,115 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(EvictParams
         for (int i = t; i < p.budget; i += kEvictThreads) keep[i] = i < len ? i : -1;
         return;
     }
+    // The first and the last slots stay; those between them compete.
+    const int lo = p.sinks, hi = len - p.recent;
+    const int chosen = p.budget - p.sinks - p.recent;
+    for (int i = t; i < p.sinks; i += kEvictThreads) keep[i] = i;
+    for (int i = t; i < p.recent; i += kEvictThreads) keep[p.budget - p.recent + i] = hi + i;
+    if (chosen == 0) return;
+
     const float* sc = p.scores + (int64_t)b * p.sc_seq + (int64_t)h * p.sc_head;
-    const int lo = p.sinks, hi = len - p.recent;  // the slots that compete
-    uint32_t want = (uint32_t)(p.budget - p.sinks - p.recent);
-    uint32_t prefix = 0;  // the digits found so far, from the top
-    int shift = 32;
-    // After the loop `prefix` is the key of the last slot that stays, and
-    // `want` how many slots of exactly that key do.
-    if (want > 0) {
-        for (int pass = 0; pass < 3; ++pass) {
-            const int bits = pass < 2 ? 11 : 10;
-            const int above = shift;
-            shift -= bits;
-            for (int i = t; i < 2048; i += kEvictThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = lo + t; i < hi; i += kEvictThreads) {
-                const uint32_t key = score_key(sc[i]);
-                if (pass == 0 || (key >> above) == (prefix >> above))
-                    atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1)], 1u);
-            }
-            __syncthreads();
-            // Thread t holds digits 2047 - 2t and the one below it: a scan over
-            // threads counts from the largest digit down.
-            const uint32_t a = hist[2047 - 2 * t], c = hist[2046 - 2 * t];
-            uint32_t sum = a + c;
+    // This wave's run: slots w0 + 64 i + lane.  Keys of competing slots are at
+    // least 0x007fffff (-infinity's); 0 stands for a slot that does not compete.
+    const int rounds = (hi - lo + kEvictThreads - 1) / kEvictThreads;
+    const int w0 = lo + wave * rounds * 64 + lane;
+    auto key_of = [&](int s, float v) { return s < hi ? score_key(v) : 0u; };
+    uint32_t held[PER > 0 ? PER : 1];
+    if constexpr (PER > 0) {
+        float v[PER];
 #pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const uint32_t o = __shfl_up(sum, s);
-                if (lane >= s) sum += o;
-            }
-            if (lane == 63) wave_sum[wave] = sum;
-            __syncthreads();
-            uint32_t before = sum - a - c;
-            for (int w = 0; w < wave; ++w) before += wave_sum[w];
-            if (before < want && want <= before + a) {
-                found[0] = 2047 - 2 * t;
-                found[1] = want - before;
-            } else if (before + a < want && want <= before + a + c) {
-                found[0] = 2046 - 2 * t;
-                found[1] = want - before - a;
-            }
-            __syncthreads();
-            prefix |= found[0] << shift;
-            want = found[1];
-            __syncthreads();
+        for (int i = 0; i < PER; ++i) {
+            const int s = w0 + 64 * i;
+            v[i] = i < rounds ? sc[s < hi ? s : hi - 1] : 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) held[i] = i < rounds ? key_of(w0 + 64 * i, v[i]) : 0u;
     }
-    const bool any = p.budget - p.sinks - p.recent > 0;
-    // Each wave's run of slots; of the keys equal to the last one that stays,
-    // those of the first slots are taken.
-    const int per = ((len + kEvictWaves - 1) / kEvictWaves + 63) & ~63;
-    const int w0 = wave * per < len ? wave * per : len;
-    const int w1 = w0 + per < len ? w0 + per : len;
-    uint32_t sure = 0, equal = 0;
-    for (int i = w0; i < w1; i += 64) {
-        const int s = i + lane;
-        bool take = s < len && (s < lo || s >= hi), eq = false;
-        if (any && s >= lo && s < hi) {
-            const uint32_t key = score_key(sc[s]);
-            take = key > prefix;
-            eq = key == prefix;
+    // fn(slot, key) for this lane's slots, in order.
+    auto each = [&](auto fn) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i < rounds) fn(w0 + 64 * i, held[i]);
+        } else {
+            for (int i = 0; i < rounds; ++i) {
+                const int s = w0 + 64 * i;
+                fn(s, key_of(s, sc[s < hi ? s : hi - 1]));
+            }
         }
-        sure += __popcll(__ballot(take));
-        equal += __popcll(__ballot(eq));
+    };
+    // `last` becomes the key of the last slot that stays, `want` how many slots
+    // of exactly that key do.
+    uint32_t want = (uint32_t)chosen, last = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass < 2 ? 2047 : 1023;
+        for (int i = t; i < COPIES * 2048; i += kEvictThreads) (&hist[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t* mine = hist[wave % COPIES];
+        each([&](int, uint32_t key) {
+            if (pass == 0 ? key != 0 : (key ^ last) >> (pass == 1 ? 21 : 10) == 0) atomicAdd(&mine[(key >> shift) & digits], 1u);
+        });
+        __syncthreads();
+        // Thread t holds digits 2047 - 2t and the one below it: a scan over
+        // threads counts from the largest digit down.
+        uint32_t a = 0, c = 0;
+#pragma unroll
+        for (int k = 0; k < COPIES; ++k) {
+            a += hist[k][2047 - 2 * t];
+            c += hist[k][2046 - 2 * t];
+        }
+        uint32_t sum = a + c;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t o = __shfl_up(sum, s);
+            if (lane >= s) sum += o;
+        }
+        if (lane == 63) wave_sum[wave] = sum;
+        __syncthreads();
+        uint32_t before = sum - a - c;
+#pragma unroll
+        for (int w = 0; w < kEvictWaves; ++w) before += w < wave ? wave_sum[w] : 0;
+        if (before < want && want <= before + a) {
+            found[0] = 2047 - 2 * t;
+            found[1] = want - before;
+        } else if (before + a < want && want <= before + a + c) {
+            found[0] = 2046 - 2 * t;
+            found[1] = want - before - a;
+        }
+        __syncthreads();
+        last |= found[0] << shift;
+        want = found[1];
     }
+    // Of the keys equal to the last one that stays, those of the first slots
+    // are taken.
+    uint32_t above = 0, equal = 0;
+    each([&](int, uint32_t key) {
+        above += __popcll(__ballot(key > last));
+        equal += __popcll(__ballot(key == last));
+    });
     if (lane == 0) {
-        hist[wave] = sure;
-        hist[64 + wave] = equal;
+        counts[0][wave] = above;
+        counts[1][wave] = equal;
     }
     __syncthreads();
-    uint32_t at = 0, eq_before = 0;
-    for (int w = 0; w < wave; ++w) {
-        at += hist[w];
-        eq_before += hist[64 + w];
+    uint32_t at = p.sinks, eq_before = 0;
+#pragma unroll
+    for (int w = 0; w < kEvictWaves; ++w) {
+        at += w < wave ? counts[0][w] : 0;
+        eq_before += w < wave ? counts[1][w] : 0;
     }
     at += eq_before < want ? eq_before : want;
     const uint64_t below = (1ull << lane) - 1;
-    for (int i = w0; i < w1; i += 64) {
-        const int s = i + lane;
-        bool take = s < len && (s < lo || s >= hi), eq = false;
-        if (any && s >= lo && s < hi) {
-            const uint32_t key = score_key(sc[s]);
-            take = key > prefix;
-            eq = key == prefix;
-        }
-        const uint64_t eqs = __ballot(eq);
-        if (eq) take = eq_before + __popcll(eqs & below) < want;
+    each([&](int s, uint32_t key) {
+        const uint64_t eqs = __ballot(key == last);
+        const bool take = key > last || (key == last && eq_before + __popcll(eqs & below) < want);
         eq_before += __popcll(eqs);
         const uint64_t takes = __ballot(take);
         if (take) keep[at + __popcll(takes & below)] = s;
         at += __popcll(takes);
-    }
+    });
 }
 
 // Kept rows to another cache: D / 8 lanes a row, K and V.

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeParams p) {
     const int slot = len - p.R + (int)(at - (int64_t)b * p.R);
     const int pos = p.positions ? p.positions[at] : slot;
     const bool ok = in && slot >= 0 && pos >= 0 && pos < p.table_rows;
-    const u32x4 x = load_cached16(p.qkv + at * p.qkv_row + (int64_t)h * D + 8 * c);
+    const u32x4 x = load_stream16(p.qkv + at * p.qkv_row + (int64_t)h * D + 8 * c);
     if (h >= p.heads + p.kv_heads) {  // v: as it is
         if (ok)
             *reinterpret_cast<u32x4*>(p.v + (int64_t)b * p.v_seq + (int64_t)slot * p.v_slot +
