@@ -130,6 +130,22 @@ class DecodeCache:
             c[0] = min(c[0], budget)
         return kept
 
+    def rollback(self, rows: list) -> None:
+        """Forget the last ``rows[b]`` slots of each sequence: the rejected rows
+        of a verified draft, behind the accepted ones."""
+        if len(rows) != self.B or any(not 0 <= n <= c[0] for n, c in zip(rows, self._host)):
+            raise ValueError(f"rollback needs 0 .. slots rows for each of {self.B} sequences, got {list(rows)}")
+        less = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
+        self.lens.sub_(less)
+        self.seen.sub_(less)
+        for c, n in zip(self._host, rows):
+            c[0] -= n
+            c[1] -= n
+        if self.scored:  # the slots' next rows start at zero
+            free = torch.arange(self.capacity, device=self.lens.device) >= self.lens[:, None, None]
+            for s in self.scores:
+                s.masked_fill_(free, 0.0)
+
     def reset(self, b: int | None = None) -> None:
         """Forget sequence ``b`` (None: all): its slots are free again."""
         at = slice(None) if b is None else b

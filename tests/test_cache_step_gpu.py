@@ -109,6 +109,24 @@ def test_window_prefix_and_tree(device, model):
     tree = tree_masks(g, B, R_).to(device)
     S.GemmStep(model, B * R_, cache=cache, tree=tree).run(x_rows(device, model, B * R_, 42))
     assert cache.lens.tolist() == [36, 36]
+    cache.rollback([4, 0])
+    assert cache.lens.tolist() == cache.seen.tolist() == [32, 36]
+    S.GemmStep(model, B, cache=cache).run(x_rows(device, model, B, 43))
+    assert cache.lens.tolist() == [33, 37]
+    for bad in ([1], [34, 0], [0, -1]):
+        with pytest.raises(ValueError, match="rollback"):
+            cache.rollback(bad)
+
+
+def test_rollback_forgets_scores(device, model):
+    B = 2
+    cache = Checked(model, B, 40, scored=True)
+    S.GemmStep(model, B * 10, cache=cache).run(x_rows(device, model, B * 10, 44))
+    cache.rollback([3, 10])
+    assert cache.lens.tolist() == [7, 0]
+    for s in cache.scores:
+        assert (s[0, :, 7:] == 0).all() and (s[1] == 0).all() and (s[0, :, :7] > 0).all()
+    S.GemmStep(model, B, cache=cache).run(x_rows(device, model, B, 45))
 
 
 @pytest.mark.parametrize("kw", [dict(scored=True), dict(window=16, sinks=2), dict(tree=True)])
