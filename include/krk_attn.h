@@ -79,14 +79,15 @@ typedef struct krk_attn_shape {
  *   out[row, h] = sum_t p_t v_t,   p = softmax over the visible t of scale * (q[row, h] . k_t)
  *
  * With `tree`, bit j of tree[b * R + i] says whether row i sees the call's own
- * row j (its slot lens - R + j), whatever the window; bits R and up are
- * ignored.  The row's position is then prefix + lens - R + (bits set) - 1, and
- * it sees the earlier keys by that.  Needs R <= 64 and window 0 or >= R.
+ * row j (its slot lens - R + j), whatever the window; bits R and up, and those of
+ * padding rows, are ignored.  The row's position is then that of the sequence's
+ * first row that has a slot, plus the bits set, less 1, and it sees the earlier
+ * keys by that.  Needs R <= 64 and window 0 or >= R.
  *
- * Padding rows, and rows that see nothing, give zeros in out and -infinity in
- * lse.  Keys that a row does not see have no part in its result, whatever they
- * hold (NaN and infinities too).  Sums, maxima and weights are held in 32
- * bits; the weights enter the products with v rounded to bf16 where 128
+ * Padding rows, and rows that see nothing (or whose scores are all -infinity),
+ * give zeros in out and -infinity in lse.  Keys that a row does not see have no
+ * part in its result, whatever they hold (NaN and infinities too).  Sums, maxima
+ * and weights are held in 32 bits; the weights enter the products with v rounded to bf16 where 128
  * rows share a workgroup (krk_attn_plan tells), else as two bf16 parts.
  */
 typedef struct krk_attn_args {

@@ -58,7 +58,7 @@ struct AttnParams {
 // `first` on (tree masks) those whose bit is set.  Padding: lo = kPadding, hi = -1.
 struct RowSight {
     int lo, hi;
-    int first;       // position of the sequence's first new row (tree)
+    int first;       // position of bit 0 (tree); before the cache where the first rows have no slot
     uint64_t bits;   // of the new rows, 0 without tree masks
 };
 
@@ -76,10 +76,13 @@ __device__ __forceinline__ RowSight row_sight(const AttnParams& p, int b, int r,
     int pos = p.prefix + slot;
     s.hi = pos;
     if (p.tree) {
-        const uint64_t all = p.R >= 64 ? ~0ull : (1ull << p.R) - 1;
-        s.bits = (uint64_t)p.tree[(int64_t)b * p.R + r] & all;
-        pos = s.first + __popcll(s.bits) - 1;
-        s.hi = s.first - 1;
+        s.bits = (uint64_t)p.tree[(int64_t)b * p.R + r];
+        if (p.R < 64) s.bits &= (1ull << p.R) - 1;
+        const int none = p.R - len;  // the first rows, which have no slot
+        if (none > 0) s.bits = none < 64 ? s.bits >> none << none : 0;
+        const int cached = p.prefix + (none > 0 ? 0 : -none);
+        pos = cached + __popcll(s.bits) - 1;
+        s.hi = cached - 1;
     }
     const int lo = p.window ? pos - p.window + 1 : 0;
     s.lo = lo > 0 ? lo : 0;

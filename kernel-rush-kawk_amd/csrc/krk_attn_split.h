@@ -422,8 +422,8 @@ __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
     KeyFrag<D> kf;
     kf.load(base, p.k.slot, kb, len, lane);
     // Which rows see what, from the first live row and the last.
-    const int live_from = len - p.R > 0 ? len - p.R : 0;  // position of the first row with a slot
-    const int hi_min = p.tree ? len - p.R - 1 : live_from;
+    const int live_from = len - p.R > 0 ? len - p.R : 0;  // slot of the first row that has one
+    const int hi_min = p.tree ? live_from - 1 : live_from;
     const int lo_max = p.window && len > p.window ? len - p.window : 0;
     const bool whole = kb + 32 <= len && kb + 31 <= hi_min && (kb >= lo_max || kb + 32 <= p.sinks);
 

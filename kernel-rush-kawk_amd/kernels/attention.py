@@ -275,7 +275,7 @@ class CacheAttention:
         rows.  ``prefix=(kp, vp)``: the shared keys and values, ``[keys,
         kv_heads, head_dim]``.  ``tree`` (int64 ``[B, R]``, R <= 64): bit j of
         row i says whether the row sees the call's own row j; its position is
-        then that of the first row plus its set bits less one.  ``scores``
+        then that of the sequence's first row plus its set bits less one.  ``scores``
         (``[B, kv_heads, capacity]`` fp32): each cached key's weight, summed over
         rows and the query heads of its group, is added; into ``scores_out``
         where given (slots below ``lens``)."""

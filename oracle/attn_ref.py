@@ -24,9 +24,10 @@ def visible(prefix: int, length: int, R: int, window: int, sinks: int, tree=None
         if tree is None:
             pos, own = first + i, set()
             top = pos
-        else:
-            own = {first + j for j in range(R) if tree[i] >> j & 1}
-            pos, top = first + len(own) - 1, first - 1
+        else:  # of the call's own rows, those that have a slot
+            own = {first + j for j in range(R) if tree[i] >> j & 1 and length - R + j >= 0}
+            cached = prefix + max(0, length - R)
+            pos, top = cached + len(own) - 1, cached - 1
         for t in range(n):
             near = t <= top and (window == 0 or t > pos - window or t < sinks)
             seen[i, t] = near or t in own

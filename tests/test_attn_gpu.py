@@ -143,6 +143,8 @@ def test_window_and_sinks(device, window, sinks, R):
     (2, 64, 4, 4, 64, 300, [64, 270], 70, 2),
     (3, 5, 8, 2, 128, 90, [90, 5, 3], 6, 1),
     (1, 1, 8, 2, 128, 90, [50], 0, 0),
+    (4, 64, 8, 2, 128, 70, [1, 63, 0, 70], 0, 0),
+    (2, 33, 16, 2, 64, 300, [300, 20], 40, 3),
 ])
 def test_tree(device, B, R, heads, kv, D, cap, lens, window, sinks):
     check_attention(device, 300 + R, B, R, heads, kv, D, cap, lens, window=window, sinks=sinks, tree=True)
@@ -168,6 +170,10 @@ def test_prompt(device, B, R, heads, kv, D, cap, lens, window, sinks):
     (2, 3, 8, 2, 128, 70, [70, 9], 64, None, 20, 100, False),
     (2, 2, 8, 2, 128, 70, [70, 9], 0, 64, 0, 0, False),
     (7, 9, 10, 2, 128, 64, [64, 9, 10, 33, 31, 8, 0], 65, None, 64, 0, False),
+    (3, 7, 8, 2, 128, 40, [5, 40, 7], 20, None, 9, 2, True),
+    (40, 1, 32, 8, 128, 33, [1 + b % 33 for b in range(40)], 300, None, 0, 0, False),
+    (6, 8, 16, 4, 64, 100, [100, 8, 60, 9, 7, 50], 500, None, 77, 5, True),
+    (2, 40, 8, 2, 128, 64, [64, 45], 130, None, 0, 0, False),
 ])
 def test_shared_prefix(device, B, R, heads, kv, D, cap, lens, prefix, built, window, sinks, tree):
     check_attention(device, 500 + B, B, R, heads, kv, D, cap, lens, prefix=prefix, built_prefix=built, window=window,
@@ -180,6 +186,9 @@ def test_shared_prefix(device, B, R, heads, kv, D, cap, lens, prefix, built, win
     (2, 32, 8, 2, 128, 300, [300, 17], 0, 0, False),
     (2, 9, 8, 2, 128, 200, [200, 30], 25, 4, False),
     (1, 20, 8, 2, 64, 150, [140], 0, 0, True),
+    (2, 4, 8, 2, 128, 150, [140, 2], 0, 0, True),
+    (1, 90, 8, 4, 128, 300, [260], 0, 0, False),
+    (1, 300, 4, 4, 64, 400, [333], 50, 70, False),
 ])
 def test_scores(device, B, R, heads, kv, D, cap, lens, window, sinks, tree):
     check_attention(device, 600 + R, B, R, heads, kv, D, cap, lens, window=window, sinks=sinks, tree=tree, scored=True)
