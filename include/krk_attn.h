@@ -60,7 +60,7 @@ typedef struct krk_cache {
 /* What a call of krk_attn_bf16 computes, fixed for an object that makes many
  * of them: it decides how the work is cut and the workspace. */
 typedef struct krk_attn_shape {
-    int B, R;            /* sequences; new rows of each (R <= 65536, B * R * heads < 2^26) */
+    int B, R;            /* sequences; new rows of each (R <= 65536, B * R * heads < 2^25, B * kv_heads < 2^23) */
     int heads, kv_heads; /* heads a multiple of kv_heads */
     int head_dim;        /* 64 or 128 */
     int capacity;        /* slots of the cache, >= 1 */

@@ -112,8 +112,9 @@ int check_layout(int B, int R, int heads, int kv_heads, int head_dim, int capaci
     if (B > 65535 || kv_heads > 65535 || R > 65536) return fail(KRK_ATTN_ERR_INVALID, "B=%d, kv_heads=%d (most 65535) or R=%d (most 65536) too large", B, kv_heads, R);
     if (heads % kv_heads) return fail(KRK_ATTN_ERR_INVALID, "heads=%d must be a multiple of kv_heads=%d", heads, kv_heads);
     if (head_dim != 64 && head_dim != 128) return fail(KRK_ATTN_ERR_UNSUPPORTED, "head_dim=%d: this build has 64 and 128", head_dim);
-    // Grids of up to 64 threads a row or 16 a slot stay below 2^32 threads.
-    if ((int64_t)B * R * heads >= ((int64_t)1 << 26)) return fail(KRK_ATTN_ERR_INVALID, "B * R * heads = %lld must be below 2^26", (long long)((int64_t)B * R * heads));
+    // Grids of up to 128 threads a row, or 256 a sequence and head, stay below 2^32 threads.
+    if ((int64_t)B * R * heads >= ((int64_t)1 << 25)) return fail(KRK_ATTN_ERR_INVALID, "B * R * heads = %lld must be below 2^25", (long long)((int64_t)B * R * heads));
+    if ((int64_t)B * kv_heads >= ((int64_t)1 << 23)) return fail(KRK_ATTN_ERR_INVALID, "B * kv_heads = %lld must be below 2^23", (long long)((int64_t)B * kv_heads));
     if (capacity >= 1 << 27) return fail(KRK_ATTN_ERR_INVALID, "capacity=%d must be below 2^27", capacity);
     return KRK_ATTN_OK;
 }

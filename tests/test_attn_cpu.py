@@ -68,7 +68,8 @@ def shape(**kw):
 @pytest.mark.parametrize("kw,msg", [
     (dict(B=0), ">= 1"), (dict(R=0), ">= 1"), (dict(R=-3), ">= 1"), (dict(kv_heads=0), ">= 1"), (dict(capacity=0), ">= 1"),
     (dict(heads=9), "multiple of kv_heads"), (dict(head_dim=96), "64 and 128"), (dict(head_dim=256), "64 and 128"),
-    (dict(B=70000), "too large"), (dict(R=70000), "too large"), (dict(B=60000, R=60000), "2^26"),
+    (dict(B=70000), "too large"), (dict(R=70000), "too large"), (dict(B=60000, R=60000), "2^25"),
+    (dict(B=65535, heads=1024, kv_heads=1), "2^25"), (dict(B=65535, heads=256, kv_heads=256), "2^23"),
     (dict(capacity=1 << 27), "2^27"), (dict(capacity=1 << 26, prefix=1 << 26), "2^27"), (dict(window=-1), "negative"),
     (dict(window=4, sinks=-1), "negative"), (dict(prefix=-1), "negative"), (dict(sinks=4), "sinks need a window"),
     (dict(window=1 << 28), "2^28"), (dict(scored=2), "scored must be"), (dict(scored=1, prefix=5), "shared prefix"),
