@@ -58,6 +58,7 @@ struct AttnParams {
 // `first` on (tree masks) those whose bit is set.  Padding: lo = kPadding, hi = -1.
 struct RowSight {
     int lo, hi;
+    int last;        // the highest position it may see; with tree masks that of bit 63, set or not
     int first;       // position of bit 0 (tree); before the cache where the first rows have no slot
     uint64_t bits;   // of the new rows, 0 without tree masks
 };
@@ -84,6 +85,7 @@ __device__ __forceinline__ RowSight row_sight(const AttnParams& p, int b, int r,
         pos = cached + __popcll(s.bits) - 1;
         s.hi = cached - 1;
     }
+    s.last = p.tree ? s.first + 63 : s.hi;
     const int lo = p.window ? pos - p.window + 1 : 0;
     s.lo = lo > 0 ? lo : 0;
     if (slot < 0) {
@@ -197,15 +199,16 @@ __device__ __forceinline__ TaskRow task_row(const AttnParams& p, const Task& t, 
 }
 
 // What a set of rows sees at most (lo_min .. hi_max) and all of them see (from
-// lo_max to hi_min), over the lanes of a wave.
+// lo_max to hi_min), over the lanes of a wave.  Without a window a sequence's
+// steps reach its last key, whatever its tree masks hold: kept scores are then
+// written for every key.
 struct Reach {
     int lo_min = 0x7fffffff, hi_max = -1, lo_max = 0, hi_min = 0x7fffffff;
     __device__ __forceinline__ void add(const RowSight& s, bool live) {
         if (live && s.lo != kPadding) {
-            const int hi = s.bits ? s.first + 63 : s.hi;
             lo_min = s.lo < lo_min ? s.lo : lo_min;
             lo_max = s.lo > lo_max ? s.lo : lo_max;
-            hi_max = hi > hi_max ? hi : hi_max;
+            hi_max = s.last > hi_max ? s.last : hi_max;
             hi_min = s.hi < hi_min ? s.hi : hi_min;
         }
     }

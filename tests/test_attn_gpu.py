@@ -415,6 +415,24 @@ def test_evict(device, case, kind, inplace):
                 assert (ko[b, n:, h] == 9).all() and (vo[b, n:, h] == 9).all() and (so[b, h, n:] == 9).all()
 
 
+def test_scores_of_rows_that_see_none_of_the_new(device):
+    """Tree masks without bits: the call's own keys get no weight, also where an
+    earlier call on the same workspace gave them some."""
+    g = gen(655)
+    B, R, heads, kv, D, cap = 2, 4, 8, 2, 128, 400
+    op = A.CacheAttention(B, R, heads, kv, D, cap, device, scored=True)
+    q, k, v = rnd(g, B * R, heads * D).to(device), rnd(g, B, cap, kv, D).to(device), rnd(g, B, cap, kv, D).to(device)
+    lens = torch.tensor([400, 259], dtype=torch.int32, device=device)
+    masks = torch.ones((B, R), dtype=torch.int64, device=device)
+    for tree, new in ((masks * 15, True), (masks * 0, False)):
+        s = torch.zeros((B, kv, cap), device=device)
+        say("scores without bits", new)
+        op(q, k, v, lens, tree=tree, scores=s)
+        for b, n in enumerate((400, 259)):
+            assert bool((s[b, :, n - R:n] > 0).all()) == new and bool((s[b, :, n - R:n] == 0).all()) != new
+            assert ((s[b].sum(-1) - R * heads // kv).abs() < 1e-3).all()
+
+
 # ------------------------------------------------- streams, graphs, devices
 def test_on_another_stream_and_in_graphs(device):
     """Calls run on the current stream; two captured graphs of two objects,
@@ -482,3 +500,117 @@ def test_same_call_twice_is_bit_equal(device):
         a = op(q, k, v, lens, prefix=shared)
         b = op(q, k, v, lens, prefix=shared)
         assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits_for_many_rows(device):
+    """The same distances for the tile kernel, the weights' second reading of K,
+    and the cache write: rows of the last 200 slots."""
+    slots, step, kv, D, heads, R = 36000, 65536, 2, 128, 8, 200
+    base = torch.zeros((slots - 1) * step + kv * 2 * D, dtype=BF, device=device)
+    view = lambda off: torch.as_strided(base, (1, slots, kv, D), (0, step, 2 * D, 1), off)
+    k, v = view(0), view(D)
+    g = gen(740)
+    qkv = rnd(g, R, (heads + 2 * kv) * D).to(device)
+    lens = torch.tensor([slots], dtype=torch.int32, device=device)
+    table = A.rope_table(slots, D, 1e6, device)
+    say("offsets past 32 bits, many rows")
+    q = A.qk_norm_rope(qkv, None, None, 1e-6, table, lens, k, v)
+    near = 2 * R
+    kc, vc = torch.zeros((1, near, kv, D), dtype=BF), torch.zeros((1, near, kv, D), dtype=BF)
+    kn, vn = kc.to(device), vc.to(device)
+    again = A.qk_norm_rope(qkv, None, None, 1e-6, table, torch.tensor([near], dtype=torch.int32, device=device), kn, vn,
+                           positions=torch.arange(slots - R, slots, dtype=torch.int32, device=device))
+    assert torch.equal(q, again)
+    assert torch.equal(k[:, -R:], kn[:, -R:]) and torch.equal(v[:, -R:], vn[:, -R:])
+    say("attention")
+    op = A.CacheAttention(1, R, heads, kv, D, slots, device, window=100, scored=True)
+    small = A.CacheAttention(1, R, heads, kv, D, near, device, window=100, scored=True)
+    s, t = torch.zeros((1, kv, slots), device=device), torch.zeros((1, kv, near), device=device)
+    a = op(q, k, v, lens, scores=s)
+    b = small(q, kn, vn, torch.tensor([near], dtype=torch.int32, device=device), scores=t)
+    # Other steps and ranges.  Each side's weights are off by 2^-8, its outputs
+    # by 2^-8 of at most the largest value; its scores by at most D * 2^-24 of
+    # sum |q k| * scale, about 100 * 0.09 here, so a weight by less than 2^-13.
+    assert ((a.double() - b.double()).abs() <= 2.0 ** -6 * vn.abs().max()).all()
+    assert ((s[..., -near:] - t).abs() <= 2.0 ** -11 * t).all() and (s[..., :-near] == 0).all()
+
+
+@pytest.mark.parametrize("what", ["decode", "scored", "tree", "prompt", "prompt_scored", "shared"])
+def test_replays_follow_the_lengths(device, what):
+    """A graph of the cache write and the attention behind it: every replay, at
+    other lengths and rows, equals the eager calls bit by bit."""
+    g = gen(1020)
+    heads, kv, D, cap = 16, 4, 128, 1200
+    B, R, kw = {"decode": (3, 1, {}), "scored": (3, 1, dict(scored=True)), "tree": (2, 8, {}), "prompt": (2, 100, {}),
+                "prompt_scored": (2, 100, dict(scored=True)), "shared": (5, 1, dict(prefix=333))}[what]
+    op = A.CacheAttention(B, R, heads, kv, D, cap, device, **kw)
+    table = A.rope_table(4000, D, 1e6, device)
+    k, v = rnd(g, B, cap, kv, D).to(device), rnd(g, B, cap, kv, D).to(device)
+    qkv = rnd(g, B * R, (heads + 2 * kv) * D).to(device)
+    lens = torch.full((B,), R, dtype=torch.int32, device=device)
+    more = {}
+    if what == "tree":
+        more["tree"] = tree_masks(g, B, R).to(device)
+    if what == "shared":
+        more["prefix"] = tuple(rnd(g, 333, kv, D).to(device) for _ in "kv")
+    s = torch.zeros((B, kv, cap), device=device)
+    if kw.get("scored"):
+        more["scores"] = s
+    q = torch.empty((B * R, heads * D), dtype=BF, device=device)
+    out = torch.empty_like(q)
+
+    def run():
+        A.qk_norm_rope(qkv, None, None, 1e-6, table, lens, k, v, q_out=q)
+        op.run(q, k, v, lens, out, **more)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    k0, v0 = k.clone(), v.clone()
+    for n in range(4):
+        lens.copy_(torch.randint(0, cap + 1, (B,), generator=g).int())
+        qkv.copy_(rnd(g, *qkv.shape))
+        got = []
+        for call in (run, graph.replay):
+            k.copy_(k0), v.copy_(v0), s.zero_(), q.zero_()
+            call()
+            torch.cuda.synchronize()
+            got.append([t.clone() for t in (out, k, v, s)])
+        for a, b in zip(*got):
+            assert torch.equal(a, b), n
+
+
+def test_two_objects_on_two_streams(device):
+    """Objects have workspaces of their own, so their calls may run at once."""
+    g = gen(1030)
+    B, heads, kv, D, cap = 2, 32, 8, 128, 3000
+    k, v = rnd(g, B, cap, kv, D).to(device), rnd(g, B, cap, kv, D).to(device)
+    q = [rnd(g, B, heads * D).to(device) for _ in range(2)]
+    lens = torch.tensor([3000, 1700], dtype=torch.int32, device=device)
+    ops = [A.CacheAttention(B, 1, heads, kv, D, cap, device) for _ in range(2)]
+    want = [op(x, k, v, lens) for op, x in zip(ops, q)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    out = [[torch.empty_like(w) for _ in range(20)] for w in want]
+    torch.cuda.synchronize()
+    for n in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                ops[i].run(q[i], k, v, lens, out[i][n])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in out[i])
+
+
+def test_broadcast_caches(device):
+    """Caches expanded over sequences and heads (strides of 0) are read as such."""
+    g = gen(1040)
+    for R in (1, 100):
+        B, heads, kv, D, cap = 3, 8, 4, 64, 200
+        k, v = rnd(g, 1, cap, 1, D).to(device), rnd(g, 1, cap, 1, D).to(device)
+        q = rnd(g, B * R, heads * D).to(device)
+        lens = torch.tensor([200, 130, 101], dtype=torch.int32, device=device)
+        op = A.CacheAttention(B, R, heads, kv, D, cap, device)
+        wide = [t.expand(B, cap, kv, D) for t in (k, v)]
+        assert torch.equal(op(q, *wide, lens), op(q, *(t.contiguous() for t in wide), lens))
