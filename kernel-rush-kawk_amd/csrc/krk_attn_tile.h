@@ -1,10 +1,12 @@
 // Cache attention for many rows of a head (prompts, batches over a shared
 // prefix): one workgroup per tile of 128 rows, K and V through LDS.
 //
-// Bound by the matrix pipe, the exponentials and LDS alike: 64 keys of a wave's
-// 32 rows are 1.05 MFLOP (1030 cycles of a SIMD's MFMA at head size 128), 32 KB
-// of LDS reads (a quarter of 1030 cycles of what a CU's LDS delivers), and 2048
-// weights at about 25 VALU cycles per 64 of them.
+// Bound by LDS and the matrix pipe alike: 64 keys of a wave's 32 rows are 1030
+// cycles of its SIMD's matrix pipe at head size 128 (2.1 MFLOP) and 32 KB of LDS
+// reads, 1030 cycles for a CU's four waves, and the keys' own 32 KB come on top.
+// The 2048 weights take about 700 cycles of the vector pipe.  Measured, two
+// waves of a SIMD need 3600 cycles for a step each, 865 TFLOP/s of an 8192-row
+// prompt with a window of 2048.
 //
 // Work split.  Four waves, each with 32 rows of its own, all reading the same
 // 64-key steps of K and V from LDS.  S^T = K Q^T and O^T = V^T P^T on
@@ -12,9 +14,11 @@
 // order of a step's second product is the one the first leaves in its lanes, so
 // weights stay in their lane.  V's operand comes transposed out of LDS
 // (ds_read_b64_tr_b16).  Two workgroups share a CU (80 KB of LDS and up to 256
-// registers a lane each) and run apart, so that one's exponentials run under the
-// other's products: 8 waves in one workgroup, in step or half a step apart,
-// were 8% slower at 8192 rows.
+// registers a lane each) and run apart: 8 waves in one workgroup, four of them
+// half a step behind, need half the DMAs but were 20% slower (5.6M GPU cycles
+// against 4.6M), as one half's weights wait for LDS and issue slots under the
+// other's products.  64 rows a wave would halve the LDS reads, but their
+// registers spill.
 //
 // The running maximum moves only when a row's grows by more than 2^8 (the
 // weights stay below 2^8 then, which costs no precision), so O is rescaled a
@@ -28,6 +32,8 @@
 // 8 bits of mantissa each, the error of a weighted mean of many values is that
 // of the final rounding again.
 #pragma once
+
+#include <type_traits>
 
 #include "krk_attn_common.h"
 
@@ -84,20 +90,39 @@ struct TileKernel {
             off[i] = row * slot + 8 * ((lane % CH) ^ (V ? v_swizzle(row) : k_swizzle(row)));
         }
     }
-    static __device__ __forceinline__ void fetch(const uint16_t* base, int64_t slot, const int64_t (&off)[DMAS], int kb,
-                                                 int limit, uint32_t to, int wave, int lane) {
-        const uint16_t* step = base + (int64_t)kb * slot;
-        if (kb + kTileStep <= limit) {
+    // Fetches a task's steps in order: this wave's share of a step's 64 rows.
+    // Places advance instead of being worked out: a wave's scalar instructions
+    // are on its path (this and the like took 2.5% off the cycles).
+    struct Stream {
+        const uint16_t* from;  // the step's first row
+        int t;
+        uint32_t to;  // its slot in the ring
+        __device__ __forceinline__ Stream(const uint16_t* base, int64_t slot, const KeySteps<kTileStep>& steps)
+            : from(base + (int64_t)steps.key(steps.t0) * slot), t(steps.t0), to(0) {}
+        template <int RING>
+        __device__ __forceinline__ void fetch(int64_t slot, const int64_t (&off)[DMAS], const KeySteps<kTileStep>& steps, int t_full,
+                                              int limit, uint32_t ring, int wave, int lane) {
+            const uint32_t dst = ring + to + wave * 1024;
+            if (t < t_full) {
 #pragma unroll
-            for (int i = 0; i < DMAS; ++i) dma_row_quiet(step + off[i], to + (wave + kTileWaves * i) * 1024);
-        } else {
+                for (int i = 0; i < DMAS; ++i) dma_row_quiet(from + off[i], dst + kTileWaves * i * 1024);
+            } else {  // rows from the limit on read the last one again
+                const int kb = steps.key(t);
 #pragma unroll
-            for (int i = 0; i < DMAS; ++i) {
-                const int over = kb + (wave + kTileWaves * i) * ROWS_PER_DMA + lane / CH - (limit - 1);
-                dma_row_quiet(step + off[i] - (over > 0 ? over : 0) * slot, to + (wave + kTileWaves * i) * 1024);
+                for (int i = 0; i < DMAS; ++i) {
+                    const int over = kb + (wave + kTileWaves * i) * ROWS_PER_DMA + lane / CH - (limit - 1);
+                    dma_row_quiet(from + off[i] - (over > 0 ? over : 0) * slot, dst + kTileWaves * i * 1024);
+                }
             }
+            if (t < steps.t1 - 1) {
+                from += kTileStep * slot;
+                ++t;
+                if (t == steps.sink_steps) from += (int64_t)(steps.from - kTileStep * t) * slot;
+            }
+            to += STEP_BYTES;
+            to = to == (uint32_t)RING * STEP_BYTES ? 0u : to;
         }
-    }
+    };
 
     static __device__ __forceinline__ bf16x8 k_operand(const unsigned char* at, int off) {
         return *reinterpret_cast<const bf16x8*>(at + off);
@@ -123,16 +148,15 @@ __device__ __forceinline__ bool odd_bf16x8(const bf16x8& v) {
     return odd;
 }
 
-// Issue order of N MFMAs and their operands' LDS reads (EACH an MFMA): AHEAD
-// reads first, then they alternate.  Left alone the compiler reads each operand
-// right before its MFMA and waits.
-template <int N, int AHEAD, int EACH>
+// Issue order of the next N MFMAs and of LDS reads for later ones, EACH behind
+// an MFMA.  Left alone the compiler reads each operand right before its MFMA
+// and waits.
+template <int N, int EACH>
 __device__ __forceinline__ void read_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+        if (EACH) __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
     }
 }
 
@@ -188,21 +212,24 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
     unsigned char* kring = lds;
     unsigned char* vring = lds + kTileKRing * T::STEP_BYTES;
     const uint32_t lds_base = (uint32_t)(uintptr_t)(lds_s16x4*)lds;
-    auto k_slot_at = [&](int t) { return (unsigned)t % kTileKRing * T::STEP_BYTES; };
-    auto v_slot_at = [&](int t) { return (unsigned)t % kTileVRing * T::STEP_BYTES; };
 
-    // Steps past the last fetch the last one again, into slots that nothing
-    // reads any more: every step then has the same number of DMAs in flight.
+    // The next fetches of K and of V: where from, where to.  Behind the last
+    // step it is fetched again, into slots that nothing reads any more: every
+    // step then has the same number of DMAs in flight.
     int64_t k_off[T::DMAS], v_from[T::DMAS];
     T::template offsets<false>(task.k_slot, wave, lane, k_off);
     T::template offsets<true>(task.v_slot, wave, lane, v_from);
-    auto fetch_k = [&](int t) {
-        T::fetch(task.k, task.k_slot, k_off, steps.key(t < t1 ? t : t1 - 1), limit,
-                 lds_base + k_slot_at(t), wave, lane);
+    typename T::Stream k_next(task.k, task.k_slot, steps), v_next(task.v, task.v_slot, steps);
+    const int t_full = steps.key(t1 - 1) + kTileStep <= limit ? t1 : t1 - 1;  // steps from here on pass the limit
+    auto fetch_k = [&]() { k_next.template fetch<kTileKRing>(task.k_slot, k_off, steps, t_full, limit, lds_base, wave, lane); };
+    auto fetch_v = [&]() {
+        v_next.template fetch<kTileVRing>(task.v_slot, v_from, steps, t_full, limit, lds_base + kTileKRing * T::STEP_BYTES, wave, lane);
     };
-    auto fetch_v = [&](int t) {
-        T::fetch(task.v, task.v_slot, v_from, steps.key(t < t1 ? t : t1 - 1), limit,
-                 lds_base + kTileKRing * T::STEP_BYTES + v_slot_at(t), wave, lane);
+    // The slots that the next scores and products read.
+    uint32_t k_read = 0, v_read = 0;
+    auto turn = [](uint32_t& slot, int ring) {
+        slot += T::STEP_BYTES;
+        slot = slot == (uint32_t)ring * T::STEP_BYTES ? 0u : slot;
     };
 
     // This lane's places in a step's K and V.
@@ -224,27 +251,38 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
-    // Scores of a step.
-    auto scores = [&](int t) {
-        const unsigned char* kb = kring + k_slot_at(t) + k_row;
+    // Scores of a step: first those of its first 32 keys, whose maximum is then
+    // taken under the others' products.
+    auto scores = [&]() {
+        const unsigned char* kb = kring + k_read + k_row;
+        turn(k_read, kTileKRing);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kt][e] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int ks = 0; ks < KS; ++ks)
                 s[kt] = mfma32(T::k_operand(kb, 32 * kt * D * 2 + ((2 * ks) ^ k_xor) * 16), qf[ks], s[kt]);
-        read_ahead<2 * KS, 6, 1>();
+        }
     };
     // No weight for what the row does not see (not called for steps that every
     // row of the wave sees whole).
     const int hi = sight.hi < task.seg + limit - 1 ? sight.hi : task.seg + limit - 1;
-    auto seen_whole = [&](const Reach& r, int kb) {
-        const int pos = task.seg + kb;
-        return kb + kTileStep <= limit && pos + kTileStep - 1 <= r.hi_min && (pos >= r.lo_max || pos + kTileStep <= p.sinks);
+    // The steps that every row of a wave, or of the workgroup, sees whole.
+    struct Steps {
+        int from, n;
+        __device__ __forceinline__ bool has(int t) const { return (unsigned)(t - from) < (unsigned)n; }
     };
+    auto whole_steps = [&](const Reach& r) {
+        Steps x;
+        const int end = r.hi_min - task.seg < limit ? r.hi_min - task.seg + 1 : limit;
+        const int low = r.lo_max - task.seg - steps.from;
+        x.from = steps.sink_steps + (low > 0 ? (low + kTileStep - 1) / kTileStep : 0);
+        const int n = steps.sink_steps + (end > steps.from ? (end - steps.from) / kTileStep : 0) - x.from;
+        x.n = n > 0 ? n : 0;
+        return x;
+    };
+    const Steps mine_whole = whole_steps(reach), all_whole = whole_steps(block);
     auto hide = [&](int t) {
         const int kb = steps.key(t);
         const int from = task.seg + kb + 4 * g2;
@@ -267,15 +305,18 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
 #pragma unroll
         for (int e = 0; e < 32; ++e) s[e >> 4][e & 15] = (vis >> e) & 1 ? s[e >> 4][e & 15] : kNegInf;
     };
-    auto maximum = [&]() {
-        float v = fmaxf(s[0][0], s[1][0]);
+    auto highest = [&](int kt) {
+        float v[4];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) v = fmaxf(fmaxf(v, s[0][e]), s[1][e]);
-        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        for (int e = 0; e < 4; ++e) v[e] = fmaxf(fmaxf(s[kt][3 * e], s[kt][3 * e + 1]), s[kt][3 * e + 2]);
+        v[0] = fmaxf(fmaxf(v[0], s[kt][12]), s[kt][13]);
+        v[1] = fmaxf(fmaxf(v[1], s[kt][14]), s[kt][15]);
+        return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
     };
     const float slack = fminf(8.0f / p.c, 1e30f);
-    auto raise = [&](float mx) {
+    auto raise = [&](float v) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        const float mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
         if (__any(mx > m + slack)) {
             const float mn = fmaxf(m, mx);
             const float ms = mn == kNegInf ? 0.0f : mn;
@@ -300,22 +341,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
             w[e >> 3][(e & 7) >> 1] = pack_bf16(a, b);
         }
         l += sum[0] + sum[1];
+        asm volatile("" : "+v"(l));  // the sums here, not behind the products
     };
-    auto products = [&](int t) {
-        const unsigned char* vb = vring + v_slot_at(t);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-                o[d] = mfma32(T::v_operand(vb + v_off[d] + 16 * ks * D * 2), __builtin_bit_cast(bf16x8, w[ks]), o[d]);
-        read_ahead<4 * DT, 8, 2>();
-    };
+    auto v_at = [&](int ks, int d) { return T::v_operand(vring + v_read + v_off[d] + 16 * ks * D * 2); };
     // A step that some row of the workgroup does not see whole may hold
     // infinities or NaNs that only some rows see.  Each wave then zeroes those
     // among the values it fetched; they are added behind the last step.
     bool any_odd = false;
-    auto tame = [&](int t) {
-        unsigned char* at = vring + v_slot_at(t);
+    auto tame = [&](uint32_t slot) {
+        unsigned char* at = vring + slot;
 #pragma unroll 1
         for (int i = 0; i < T::DMAS; ++i) {
             u32x4* x = reinterpret_cast<u32x4*>(at + (wave + kTileWaves * i) * 1024 + lane * 16);
@@ -328,43 +362,73 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
     };
 
     if (t0 < t1) {
+        // A step's maximum, behind its scores.
+        auto settle = [&](int t, float first) {
+            if (!mine_whole.has(t)) {
+                hide(t);
+                first = highest(0);
+            }
+            raise(fmaxf(first, highest(1)));
+        };
+        // The products with V, and the next step's scores where there is one.
+        auto multiply = [&](const bf16x8 (&first)[DT], auto more) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    o[d] = mfma32(ks ? v_at(ks, d) : first[d], __builtin_bit_cast(bf16x8, w[ks]), o[d]);
+            turn(v_read, kTileVRing);
+            float top = 0.0f;
+            if constexpr (decltype(more)::value) {
+                scores();
+                top = highest(0);
+                read_ahead<4 * DT, 2>();
+                read_ahead<KS, 1>();
+                read_ahead<KS, 0>();
+            } else {
+                read_ahead<3 * DT, 2>();
+                read_ahead<DT, 0>();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            return top;
+        };
         // K two steps ahead of the scores, V one ahead of its products.
-        fetch_k(t0);
-        fetch_k(t0 + 1);
-        fetch_v(t0);
-        fetch_k(t0 + 2);
+        fetch_k();
+        fetch_k();
+        fetch_v();
+        fetch_k();
         vm_wait_stages<T::DMAS>(3);  // K of the first step has landed
         // q has landed as well; said here, or the compiler waits for it in the
         // loop, and with it for the DMAs just issued.
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
         bare_barrier();
-        auto next_scores = [&](int t) {
-            scores(t);
-            __builtin_amdgcn_sched_barrier(0);
-            if (!seen_whole(reach, steps.key(t))) hide(t);
-            raise(maximum());
-        };
-        next_scores(t0);
-        for (int t = t0; t < t1; ++t) {
+        scores();
+        settle(t0, highest(0));
+        auto step = [&](int t, auto more) {
             // K of step t + 1 and V of step t have landed (K of step t + 2,
             // fetched behind them, may not have), and every wave is through
             // with the slots that the next DMAs fill.
             vm_wait_stages<T::DMAS>(1);
-            if (!seen_whole(block, steps.key(t))) tame(t);
+            if (!all_whole.has(t)) tame(v_read);
             lds_wait();
             bare_barrier();
-            fetch_v(t + 1);
-            fetch_k(t + 3);
+            bf16x8 first[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) first[d] = v_at(0, d);
+            fetch_v();
+            fetch_k();
             weigh();
-            // The other workgroup's wave of this SIMD leaves the matrix pipe to
-            // the one that is at its products (3% fewer cycles).
+            // The other workgroup's wave of this SIMD leaves the matrix pipe
+            // to the one that is at its products (3% fewer cycles).
             __builtin_amdgcn_s_setprio(1);
-            products(t);
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < t1) next_scores(t + 1);
+            const float top = multiply(first, more);
+            if constexpr (decltype(more)::value) settle(t + 1, top);
             __builtin_amdgcn_s_setprio(0);
-        }
+        };
+        for (int t = t0; t < t1 - 1; ++t) step(t, std::true_type{});
+        step(t1 - 1, std::false_type{});
         vm_wait_stages<T::DMAS>(0);
         // Behind the wave's output rows below.
         int* flags = reinterpret_cast<int*>(lds + tile_lds_bytes<D>() - 64);
@@ -377,7 +441,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
 #pragma unroll 1
             for (int t = t0; t < t1; ++t) {
                 const int kb = steps.key(t);
-                if (seen_whole(block, kb)) continue;
+                if (all_whole.has(t)) continue;
 #pragma unroll 1
                 for (int key = kb; key < kb + kTileStep && key < limit; ++key) {
                     const bool ok = sees(sight, task.seg + key, p.sinks);
