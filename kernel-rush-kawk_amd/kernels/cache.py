@@ -132,7 +132,8 @@ class DecodeCache:
 
     def rollback(self, rows: list) -> None:
         """Forget the last ``rows[b]`` slots of each sequence: the rejected rows
-        of a verified draft, behind the accepted ones."""
+        of a verified draft, behind the accepted ones.  What they added to the
+        scores of the keys before them stays."""
         if len(rows) != self.B or any(not 0 <= n <= c[0] for n, c in zip(rows, self._host)):
             raise ValueError(f"rollback needs 0 .. slots rows for each of {self.B} sequences, got {list(rows)}")
         less = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
