@@ -68,8 +68,13 @@ __device__ __forceinline__ int seq_len(const AttnParams& p, int b) {
     return n < 0 ? 0 : n > p.capacity ? p.capacity : n;
 }
 
-// Row r of sequence b, whose cache holds len keys.
-__device__ __forceinline__ RowSight row_sight(const AttnParams& p, int b, int r, int len) {
+// The tree masks of row r of sequence b.
+__device__ __forceinline__ uint64_t tree_bits(const AttnParams& p, int b, int r) {
+    return p.tree ? (uint64_t)p.tree[(int64_t)b * p.R + r] : 0;
+}
+
+// Row r of a sequence whose cache holds len keys.
+__device__ __forceinline__ RowSight row_sight(const AttnParams& p, int r, int len, uint64_t bits) {
     RowSight s;
     const int slot = len - p.R + r;
     s.first = p.prefix + len - p.R;
@@ -77,8 +82,7 @@ __device__ __forceinline__ RowSight row_sight(const AttnParams& p, int b, int r,
     int pos = p.prefix + slot;
     s.hi = pos;
     if (p.tree) {
-        s.bits = (uint64_t)p.tree[(int64_t)b * p.R + r];
-        if (p.R < 64) s.bits &= (1ull << p.R) - 1;
+        s.bits = p.R < 64 ? bits & ((1ull << p.R) - 1) : bits;
         const int none = p.R - len;  // the first rows, which have no slot
         if (none > 0) s.bits = none < 64 ? s.bits >> none << none : 0;
         const int cached = p.prefix + (none > 0 ? 0 : -none);
@@ -181,11 +185,12 @@ __device__ __forceinline__ Task task_of(const AttnParams& p, int id, int own_row
     return t;
 }
 
-// Row `row` of a task's list (the last one again behind its end): what it
-// sees, and where its q is.
+// Row `row` of a task's list (the last one again behind its end), and what it
+// takes to say what the row sees.
 struct TaskRow {
-    int b, r, head;
-    RowSight sight;
+    int b, r, head, len;
+    uint64_t bits;
+    __device__ __forceinline__ RowSight sight(const AttnParams& p) const { return row_sight(p, r, len, bits); }
 };
 __device__ __forceinline__ TaskRow task_row(const AttnParams& p, const Task& t, int row) {
     TaskRow x;
@@ -194,7 +199,8 @@ __device__ __forceinline__ TaskRow task_row(const AttnParams& p, const Task& t, 
     const int jj = t.shared ? j - x.b * p.RG : j;
     x.r = jj / p.G;
     x.head = t.h * p.G + (jj - x.r * p.G);
-    x.sight = row_sight(p, x.b, x.r, t.shared ? seq_len(p, x.b) : t.limit);
+    x.len = t.shared ? seq_len(p, x.b) : t.limit;
+    x.bits = tree_bits(p, x.b, x.r);
     return x;
 }
 
@@ -235,6 +241,18 @@ struct Reach {
         return __builtin_amdgcn_readfirstlane(v);
     }
 };
+
+// The same from the lengths alone, of all of a task's rows; not for a shared
+// prefix with a window, where it takes every sequence's.
+__device__ __forceinline__ Reach reach_at_most(const AttnParams& p, const Task& t) {
+    Reach r;
+    const int first = t.limit - p.R > 0 ? t.limit - p.R : 0;  // slot of the first row that has one
+    r.hi_max = t.seg + t.limit - 1;
+    // A row with tree masks may lie one position before the first.
+    const int lo = p.window ? t.seg + first - (p.tree ? 1 : 0) - p.window + 1 : 0;
+    r.lo_min = lo > 0 ? lo : 0;
+    return r;
+}
 
 // A task's keys in steps of STEP: those that hold sinks, then from the first
 // key that some row's window holds to the last that some row sees.  The task

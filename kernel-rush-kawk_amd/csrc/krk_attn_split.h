@@ -44,22 +44,39 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
 
     const int limit = task.limit;
 
-    // This lane's rows: what they see, and their q.
+    // This lane's rows, and their q.  Loads first: what the rows see is worked
+    // out while the first keys are on their way.
+    TaskRow rows[MT];
     RowSight sight[MT];
     u32x4 qf[MT][KS];
-    Reach reach;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int row = task.row0 + 16 * i + n16;
-        const TaskRow x = task_row(p, task, row);
-        sight[i] = x.sight;
-        reach.add(x.sight, row < task.rows);
-        const uint16_t* qr = p.q + ((int64_t)x.b * p.R + x.r) * p.q_row + (int64_t)x.head * D + 8 * q4;
+        rows[i] = task_row(p, task, task.row0 + 16 * i + n16);
+        const uint16_t* qr = p.q + ((int64_t)rows[i].b * p.R + rows[i].r) * p.q_row + (int64_t)rows[i].head * D + 8 * q4;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[i][s] = load_cached16(qr + 32 * s);
     }
-    reach.join_lanes();
-    const KeySteps<32> steps(p, task, reach);
+    Reach reach;
+    auto see = [&]() {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            sight[i] = rows[i].sight(p);
+            reach.add(sight[i], task.row0 + 16 * i + n16 < task.rows);
+        }
+        reach.join_lanes();
+    };
+    const bool late = task.shared && p.window;
+    if (late) see();
+    const KeySteps<32> steps(p, task, late ? reach : reach_at_most(p, task));
+    KeyFrag<D> kf;
+    ValueFrag<D> vf;
+    const int t1 = steps.t1;
+    int t = steps.t0 + wave;
+    if (t < t1) {
+        kf.load(task.k, task.k_slot, steps.key(t), limit, lane);
+        vf.load(task.v, task.v_slot, steps.key(t), limit, lane);
+    }
+    if (!late) see();
 
     f32x4 acc[MT][VD];
     float m[MT], l[MT];
@@ -75,14 +92,6 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
     // it: the products run on zeros in their place, and the rows that see them
     // get them behind the last step.
     bool any_odd = false;
-    KeyFrag<D> kf;
-    ValueFrag<D> vf;
-    const int t1 = steps.t1;
-    int t = steps.t0 + wave;
-    if (t < t1) {
-        kf.load(task.k, task.k_slot, steps.key(t), limit, lane);
-        vf.load(task.v, task.v_slot, steps.key(t), limit, lane);
-    }
     for (; t < t1; t += kSplitWaves) {
         const int kb = steps.key(t);
         const int next = t + kSplitWaves;
@@ -215,11 +224,12 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
     __syncthreads();
     const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
     const bool last = p.splits + p.prefix_splits == 1;
-    constexpr int PER_ROW = D / 4;
-    for (int e = threadIdx.x; e < TR * PER_ROW; e += kSplitThreads) {
-        const int n = e / PER_ROW, d = 4 * (e % PER_ROW);
+    constexpr int PER_ROW = D / 4, ROWS = kSplitThreads / PER_ROW;
+    const int d = 4 * (threadIdx.x % PER_ROW);
+#pragma unroll
+    for (int i = 0; i < TR / ROWS; ++i) {  // unrolled: one after the other, each waits 800 cycles for LDS
+        const int n = i * ROWS + threadIdx.x / PER_ROW;
         const int row = task.row0 + n;
-        if (row >= task.rows) break;  // rows grow with e
         float mw[kSplitWaves], M = kNegInf, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kSplitWaves; ++w) {
@@ -234,14 +244,19 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
             L += f * lo_ml[w * TR + n].y;
             o += f * *reinterpret_cast<const f32x4*>(lo_o + ((size_t)w * TR + n) * LD + d);
         }
-        const int b = task.shared ? row / p.RG : task.b0;
-        const int j = task.shared ? row - b * p.RG : row;
-        if (last) {
-            finish_row(p, b, task.h, j, D, d, o, M, L);
-        } else {
+        if (row < task.rows) {
+            const int b = task.shared ? row / p.RG : task.b0;
+            const int j = task.shared ? row - b * p.RG : row;
             const int64_t g = (int64_t)task.part * all_rows + ((int64_t)b * p.kv_heads + task.h) * p.RG + j;
-            put_agent(p.part + g * D + d, o);
-            if (d == 0) put_agent(p.ml + g, make_float2(M, L));
+            if (last) {
+                finish_row(p, b, task.h, j, D, d, o, M, L);
+            } else if (p.ctr) {  // for a workgroup of this launch, maybe on another XCD
+                put_agent(p.part + g * D + d, o);
+                if (d == 0) put_agent(p.ml + g, make_float2(M, L));
+            } else {
+                *reinterpret_cast<f32x4*>(p.part + g * D + d) = o;
+                if (d == 0) p.ml[g] = make_float2(M, L);
+            }
         }
     }
 }
@@ -476,7 +491,8 @@ __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
                     w[e] = __builtin_fmaf(exp2_raw(__builtin_fmaf(s[e >> 2][e & 3], p.c, -now.x)), now.y, w[e]);
             } else {
                 const int j = row0 + i0 + n16;
-                const RowSight sight = row_sight(p, b, (j < p.RG ? j : p.RG - 1) / p.G, len);
+                const int r = (j < p.RG ? j : p.RG - 1) / p.G;
+                const RowSight sight = row_sight(p, r, len, tree_bits(p, b, r));
                 // A row that sees nothing (or is none) adds nothing, whatever its q.
                 const bool adds = now.y != 0.0f;
 #pragma unroll

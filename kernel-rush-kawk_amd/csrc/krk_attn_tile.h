@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
 
     const int my_row = task.row0 + wave * 32 + n32;
     const TaskRow mine = task_row(p, task, my_row);
-    const RowSight sight = mine.sight;
+    const RowSight sight = mine.sight(p);
     bf16x8 qf[KS];
     Reach reach;  // of this wave's rows
     Reach block;  // of the workgroup's
