@@ -141,6 +141,7 @@ struct Plan {
     Cut own, prefix;
     int64_t all_rows;
     bool join_in_kernel;
+    bool join_prefix;  // the own caches' launch joins the prefix's ranges
     bool keep_raw;  // scored: q.k goes through the workspace instead of K being read again
     int64_t raw_row;
     size_t ctr, part, ml, stat, raw, bytes;  // workspace: sizes of its parts and their sum
@@ -184,6 +185,10 @@ Plan make_plan(const krk_attn_shape& s) {
         // join all sequences of its rows, one after the other (8 of them, 8 us).
         p.join_in_kernel = p.own.rows <= 32 && !s.prefix && RG * n * s.head_dim <= 24 << 10;
         if (p.join_in_kernel) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
+        // A launch of its own behind the prefix's anyway, in whole caches of single
+        // rows: it reads the prefix's ranges under its first keys' loads (64
+        // sequences over 32768 shared keys: 91 us a call, 98 with a join behind).
+        p.join_prefix = p.prefix.rows == krk::kTileRows && p.own.rows == 16 && p.own.splits == 1;
         p.part = align_up((size_t)n * p.all_rows * s.head_dim * sizeof(float), 256);
         p.ml = align_up((size_t)n * p.all_rows * sizeof(float2), 256);
     }
@@ -198,10 +203,10 @@ Plan make_plan(const krk_attn_shape& s) {
 }
 
 // ---------------------------------------------------------------- launches
-template <int D, int MTO, int MTP>
+template <int D, int MTO, int MTP, bool JOIN = false>
 int launch_split(const krk::AttnParams& p, int64_t blocks, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    const void* fn = reinterpret_cast<const void*>(&krk::attn_split_kernel<D, MTO, MTP>);
+    const void* fn = reinterpret_cast<const void*>(&krk::attn_split_kernel<D, MTO, MTP, JOIN>);
     const size_t shm = krk::split_lds_bytes<D, (MTO > MTP ? MTO : MTP)>();
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "attn_split_kernel LDS size");
     void* args[] = {(void*)&p};
@@ -232,7 +237,11 @@ int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
         rc = launch_tile<D>(p, shared, stream);
         krk::AttnParams o = p;
         o.prefix_row_tiles = 0;
-        if (!rc) rc = plan.own.rows == 32 ? launch_split<D, 2, 2>(o, own, stream) : launch_split<D, 1, 1>(o, own, stream);
+        if (!rc) {
+            if (plan.own.rows == 32) rc = launch_split<D, 2, 2>(o, own, stream);
+            else if (plan.join_prefix) rc = launch_split<D, 1, 1, true>(o, own, stream);
+            else rc = launch_split<D, 1, 1>(o, own, stream);
+        }
     } else if (plan.own.rows == 32) {
         rc = launch_split<D, 2, 2>(p, own + shared, stream);
     } else if (plan.prefix.rows == 32) {
@@ -241,7 +250,7 @@ int launch_attn(krk::AttnParams p, const Plan& plan, hipStream_t stream) {
         rc = launch_split<D, 1, 1>(p, own + shared, stream);
     }
     if (rc) return rc;
-    if (plan.own.splits + plan.prefix.splits > 1 && !plan.join_in_kernel) {
+    if (plan.own.splits + plan.prefix.splits > 1 && !plan.join_in_kernel && !plan.join_prefix) {
         const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::attn_join_kernel<D>),
                                              dim3((unsigned)cdiv(plan.all_rows, 256 / (D / 4) / krk::kGroups)), dim3(256), args, 0, stream);
         if (int rc = hip_status(e, "attn_join_kernel launch")) return rc;

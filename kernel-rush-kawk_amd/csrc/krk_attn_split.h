@@ -33,7 +33,49 @@ constexpr size_t split_lds_bytes() {
     return (size_t)kSplitWaves * 16 * MT * ((D + 4) * sizeof(float) + sizeof(float2));
 }
 
-template <int D, int MT>
+// Four outputs of a row over some of its key ranges, and their maximum and sum.
+struct Joined {
+    float M = kNegInf, L = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    __device__ __forceinline__ void add(const AttnParams& p, float m, float l, const f32x4& x) {
+        const float mn = fmaxf(M, m);
+        const float ms = mn == kNegInf ? 0.0f : mn;
+        const float f0 = exp2_raw((M - ms) * p.c), f1 = exp2_raw((m - ms) * p.c);
+        L = L * f0 + f1 * l;
+        o = o * f0 + f1 * x;
+        M = mn;
+    }
+};
+
+// Joins key ranges from, from + step, ... of row `row` (of all rows); kJoin
+// loads are in flight at a time.  AGENT: they were written by this launch, so
+// each is a round trip beyond this XCD's L2.
+constexpr int kJoin = 8;
+template <int D, bool AGENT>
+__device__ __forceinline__ Joined join_ranges(const AttnParams& p, int64_t row, int d, int from, int step) {
+    const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
+    const int n = p.splits + p.prefix_splits;
+    Joined y;
+    for (int s0 = from; s0 < n; s0 += kJoin * step) {
+        float2 ml[kJoin];
+        f32x4 x[kJoin];
+#pragma unroll
+        for (int s = 0; s < kJoin; ++s) {
+            const int at = s0 + s * step;
+            const int64_t g = (at < n ? at : s0) * all_rows + row;
+            ml[s] = AGENT ? get_agent(p.ml + g) : p.ml[g];
+            x[s] = AGENT ? get_agent(p.part + g * D + d) : *reinterpret_cast<const f32x4*>(p.part + g * D + d);
+        }
+#pragma unroll
+        for (int s = 0; s < kJoin; ++s)
+            if (s0 + s * step < n) y.add(p, ml[s].x, ml[s].y, x[s]);
+    }
+    return y;
+}
+
+// JOIN: the prefix's ranges were taken by an earlier launch and this workgroup's
+// is all of the own cache; it joins them.
+template <int D, int MT, bool JOIN>
 __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task, unsigned char* lds) {
     constexpr int TR = 16 * MT;
     constexpr int KS = D / 32;
@@ -77,6 +119,20 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
         vf.load(task.v, task.v_slot, steps.key(t), limit, lane);
     }
     if (!late) see();
+
+    // Of the merge at the end: this thread's outputs of rows i * ROWS + ...
+    constexpr int PER_ROW = D / 4, ROWS = kSplitThreads / PER_ROW;
+    const int d = 4 * (threadIdx.x % PER_ROW);
+    const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
+    Joined shared[JOIN ? TR / ROWS : 1];
+    if constexpr (JOIN) {  // under the first keys' loads
+#pragma unroll
+        for (int i = 0; i < TR / ROWS; ++i) {
+            const int row = task.row0 + i * ROWS + threadIdx.x / PER_ROW;
+            if (row < task.rows)
+                shared[i] = join_ranges<D, false>(p, ((int64_t)task.b0 * p.kv_heads + task.h) * p.RG + row, d, p.splits, 1);
+        }
+    }
 
     f32x4 acc[MT][VD];
     float m[MT], l[MT];
@@ -222,10 +278,7 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
                     f32x4{acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]};
     }
     __syncthreads();
-    const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
     const bool last = p.splits + p.prefix_splits == 1;
-    constexpr int PER_ROW = D / 4, ROWS = kSplitThreads / PER_ROW;
-    const int d = 4 * (threadIdx.x % PER_ROW);
 #pragma unroll
     for (int i = 0; i < TR / ROWS; ++i) {  // unrolled: one after the other, each waits 800 cycles for LDS
         const int n = i * ROWS + threadIdx.x / PER_ROW;
@@ -248,7 +301,10 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
             const int b = task.shared ? row / p.RG : task.b0;
             const int j = task.shared ? row - b * p.RG : row;
             const int64_t g = (int64_t)task.part * all_rows + ((int64_t)b * p.kv_heads + task.h) * p.RG + j;
-            if (last) {
+            if constexpr (JOIN) {
+                shared[i].add(p, M, L, o);
+                finish_row(p, b, task.h, j, D, d, shared[i].o, shared[i].M, shared[i].L);
+            } else if (last) {
                 finish_row(p, b, task.h, j, D, d, o, M, L);
             } else if (p.ctr) {  // for a workgroup of this launch, maybe on another XCD
                 put_agent(p.part + g * D + d, o);
@@ -259,46 +315,6 @@ __device__ __forceinline__ void split_task(const AttnParams& p, const Task& task
             }
         }
     }
-}
-
-// Four outputs of a row over some of its key ranges, and their maximum and sum.
-struct Joined {
-    float M = kNegInf, L = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    __device__ __forceinline__ void add(const AttnParams& p, float m, float l, const f32x4& x) {
-        const float mn = fmaxf(M, m);
-        const float ms = mn == kNegInf ? 0.0f : mn;
-        const float f0 = exp2_raw((M - ms) * p.c), f1 = exp2_raw((m - ms) * p.c);
-        L = L * f0 + f1 * l;
-        o = o * f0 + f1 * x;
-        M = mn;
-    }
-};
-
-// Joins key ranges from, from + step, ... of row `row` (of all rows); kJoin
-// loads are in flight at a time.  AGENT: they were written by this launch, so
-// each is a round trip beyond this XCD's L2.
-constexpr int kJoin = 8;
-template <int D, bool AGENT>
-__device__ __forceinline__ Joined join_ranges(const AttnParams& p, int64_t row, int d, int from, int step) {
-    const int64_t all_rows = (int64_t)p.B * p.kv_heads * p.RG;
-    const int n = p.splits + p.prefix_splits;
-    Joined y;
-    for (int s0 = from; s0 < n; s0 += kJoin * step) {
-        float2 ml[kJoin];
-        f32x4 x[kJoin];
-#pragma unroll
-        for (int s = 0; s < kJoin; ++s) {
-            const int at = s0 + s * step;
-            const int64_t g = (at < n ? at : s0) * all_rows + row;
-            ml[s] = AGENT ? get_agent(p.ml + g) : p.ml[g];
-            x[s] = AGENT ? get_agent(p.part + g * D + d) : *reinterpret_cast<const f32x4*>(p.part + g * D + d);
-        }
-#pragma unroll
-        for (int s = 0; s < kJoin; ++s)
-            if (s0 + s * step < n) y.add(p, ml[s].x, ml[s].y, x[s]);
-    }
-    return y;
 }
 
 // Joins all rows of (b, h) with the whole workgroup: every four outputs of a
@@ -342,14 +358,14 @@ __device__ __forceinline__ void join_rows(const AttnParams& p, int b, int h, uns
 // prefix), the workgroup that finishes last for a sequence and head does it: no
 // second launch (one decode row over 1000 keys: 13.3 us a call in two launches,
 // 9.1 in one).
-template <int D, int MTO, int MTP>
+template <int D, int MTO, int MTP, bool JOIN>
 __global__ void __launch_bounds__(kSplitThreads, 2) attn_split_kernel(AttnParams p) {
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int last;
     const Task task = task_of(p, blockIdx.x, 16 * MTO, 16 * MTP);
-    if (MTO == MTP || !task.shared) split_task<D, MTO>(p, task, lds);
-    else split_task<D, MTP>(p, task, lds);
-    if (!p.ctr) return;
+    if (MTO == MTP || !task.shared) split_task<D, MTO, JOIN>(p, task, lds);
+    else split_task<D, MTP, false>(p, task, lds);
+    if (JOIN || !p.ctr) return;
     drain_memory();
     __syncthreads();
     uint32_t* ctr = p.ctr + (int64_t)task.b0 * p.kv_heads + task.h;

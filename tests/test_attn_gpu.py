@@ -174,6 +174,9 @@ def test_prompt(device, B, R, heads, kv, D, cap, lens, window, sinks):
     (40, 1, 32, 8, 128, 33, [1 + b % 33 for b in range(40)], 300, None, 0, 0, False),
     (6, 8, 16, 4, 64, 100, [100, 8, 60, 9, 7, 50], 500, None, 77, 5, True),
     (2, 40, 8, 2, 128, 64, [64, 45], 130, None, 0, 0, False),
+    (70, 1, 16, 8, 64, 200, [1 + 53 * b % 200 for b in range(69)] + [0], 500, None, 0, 0, False),
+    (64, 2, 8, 4, 128, 150, [2 + 37 * b % 149 for b in range(63)] + [1], 333, 400, 60, 5, False),
+    (33, 4, 8, 8, 128, 300, [4 + 41 * b % 297 for b in range(33)], 70, None, 0, 0, True),
 ])
 def test_shared_prefix(device, B, R, heads, kv, D, cap, lens, prefix, built, window, sinks, tree):
     check_attention(device, 500 + B, B, R, heads, kv, D, cap, lens, prefix=prefix, built_prefix=built, window=window,
