@@ -185,8 +185,8 @@ Plan make_plan(const krk_attn_shape& s) {
         // join all sequences of its rows, one after the other (8 of them, 8 us).
         p.join_in_kernel = p.own.rows <= 32 && !s.prefix && RG * n * s.head_dim <= 24 << 10;
         if (p.join_in_kernel) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
-        // A launch of its own behind the prefix's anyway, in whole caches of single
-        // rows: it reads the prefix's ranges under its first keys' loads (64
+        // A launch of its own behind the prefix's anyway, in whole caches of up to 16
+        // rows a head: it reads the prefix's ranges under its first keys' loads (64
         // sequences over 32768 shared keys: 91 us a call, 98 with a join behind).
         p.join_prefix = p.prefix.rows == krk::kTileRows && p.own.rows == 16 && p.own.splits == 1;
         p.part = align_up((size_t)n * p.all_rows * s.head_dim * sizeof(float), 256);
