@@ -479,7 +479,6 @@ __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
         const int j = row0 + (int)threadIdx.x;  // the first 32 threads
         // Behind the last row: exp2(-infinity) times 0.
         st = j < p.RG && threadIdx.x < kWeightRows ? stat[j] : make_float2(__builtin_inff(), 0.0f);
-        st.x *= p.c;
     };
     fetch(0);
     for (int row0 = 0; row0 < p.RG; row0 += kWeightRows) {
@@ -506,7 +505,7 @@ __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
             if (whole) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    w[e] = __builtin_fmaf(exp2_raw(__builtin_fmaf(s[e >> 2][e & 3], p.c, -now.x)), now.y, w[e]);
+                    w[e] = __builtin_fmaf(exp2_raw((s[e >> 2][e & 3] - now.x) * p.c), now.y, w[e]);
             } else {
                 const int j = row0 + i0 + n16;
                 const int r = (j < p.RG ? j : p.RG - 1) / p.G;
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int key = kb + 8 * q4 + e;
-                    const float x = exp2_raw(__builtin_fmaf(s[e >> 2][e & 3], p.c, -now.x)) * now.y;
+                    const float x = exp2_raw((s[e >> 2][e & 3] - now.x) * p.c) * now.y;
                     w[e] += adds && key < len && sees(sight, key, p.sinks) ? x : 0.0f;
                 }
             }

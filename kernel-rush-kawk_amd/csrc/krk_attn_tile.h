@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
     }
 
     f32x16 o[DT], s[2];
-    float m = kNegInf, mc = 0.0f, l = 0.0f;
+    float m = kNegInf, l = 0.0f;
+    float ref = 0.0f;  // m, or 0 before the row has seen a key
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -319,23 +320,24 @@ __global__ void __launch_bounds__(kTileThreads, 2) attn_tile_kernel(AttnParams p
         const float mx = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
         if (__any(mx > m + slack)) {
             const float mn = fmaxf(m, mx);
-            const float ms = mn == kNegInf ? 0.0f : mn;
-            const float alpha = exp2_raw((m - ms) * p.c);
+            ref = mn == kNegInf ? 0.0f : mn;
+            const float alpha = exp2_raw((m - ref) * p.c);
             m = mn;
-            mc = ms * p.c;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
     };
-    // Its weights, rounded to bf16 as the operand of the second product.
+    // Its weights, rounded to bf16 as the operand of the second product.  The
+    // difference first: one fma of s * c - m * c would be 2% faster, but its m * c is
+    // rounded, and at scores of 10^9 that turns weights of 1 into 0 or infinity.
     u32x4 w[4];
     auto weigh = [&]() {
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-            const float a = exp2_raw(__builtin_fmaf(s[e >> 4][e & 15], p.c, -mc));
-            const float b = exp2_raw(__builtin_fmaf(s[e >> 4][(e & 15) + 1], p.c, -mc));
+            const float a = exp2_raw((s[e >> 4][e & 15] - ref) * p.c);
+            const float b = exp2_raw((s[e >> 4][(e & 15) + 1] - ref) * p.c);
             sum[0] += a;
             sum[1] += b;
             w[e >> 3][(e & 7) >> 1] = pack_bf16(a, b);

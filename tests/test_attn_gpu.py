@@ -221,6 +221,30 @@ def test_flat_and_peaked_scores(device, spread):
     check_attention(device, 661, 1, 200, 4, 2, 128, 250, [250], spread=spread)
 
 
+@pytest.mark.parametrize("R", [1, 20, 150])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e9])
+def test_huge_scores(device, R, size):
+    """Scores of up to 10^19: the highest key takes all of a row's weight, in the
+    outputs and the scores."""
+    g = gen(675)
+    heads, kv, D, cap = 4, 2, 128, 300
+    q, k, v = rnd(g, R, heads * D, scale=size), rnd(g, 1, cap, kv, D, scale=size / 10), rnd(g, 1, cap, kv, D)
+    say("huge scores", R, size)
+    op = A.CacheAttention(1, R, heads, kv, D, cap, device, scored=True)
+    s = torch.zeros((1, kv, cap), device=device)
+    out = op(q.to(device), k.to(device), v.to(device), torch.tensor([cap], dtype=torch.int32, device=device), scores=s)
+    kh = k[0].double().repeat_interleave(heads // kv, dim=1)
+    dots = torch.einsum("rhd,thd->rht", q.view(R, heads, D).double(), kh)
+    dots[~(torch.arange(cap)[None] <= torch.arange(cap - R, cap)[:, None])[:, None].expand(R, heads, cap)] = -math.inf
+    two = dots.topk(2, dim=-1)
+    # fp32 sums of 128 products of up to (4 * size) * (4 * size / 10): off by less than 2^-9 of size^2 each.
+    clear = two.values[..., 0] - two.values[..., 1] > size * size * 2.0 ** -8 + 1000
+    assert clear.float().mean() > 0.9
+    want = v[0].repeat_interleave(heads // kv, dim=1)[two.indices[..., 0], torch.arange(heads)]
+    assert torch.equal(out.cpu().view(R, heads, D)[clear], want[clear])
+    assert out.isfinite().all() and abs(float(s.sum()) - R * heads) <= 1e-3 * R * heads
+
+
 @pytest.mark.parametrize("R", [1, 4, 150])
 def test_other_scales(device, R):
     check_attention(device, 670, 1, R, 8, 2, 64, 300, [222], scale=1.0)
