@@ -49,6 +49,13 @@ _current = torch._C._cuda_getDevice
 _NO_CACHE = (0, 0, 0, 0)
 
 
+def _ints(**sizes) -> None:
+    """Sizes that fit the structs' ints (which would take others modulo 2^32)."""
+    for name, n in sizes.items():
+        if not isinstance(n, int) or not -1 << 31 <= n < 1 << 31:
+            raise ValueError(f"{name} must be an int of 32 bits, got {n!r}")
+
+
 def _launch(fn, index: int, *args) -> None:
     """``fn(*args, stream)`` on GPU ``index`` and torch's current stream there."""
     stream = _raw_stream(index)
@@ -156,6 +163,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.T
     the rows' slots.  Rows without a slot, or whose position is outside the
     table, leave ``q_out`` and the cache as they were."""
     index = _index("qkv", qkv)
+    if not 0.0 <= eps <= 3e38:
+        raise ValueError(f"eps={eps} must be finite and >= 0")
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a [B, capacity, kv_heads, head_dim] tensor")
     if not isinstance(table, torch.Tensor) or table.dim() != 2:
@@ -202,13 +211,17 @@ class CacheAttention:
 
     def __init__(self, B: int, R: int, heads: int, kv_heads: int, head_dim: int, capacity: int, device, *,
                  window: int = 0, sinks: int = 0, prefix: int = 0, scored: bool = False, scale: float | None = None):
+        _ints(B=B, R=R, heads=heads, kv_heads=kv_heads, head_dim=head_dim, capacity=capacity, window=window, sinks=sinks,
+              prefix=prefix)
+        if scale is not None and not 0.0 < scale <= 3e38:
+            raise ValueError(f"scale={scale} must be positive and finite")
         self.B, self.R, self.heads, self.kv_heads, self.head_dim = B, R, heads, kv_heads, head_dim
         self.capacity, self.window, self.sinks, self.prefix, self.scored = capacity, window, sinks, prefix, bool(scored)
         self.device = torch.device(device)
-        self.scale = float(head_dim ** -0.5 if scale is None else scale)
         self._shape = AttnShape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, int(self.scored))
         lib = _lib.load()
         _lib.check(lib.krk_attn_check(_byref(self._shape)))
+        self.scale = float(head_dim ** -0.5 if scale is None else scale)
         nbytes = int(lib.krk_attn_workspace_bytes(_byref(self._shape)))
         self._q_shape = (B * R, heads * head_dim)
         self._cache_shape = (B, capacity, kv_heads, head_dim)
@@ -296,6 +309,7 @@ class CacheEviction:
 
     def __init__(self, B: int, kv_heads: int, head_dim: int, capacity: int, budget: int, device, *, sinks: int = 0,
                  recent: int = 0):
+        _ints(B=B, kv_heads=kv_heads, head_dim=head_dim, capacity=capacity, budget=budget, sinks=sinks, recent=recent)
         if not 1 <= budget <= capacity:
             raise ValueError(f"budget={budget} must be 1 .. capacity={capacity}")
         if sinks < 0 or recent < 0 or sinks + recent > budget:

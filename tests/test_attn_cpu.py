@@ -86,6 +86,25 @@ def test_shapes_refused(lib, kw, msg):
             A.CacheAttention(*d.values(), "cpu", scored=bool(kw.get("scored")), **opts)
 
 
+@pytest.mark.parametrize("kw,msg", [
+    (dict(window=1 << 32), "window"), (dict(capacity=(1 << 32) + 500), "capacity"), (dict(R=1.0), "R must"),
+    (dict(B=None), "B must"), (dict(prefix="3"), "prefix"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=1e300), "scale"),
+    (dict(head_dim=0), "64 and 128"),
+])
+def test_sizes_that_do_not_fit(kw, msg):
+    d = dict(B=2, R=1, heads=8, kv_heads=2, head_dim=128, capacity=500, device="cpu")
+    with pytest.raises(ValueError, match=msg):
+        A.CacheAttention(**{**d, **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(budget=1 << 32, capacity=1 << 33), dict(sinks=1.5), dict(B=None), dict(recent="2")])
+def test_eviction_sizes_that_do_not_fit(kw):
+    d = dict(B=2, kv_heads=2, head_dim=128, capacity=500, budget=100, device="cpu")
+    with pytest.raises(ValueError, match="32 bits"):
+        A.CacheEviction(**{**d, **kw})
+
+
 def test_null_arguments(lib):
     assert lib.krk_attn_check(None) < 0 and lib.krk_attn_plan(None, None) < 0
     assert lib.krk_attn_bf16(None, None, None, 0, None) < 0
