@@ -147,19 +147,40 @@ struct Plan {
     size_t ctr, part, ml, stat, raw, bytes;  // workspace: sizes of its parts and their sum
 };
 
-// `lists` row lists of `rows` rows each, over at most `keys` keys.  Key ranges:
-// one workgroup per CU, which is enough to draw 6 TB/s (32 sequences with
-// windows of 4096 keys: 89 us in one range, 96 in two, 101 in six); two where
-// sequences may differ in length (`ragged`) or several tiles of rows share their
-// keys and the matrix pipe is what counts.  But a step for every wave of the
-// split kernel and four steps of the tile kernel at least.
-Cut make_cut(int64_t rows, int64_t lists, int64_t keys, bool ragged) {
+// Key ranges of the tile kernel, where a range costs: its partial results are
+// written and read at 8 * D bytes a row.  Measured, in us: 6 and 1.45 a step (D =
+// 64: 1.05) for up to 512 workgroups, 4 for the join and the partial results at
+// 3.5 TB/s.  s ranges then take 6 + T / s + 4 + C * s, least at sqrt(T / C), but
+// not more than 512 workgroups, and not so many that only some CUs have two
+// (3500 rows of 4 heads: 56 us in 2 ranges, 51 in 4; 2000 rows of 32 heads: 91 in
+// one, 126 in 2; 100 rows of 32 heads over 4000 keys: 39 in 4, 33 in 8 and 16).
+int tile_splits(int64_t rows, int64_t tiles, int64_t keys, int D) {
+    const double T = (double)cdiv(keys, krk::kTileStep) * (D == 128 ? 1.45 : 1.05);
+    const double C = (double)rows * D * 8 / 3.5e6;
+    const int64_t full = 2 * kCuCount / tiles, half = kCuCount / tiles;
+    const int64_t most = cdiv(keys, 4 * krk::kTileStep);
+    int64_t s = (int64_t)__builtin_sqrt(T / C);
+    s = s < full ? s : full;
+    if (s < full && s > half) s = half;
+    s = s < most ? s : most;
+    return s > 1 && T / s + 4 + C * s < T ? (int)s : 1;
+}
+
+// `lists` row lists of `rows` rows each, over at most `keys` keys.  Key ranges of
+// the split kernel: one workgroup per CU, which is enough to draw 6 TB/s (32
+// sequences with windows of 4096 keys: 89 us in one range, 96 in two, 101 in six);
+// two where sequences may differ in length (`ragged`).  But a step for every wave
+// at least.
+Cut make_cut(int64_t rows, int64_t lists, int64_t keys, bool ragged, int D) {
     Cut c;
     c.rows = rows <= 16 ? 16 : rows <= 64 ? 32 : krk::kTileRows;
     c.tiles = (int)cdiv(rows, c.rows);
-    const bool two = c.rows == 16 ? ragged : c.rows == krk::kTileRows && c.tiles > 1;
-    const int64_t want = cdiv(kCuCount * (two ? 2 : 1), lists * c.tiles);
-    const int64_t most = cdiv(keys, c.rows <= 32 ? 32 * krk::kSplitWaves : 4 * krk::kTileStep);
+    if (c.rows == krk::kTileRows) {
+        c.splits = tile_splits(rows * lists, lists * c.tiles, keys, D);
+        return c;
+    }
+    const int64_t want = cdiv(kCuCount * (c.rows == 16 && ragged ? 2 : 1), lists * c.tiles);
+    const int64_t most = cdiv(keys, 32 * krk::kSplitWaves);
     c.splits = (int)(want < most ? want : most);
     return c;
 }
@@ -170,14 +191,15 @@ Plan make_plan(const krk_attn_shape& s) {
     p.all_rows = RG * s.B * s.kv_heads;
     int64_t keys = s.capacity;
     if (s.window) {
-        const int64_t near = (int64_t)s.window + s.sinks + s.R + 64;
+        const int64_t G = s.heads / s.kv_heads, span = krk::kTileRows / G + 2;  // positions of a workgroup's rows
+        const int64_t near = (int64_t)s.window + s.sinks + (s.R < span ? s.R : span) + 64;
         keys = near < keys ? near : keys;
     }
-    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, false);
+    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, false, s.head_dim);
     // In one launch with the prefix's, the own caches' workgroups have half of
     // the chip's places.
     const bool alone = p.prefix.rows == 0 || p.prefix.rows == krk::kTileRows;
-    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, alone && keys == s.capacity);
+    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, alone && keys == s.capacity, s.head_dim);
     const int n = p.own.splits + p.prefix.splits;
     if (n > 1) {
         // One workgroup joins a sequence's head: up to 96 KB of partial results.
