@@ -168,10 +168,9 @@ int tile_splits(int64_t rows, int64_t tiles, int64_t keys, int D) {
 
 // `lists` row lists of `rows` rows each, over at most `keys` keys.  Key ranges of
 // the split kernel: one workgroup per CU, which is enough to draw 6 TB/s (32
-// sequences with windows of 4096 keys: 89 us in one range, 96 in two, 101 in six);
-// two where sequences may differ in length (`ragged`).  But a step for every wave
-// at least.
-Cut make_cut(int64_t rows, int64_t lists, int64_t keys, bool ragged, int D) {
+// sequences with windows of 4096 keys: 89 us in one range, 96 in two, 101 in six;
+// of 2000 to 4000 keys: 80, 85 and 87).  But a step for every wave at least.
+Cut make_cut(int64_t rows, int64_t lists, int64_t keys, int D) {
     Cut c;
     c.rows = rows <= 16 ? 16 : rows <= 64 ? 32 : krk::kTileRows;
     c.tiles = (int)cdiv(rows, c.rows);
@@ -179,7 +178,7 @@ Cut make_cut(int64_t rows, int64_t lists, int64_t keys, bool ragged, int D) {
         c.splits = tile_splits(rows * lists, lists * c.tiles, keys, D);
         return c;
     }
-    const int64_t want = cdiv(kCuCount * (c.rows == 16 && ragged ? 2 : 1), lists * c.tiles);
+    const int64_t want = cdiv(kCuCount, lists * c.tiles);
     const int64_t most = cdiv(keys, 32 * krk::kSplitWaves);
     c.splits = (int)(want < most ? want : most);
     return c;
@@ -195,11 +194,8 @@ Plan make_plan(const krk_attn_shape& s) {
         const int64_t near = (int64_t)s.window + s.sinks + (s.R < span ? s.R : span) + 64;
         keys = near < keys ? near : keys;
     }
-    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, false, s.head_dim);
-    // In one launch with the prefix's, the own caches' workgroups have half of
-    // the chip's places.
-    const bool alone = p.prefix.rows == 0 || p.prefix.rows == krk::kTileRows;
-    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, alone && keys == s.capacity, s.head_dim);
+    if (s.prefix) p.prefix = make_cut(RG * s.B, s.kv_heads, s.prefix, s.head_dim);
+    p.own = make_cut(RG, (int64_t)s.B * s.kv_heads, keys, s.head_dim);
     const int n = p.own.splits + p.prefix.splits;
     if (n > 1) {
         // One workgroup joins a sequence's head: up to 96 KB of partial results.
