@@ -4,8 +4,8 @@
 // Bound by LDS and the matrix pipe alike: 64 keys of a wave's 32 rows are 1030
 // cycles of its SIMD's matrix pipe at head size 128 (2.1 MFLOP) and 32 KB of LDS
 // reads, 1030 cycles for a CU's four waves, and the keys' own 32 KB come on top.
-// The 2048 weights take about 700 cycles of the vector pipe.  Measured, two
-// waves of a SIMD need 3600 cycles for a step each, 865 TFLOP/s of an 8192-row
+// The 2048 weights take about 750 cycles of the vector pipe.  Measured, two
+// waves of a SIMD need 3700 cycles for a step each, 880 TFLOP/s of an 8192-row
 // prompt with a window of 2048.
 //
 // Work split.  Four waves, each with 32 rows of its own, all reading the same
