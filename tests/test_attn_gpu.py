@@ -162,6 +162,38 @@ def test_prompt(device, B, R, heads, kv, D, cap, lens, window, sinks):
     check_attention(device, 400 + R, B, R, heads, kv, D, cap, lens, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("B,R,heads,kv,D,cap,lens,window,sinks,tree,scored", [
+    (1, 70, 8, 2, 128, 2600, [2500], 0, 0, False, False),
+    (2, 40, 8, 2, 128, 2000, [1990, 701], 0, 0, False, True),
+    (1, 100, 8, 4, 64, 3000, [2900], 1500, 70, False, True),
+    (1, 64, 8, 2, 128, 2100, [2033], 0, 0, True, False),
+    (2, 64, 8, 4, 128, 2100, [2033, 70], 1900, 2, True, False),
+])
+def test_many_rows_in_key_ranges(device, B, R, heads, kv, D, cap, lens, window, sinks, tree, scored):
+    op = check_attention(device, 450 + R, B, R, heads, kv, D, cap, lens, window=window, sinks=sinks, tree=tree, scored=scored)
+    assert op.plan["rows"] == 128 and op.plan["splits"] > 1
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_nonfinite_values_in_key_ranges(device, what):
+    """As below, with the keys of 128-row workgroups in several ranges: values
+    at a window's edge and among the new rows."""
+    g = gen(710)
+    R, heads, kv, D, cap, n, window = 80, 8, 2, 128, 2400, 2303, 2000
+    q, k, v = rnd(g, R, heads * D), rnd(g, 1, cap, kv, D), rnd(g, 1, cap, kv, D)
+    for at in (250, 300, 1200, 2270):
+        v[0, at, at // 300 % 2, at % 7::16] = what
+    op = A.CacheAttention(1, R, heads, kv, D, cap, device, window=window)
+    assert op.plan["rows"] == 128 and op.plan["splits"] > 1
+    say("nonfinite in ranges", what)
+    lens = torch.tensor([n], dtype=torch.int32)
+    out = op(q.to(device), k.to(device), v.to(device), lens.to(device)).cpu().view(1, R, heads, D).double()
+    ref, _, _, size, top = R64.attention(q, k, v, lens, heads=heads, R=R, window=window)
+    fin = size.isfinite()
+    tol = torch.where(fin, R64.attention_tolerance(torch.where(fin, ref, 0), torch.where(fin, size, 0), top, D, cap, weight_half(op)), 1.0)
+    close(out, ref, tol, "out")
+
+
 @pytest.mark.parametrize("B,R,heads,kv,D,cap,lens,prefix,built,window,sinks,tree", [
     (1, 1, 8, 2, 128, 40, [3], 1, None, 0, 0, False),
     (16, 1, 8, 2, 128, 60, list(range(1, 60, 4))[:15] + [0], 333, None, 0, 0, False),
