@@ -64,6 +64,21 @@ class DecodeCache:
                                             prefix=self.prefix_keys, scored=self.scored)
         return self._ops[R]
 
+    def check(self, R: int, tree: torch.Tensor | None = None) -> None:
+        """ValueError for a step of ``R`` rows per sequence that no cache of this
+        shape takes, or for ``tree`` masks that it does not."""
+        self._op(R)
+        if tree is None:
+            return
+        if self.scored:
+            raise ValueError("scores are kept for accepted rows only: a draft tree's rows may still be rejected")
+        if R > 64 or 0 < self.window < R:
+            raise ValueError(f"tree masks need R <= 64 and a window of 0 or >= R, got R={R} window={self.window}")
+        if not isinstance(tree, torch.Tensor) or tree.dtype is not torch.int64 or tree.shape != (self.B, R):
+            raise ValueError(f"tree must be an int64 tensor of shape {(self.B, R)}")
+        if tree.device != self.lens.device or not tree.is_contiguous():
+            raise ValueError(f"tree must be contiguous and on {self.lens.device}, got {tree.device} and strides {tree.stride()}")
+
     def reserve(self, R: int) -> None:
         """Count ``R`` more rows of every sequence on the host; ValueError where
         they do not fit."""
@@ -79,22 +94,21 @@ class DecodeCache:
     def begin(self, R: int, tree: torch.Tensor | None = None, reserve: bool = True) -> None:
         """A step of ``R`` rows per sequence starts: ``lens`` and ``seen`` move
         on, and the rows' positions follow (``tree``: ancestor masks, int64
-        ``[B, R]``; a node's position is its depth below the first row's)."""
-        if tree is not None and self.scored:
-            raise ValueError("scores are kept for accepted rows only: a draft tree's rows may still be rejected")
-        op = self._op(R)
+        ``[B, R]``; a node's position is its depth below the first row's).  A
+        step that is refused leaves the cache as it was."""
+        self.check(R, tree)
         if reserve:
             self.reserve(R)
-        self.lens.add_(R)
-        self.seen.add_(R)
         dev = self.lens.device
         if tree is None:
             depth = torch.arange(R, dtype=torch.int32, device=dev)
         else:
             bits = tree[..., None] >> torch.arange(R, device=dev) & 1
             depth = bits.sum(dim=-1).int() - 1
-        self._positions = ((self.seen + (self.prefix_keys - R))[:, None] + depth).reshape(self.B * R)
-        self._tree, self._rows, self._current = tree, R, op
+        self._positions = ((self.seen + self.prefix_keys)[:, None] + depth).reshape(self.B * R)
+        self.lens.add_(R)
+        self.seen.add_(R)
+        self._tree, self._rows, self._current = tree, R, self._op(R)
 
     def attend(self, i: int, qkv: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """Layer ``i`` between its qkv and o projections: q and k normed and
@@ -136,6 +150,7 @@ class DecodeCache:
         scores of the keys before them stays."""
         if len(rows) != self.B or any(not 0 <= n <= c[0] for n, c in zip(rows, self._host)):
             raise ValueError(f"rollback needs 0 .. slots rows for each of {self.B} sequences, got {list(rows)}")
+        self._rows = 0
         less = torch.tensor(rows, dtype=torch.int32, device=self.lens.device)
         self.lens.sub_(less)
         self.seen.sub_(less)
@@ -159,6 +174,7 @@ class DecodeCache:
         return [list(c) for c in self._host], [t.clone() for t in (self.lens, self.seen, *(self.scores or ()))]
 
     def _restore(self, state: tuple) -> None:
+        self._rows = 0
         self._host = [list(c) for c in state[0]]
         for t, s in zip((self.lens, self.seen, *(self.scores or ())), state[1]):
             t.copy_(s)

@@ -101,6 +101,11 @@ class GemmStep:
             raise ValueError(f"M={M} rows for a cache of {cache.B} sequences")
         if tree is not None and cache is None:
             raise ValueError("tree masks need a cache")
+        if cache is not None:
+            cfg = m.cfg
+            if (cache.heads, cache.kv_heads, cache.head_dim, len(cache.k)) != (cfg.heads, cfg.kv_heads, cfg.head_dim, len(m.layers)):
+                raise ValueError("the cache was built for another model")
+            cache.check(M // cache.B, tree)
         self.cache, self.tree = cache, tree
         self.mm = mm if mm is not None else decode_matmuls(m, M, log, tune=tune, select_k=select_k)
         if select_k is not None and "lm_select" not in self.mm:
@@ -120,16 +125,25 @@ class GemmStep:
         return 4 * len(self.m.layers) + 1
 
     def run(self, x: torch.Tensor) -> torch.Tensor:
-        if self.cache is not None:
-            self.cache.reserve(self.M // self.cache.B)
-        return self._run(x)
+        """One step.  A step that is refused or fails leaves the cache's counts
+        as they were (a failure between layers may have added to the scores of
+        earlier keys)."""
+        cache = self.cache
+        if cache is None:
+            return self._run(x)
+        rows = self.M // cache.B
+        cache.begin(rows, self.tree)
+        try:
+            return self._run(x)
+        except BaseException:
+            cache.rollback([rows] * cache.B)
+            raise
 
     def _run(self, x: torch.Tensor) -> torch.Tensor:
+        """The step's launches, behind the cache's begin()."""
         m, mm, cache = self.m, self.mm, self.cache
         xa, xb = self.xa, self.xb
         cur, y = x, self.zero
-        if cache is not None:
-            cache.begin(self.M // cache.B, self.tree, reserve=False)
         for i, layer in enumerate(m.layers):
             qkv = mm["qkv"](cur, y, layer.in_norm, xa, layer.wqkv)
             if cache is not None:
@@ -146,24 +160,38 @@ class GemmStep:
         replay() then recomputes self.out from the current contents of x and
         attn_out, or continues the cache by the rows of x.  A cache is left as
         it was, but for slots behind its lengths."""
-        state = None
-        if self.cache is not None:
-            state = self.cache._state()
-            self.cache.reserve(self.M // self.cache.B)  # ValueError if a step does not fit
-            self.cache._restore(state)
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(s):
-            for _ in range(2):
-                self._run(x)
-                if state is not None:
-                    self.cache._restore(state)
-        torch.cuda.current_stream().wait_stream(s)
-        torch.cuda.synchronize()
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            self.out = self._run(x)
-        self.graph = g
+        cache, state = self.cache, None
+        if cache is not None:
+            rows = self.M // cache.B
+            cache.check(rows, self.tree)
+            state = cache._state()
+            cache.reserve(rows)  # ValueError if a step does not fit
+            cache._restore(state)
+
+        def step():
+            if cache is not None:
+                cache.begin(rows, self.tree, reserve=False)
+            return self._run(x)
+
+        try:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                for _ in range(2):
+                    step()
+                    if state is not None:
+                        cache._restore(state)
+            torch.cuda.current_stream().wait_stream(s)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = step()
+        except BaseException:
+            if state is not None:
+                torch.cuda.synchronize()
+                cache._restore(state)
+            raise
+        self.graph, self.out = g, out
         return g
 
     def replay(self) -> torch.Tensor:
@@ -171,6 +199,7 @@ class GemmStep:
             raise RuntimeError("capture() first")
         if self.cache is not None:
             self.cache.reserve(self.M // self.cache.B)
+            self.cache._rows = 0
         self.graph.replay()
         return self.out
 

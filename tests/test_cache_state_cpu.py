@@ -1,0 +1,98 @@
+"""What a DecodeCache counts, without a GPU: refused and failed steps leave it
+as it was."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from kernels import cache as C
+from kernels import step as S
+
+BF = torch.bfloat16
+
+
+def model(layers=2, heads=4, kv_heads=2, hidden=16):
+    cfg = S.QwenConfig(hidden=hidden, intermediate=32, layers=layers, heads=heads, kv_heads=kv_heads, head_dim=128, vocab=10)
+    ones = torch.ones(128, dtype=BF)
+    layer = SimpleNamespace(in_norm=None, post_norm=None, wqkv=None, wo=None, wgu=None, wd=None, q_norm=ones, k_norm=ones)
+    return SimpleNamespace(cfg=cfg, device=torch.device("cpu"), layers=[layer] * layers, lm_head=None, final_norm=None)
+
+
+def projections(m, M, fail=None):
+    """Stand-ins for the five projections; the one named ``fail`` raises."""
+    cols = {"qkv": (m.cfg.heads + 2 * m.cfg.kv_heads) * 128, "o": m.cfg.hidden, "gu": m.cfg.intermediate, "d": m.cfg.hidden,
+            "lm": m.cfg.vocab}
+
+    def make(name):
+        def call(*_):
+            if name == fail:
+                raise ValueError(f"{name} refused")
+            return torch.zeros((M, cols[name]), dtype=BF)
+        return call
+
+    return {name: make(name) for name in cols}
+
+
+def counts(c):
+    return c.lens.tolist(), c.seen.tolist(), [list(h) for h in c._host]
+
+
+def masks(B, R, **kw):
+    return torch.ones((B, R), **{"dtype": torch.int64, **kw})
+
+
+@pytest.mark.parametrize("kw,R,tree,msg", [
+    (dict(scored=True), 2, masks(2, 2), "draft tree"),
+    ({}, 65, masks(2, 65), "64"),
+    (dict(window=3), 4, masks(2, 4), "window"),
+    ({}, 2, masks(2, 3), "tree"),
+    ({}, 2, masks(1, 2), "tree"),
+    ({}, 2, masks(2, 2, dtype=torch.int32), "tree"),
+    ({}, 2, masks(2, 4)[:, ::2], "contiguous"),
+    ({}, 2, [[1, 3], [1, 3]], "tree"),
+    ({}, 70000, None, "too large"),
+])
+def test_refused_steps_leave_the_cache(kw, R, tree, msg):
+    m = model()
+    c = C.DecodeCache(m, 2, 100000 if R > 100 else 200, **kw)
+    c.begin(5)
+    before = counts(c)
+    with pytest.raises(ValueError, match=msg):
+        c.begin(R, tree=tree)
+    assert counts(c) == before == ([5, 5], [5, 5], [[5, 5], [5, 5]])
+    x = torch.zeros((2 * R, 16), dtype=BF)
+    with pytest.raises(ValueError, match=msg):
+        S.GemmStep(m, 2 * R, mm=projections(m, 2 * R), cache=c, tree=tree).run(x)
+    step = S.GemmStep(m, 2 * R, mm=projections(m, 2 * R), cache=c) if R < 70000 else None
+    for call in (step.run, step.capture) if step else ():
+        step.tree = tree
+        with pytest.raises(ValueError, match=msg):
+            call(x)
+        assert counts(c) == before
+
+
+@pytest.mark.parametrize("fail", ["qkv", "attend"])
+def test_failed_steps_leave_the_cache(fail):
+    """A projection or an operator that raises behind begin() (here: CPU tensors
+    are refused by every operator)."""
+    m = model()
+    c = C.DecodeCache(m, 2, 20)
+    c.begin(5)
+    before = counts(c)
+    step = S.GemmStep(m, 6, mm=projections(m, 6, fail), cache=c)
+    with pytest.raises(ValueError, match="refused" if fail == "qkv" else "GPU"):
+        step.run(torch.zeros((6, 16), dtype=BF))
+    assert counts(c) == before
+    with pytest.raises(RuntimeError, match="begin"):
+        c.attend(0, None, None)
+    c.begin(15)  # all of the room is still there
+
+
+def test_a_step_of_another_model_is_refused():
+    c = C.DecodeCache(model(), 2, 20)
+    for other in (model(layers=3), model(heads=8), model(kv_heads=4)):
+        with pytest.raises(ValueError, match="another model"):
+            S.GemmStep(other, 2, mm=projections(other, 2), cache=c)
