@@ -113,8 +113,9 @@ typedef struct krk_attn_args {
  * aligned (may be NULL when that is 0).  It must be zero-filled once before its
  * first use; every call leaves its counters, at the start, zero again and
  * partial results behind them.  Calls that share one workspace must be ordered
- * on one stream; for another shape it is zero-filled again first.  Results are
- * deterministic. */
+ * on one stream.  Shapes of the same B and kv_heads may share one (of the largest
+ * one's size); for another B or kv_heads it is zero-filled again first.  Results
+ * are deterministic. */
 int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* workspace, size_t workspace_bytes,
                   void* stream);
 

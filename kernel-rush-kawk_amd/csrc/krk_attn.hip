@@ -202,7 +202,6 @@ Plan make_plan(const krk_attn_shape& s) {
         // Not behind a prefix: the workgroup that finishes its last range would
         // join all sequences of its rows, one after the other (8 of them, 8 us).
         p.join_in_kernel = p.own.rows <= 32 && !s.prefix && RG * n * s.head_dim <= 24 << 10;
-        if (p.join_in_kernel) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
         // A launch of its own behind the prefix's anyway, in whole caches of up to 16
         // rows a head: it reads the prefix's ranges under its first keys' loads (64
         // sequences over 32768 shared keys: 91 us a call, 98 with a join behind).
@@ -216,7 +215,11 @@ Plan make_plan(const krk_attn_shape& s) {
         p.raw_row = (int64_t)align_up((size_t)s.capacity, 32);
         if (p.keep_raw) p.raw = align_up((size_t)p.all_rows * p.raw_row * sizeof(float), 256);
     }
-    p.bytes = p.ctr + p.part + p.ml + p.stat + p.raw;
+    p.bytes = p.part + p.ml + p.stat + p.raw;
+    // The counters have their place whether this shape uses them or not: shapes of one
+    // B and kv_heads may then share a workspace without filling it again.
+    if (p.bytes) p.ctr = align_up((size_t)s.B * s.kv_heads * sizeof(uint32_t), 256);
+    p.bytes += p.ctr;
     return p;
 }
 
@@ -411,7 +414,8 @@ int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* 
         w += n;
         return at;
     };
-    p.ctr = reinterpret_cast<uint32_t*>(take(plan.ctr));
+    uint32_t* ctr = reinterpret_cast<uint32_t*>(take(plan.ctr));
+    p.ctr = plan.join_in_kernel ? ctr : nullptr;
     p.part = reinterpret_cast<float*>(take(plan.part));
     p.ml = reinterpret_cast<float2*>(take(plan.ml));
     p.stat = reinterpret_cast<float2*>(take(plan.stat));

@@ -33,7 +33,7 @@ import torch
 from . import _attn_lib as _lib
 from ._attn_lib import AttnArgs, AttnPlan, AttnShape, EvictArgs, RopeArgs
 
-__all__ = ["CacheAttention", "CacheEviction", "qk_norm_rope", "rope_table"]
+__all__ = ["CacheAttention", "CacheEviction", "qk_norm_rope", "rope_table", "workspace_bytes"]
 
 _BF16 = torch.bfloat16
 _byref = ctypes.byref
@@ -195,6 +195,22 @@ def qk_norm_rope(qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.T
     return q_out
 
 
+def _attn_shape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, scored) -> AttnShape:
+    """The library's description of a shape that it takes (ValueError for others)."""
+    _ints(B=B, R=R, heads=heads, kv_heads=kv_heads, head_dim=head_dim, capacity=capacity, window=window, sinks=sinks,
+          prefix=prefix)
+    shape = AttnShape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, int(bool(scored)))
+    _lib.check(_lib.load().krk_attn_check(_byref(shape)))
+    return shape
+
+
+def workspace_bytes(B: int, R: int, heads: int, kv_heads: int, head_dim: int, capacity: int, *, window: int = 0,
+                    sinks: int = 0, prefix: int = 0, scored: bool = False) -> int:
+    """Bytes of workspace that a :class:`CacheAttention` of this shape needs."""
+    shape = _attn_shape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, scored)
+    return int(_lib.load().krk_attn_workspace_bytes(_byref(shape)))
+
+
 class CacheAttention:
     """Attention of ``R`` new rows of each of ``B`` sequences over their cache,
     for a fixed shape: ``f(q, k, v, lens) -> out``.
@@ -206,26 +222,31 @@ class CacheAttention:
     position ``prefix keys + s``.  ``scored`` objects update their keys' scores.
     ``scale`` is ``head_dim ** -0.5`` unless given.
 
-    The workspace belongs to the object.  Results are deterministic.
+    The workspace (:func:`workspace_bytes`) belongs to the object, or is
+    ``workspace``: zero-filled uint8 memory that objects of one B and kv_heads may
+    share if all their calls are ordered on one stream.  Results are deterministic.
     """
 
     def __init__(self, B: int, R: int, heads: int, kv_heads: int, head_dim: int, capacity: int, device, *,
-                 window: int = 0, sinks: int = 0, prefix: int = 0, scored: bool = False, scale: float | None = None):
-        _ints(B=B, R=R, heads=heads, kv_heads=kv_heads, head_dim=head_dim, capacity=capacity, window=window, sinks=sinks,
-              prefix=prefix)
+                 window: int = 0, sinks: int = 0, prefix: int = 0, scored: bool = False, scale: float | None = None,
+                 workspace: torch.Tensor | None = None):
+        self._shape = _attn_shape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, scored)
         if scale is not None and not 0.0 < scale <= 3e38:
             raise ValueError(f"scale={scale} must be positive and finite")
         self.B, self.R, self.heads, self.kv_heads, self.head_dim = B, R, heads, kv_heads, head_dim
         self.capacity, self.window, self.sinks, self.prefix, self.scored = capacity, window, sinks, prefix, bool(scored)
         self.device = torch.device(device)
-        self._shape = AttnShape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, int(self.scored))
-        lib = _lib.load()
-        _lib.check(lib.krk_attn_check(_byref(self._shape)))
         self.scale = float(head_dim ** -0.5 if scale is None else scale)
-        nbytes = int(lib.krk_attn_workspace_bytes(_byref(self._shape)))
+        nbytes = int(_lib.load().krk_attn_workspace_bytes(_byref(self._shape)))
         self._q_shape = (B * R, heads * head_dim)
         self._cache_shape = (B, capacity, kv_heads, head_dim)
-        self.workspace = torch.zeros(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        if workspace is None:
+            workspace = torch.zeros(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        elif workspace.dtype is not torch.uint8 or workspace.numel() < nbytes or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be {nbytes} contiguous bytes (uint8) or more, got {workspace.dtype} {tuple(workspace.shape)}")
+        elif workspace.device.type != self.device.type or self.device.index not in (None, workspace.device.index):
+            raise ValueError(f"workspace on {workspace.device}; this object is built on {self.device}")
+        self.workspace = workspace
 
     @property
     def plan(self) -> dict:

@@ -53,15 +53,23 @@ class DecodeCache:
         self.table = A.rope_table(self.max_positions, cfg.head_dim, cfg.theta, dev)
         self._host = [[0, 0] for _ in range(B)]  # slots and tokens of each sequence
         self._ops: dict = {}
+        self._workspace: torch.Tensor | None = None
         self._evictions: dict = {}
         self._rows = 0
         self._positions = self._tree = None
 
     def _op(self, R: int) -> A.CacheAttention:
+        """The attention of ``R`` rows per sequence.  Its calls are ordered by the
+        cache itself, so all row counts share one workspace.  One that needs more
+        takes at least twice as much: earlier ones, whose addresses graphs may
+        hold, add up to less than the last."""
         if R not in self._ops:
-            self._ops[R] = A.CacheAttention(self.B, R, self.heads, self.kv_heads, self.head_dim, self.capacity,
-                                            self.lens.device, window=self.window, sinks=self.sinks,
-                                            prefix=self.prefix_keys, scored=self.scored)
+            kw = dict(window=self.window, sinks=self.sinks, prefix=self.prefix_keys, scored=self.scored)
+            shape = self.B, R, self.heads, self.kv_heads, self.head_dim, self.capacity
+            need, have = A.workspace_bytes(*shape, **kw), 0 if self._workspace is None else self._workspace.numel()
+            if need > have:
+                self._workspace = torch.zeros(max(need, 2 * have), dtype=torch.uint8, device=self.lens.device)
+            self._ops[R] = A.CacheAttention(*shape, self.lens.device, workspace=self._workspace if need else None, **kw)
         return self._ops[R]
 
     def check(self, R: int, tree: torch.Tensor | None = None) -> None:

@@ -8,6 +8,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from kernels import attention as A
 from kernels import cache as C
 from kernels import step as S
 
@@ -96,3 +97,28 @@ def test_a_step_of_another_model_is_refused():
     for other in (model(layers=3), model(heads=8), model(kv_heads=4)):
         with pytest.raises(ValueError, match="another model"):
             S.GemmStep(other, 2, mm=projections(other, 2), cache=c)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(scored=True), dict(window=64, sinks=4)])
+def test_many_row_counts_share_one_workspace(kw):
+    """A thousand prompt lengths: the memory held stays below four times what the
+    largest of them needs, and every shape's counters lie in the same place."""
+    c = C.DecodeCache(model(), 3, 1500, **kw)
+    for R in [1, 700, *range(2, 1000)]:
+        c._op(R)
+    need = max(A.workspace_bytes(3, R, 4, 2, 128, 1500, **kw) for R in range(1, 1000))
+    held = {op.workspace.data_ptr(): op.workspace.numel() for op in c._ops.values() if op.workspace is not None}
+    assert need <= max(held.values()) and sum(held.values()) <= 4 * need
+
+
+def test_given_workspaces():
+    need = A.workspace_bytes(2, 1, 8, 2, 128, 5000)
+    assert need > 0 and A.workspace_bytes(2, 1, 8, 2, 128, 50) == 0
+    make = lambda ws: A.CacheAttention(2, 1, 8, 2, 128, 5000, "cpu", workspace=ws)
+    ws = torch.zeros(need + 5, dtype=torch.uint8)
+    assert make(ws).workspace is ws
+    for bad in (ws[:need - 1], ws.float(), torch.zeros(2 * need, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            make(bad)
+    with pytest.raises(ValueError, match="64 and 128"):
+        A.workspace_bytes(2, 1, 8, 2, 96, 50)

@@ -6,11 +6,12 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kernels import attention as A
 from kernels import cache as C
 from kernels import step as S
 from oracle import gemm_ref as R
 
-from test_attn_gpu import say
+from test_attn_gpu import gen, rnd, say
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,32 @@ def test_failed_captures_leave_the_cache(device, model, at):
     got, want = steps[0].replay(), steps[1].run(x)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(caches[0].lens, caches[1].lens)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(scored=True), dict(window=40, sinks=3), "prefix"])
+def test_steps_of_many_sizes_share_a_workspace(device, model, kw):
+    """Steps whose attention joins its ranges in the kernel, in a launch of its
+    own, or has one range, in turn on one workspace: each equals an object of its
+    own bit by bit."""
+    g = gen(1100)
+    B, heads, kv, D, cap = 2, 8, 2, 128, 1500
+    shared = None
+    if kw == "prefix":
+        shared, kw = tuple(rnd(g, 300, kv, D).to(device) for _ in "kv"), {}
+    cache = C.DecodeCache(model, B, cap, prefix=None if shared is None else [shared] * 2, **kw)
+    cache.k[0].copy_(rnd(g, B, cap, kv, D)), cache.v[0].copy_(rnd(g, B, cap, kv, D))
+    scores = torch.zeros((B, kv, cap), device=device)
+    for R_ in (1, 4, 100, 2, 16, 1, 33, 300, 5, 1, 100, 16, 2):
+        q = rnd(g, B * R_, heads * D).to(device)
+        own = A.CacheAttention(B, R_, heads, kv, D, cap, device, prefix=0 if shared is None else 300, **kw)
+        say("one workspace", R_, own.plan)
+        for n in (1500, 700, R_):
+            lens = torch.tensor([n, n // 2 + 1], dtype=torch.int32, device=device)
+            got, want = [], []
+            for op, to in ((cache._op(R_), got), (own, want)):
+                more = dict(scores=scores, scores_out=torch.zeros_like(scores)) if kw.get("scored") else {}
+                to.append(op(q, cache.k[0], cache.v[0], lens, prefix=shared, **more))
+                to.extend(t for name, t in more.items() if name == "scores_out")
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), (R_, n)
+    assert len({op.workspace.data_ptr() for op in cache._ops.values() if op.workspace is not None}) < len(cache._ops)
