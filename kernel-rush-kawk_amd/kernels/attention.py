@@ -21,7 +21,8 @@ shorter than R, an idle one) are padding and give zeros.
 
 Calls launch on torch's current stream, never synchronise, and may be captured
 in a graph; an object's workspace is its own, so its calls are ordered on one
-stream.  All compute runs in libkrk_attn.so; there is no fallback.
+stream.  Building an object waits until its workspace is filled (and is refused
+while a graph is captured), so its first call may come on any stream.  All compute runs in libkrk_attn.so; there is no fallback.
 """
 
 from __future__ import annotations
@@ -211,6 +212,22 @@ def workspace_bytes(B: int, R: int, heads: int, kv_heads: int, head_dim: int, ca
     return int(_lib.load().krk_attn_workspace_bytes(_byref(shape)))
 
 
+def filled(device: torch.device) -> None:
+    """Wait for the current stream, on which memory of an object was just filled:
+    its calls may come on any other."""
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+
+
+def zero_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Zero-filled memory, ready for calls on every stream when this returns."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a workspace is filled when its object is built: build it before the capture")
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    filled(device)
+    return ws
+
+
 class CacheAttention:
     """Attention of ``R`` new rows of each of ``B`` sequences over their cache,
     for a fixed shape: ``f(q, k, v, lens) -> out``.
@@ -241,7 +258,7 @@ class CacheAttention:
         self._q_shape = (B * R, heads * head_dim)
         self._cache_shape = (B, capacity, kv_heads, head_dim)
         if workspace is None:
-            workspace = torch.zeros(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+            workspace = zero_workspace(nbytes, self.device) if nbytes else None
         elif workspace.dtype is not torch.uint8 or workspace.numel() < nbytes or not workspace.is_contiguous():
             raise ValueError(f"workspace must be {nbytes} contiguous bytes (uint8) or more, got {workspace.dtype} {tuple(workspace.shape)}")
         elif workspace.device.type != self.device.type or self.device.index not in (None, workspace.device.index):

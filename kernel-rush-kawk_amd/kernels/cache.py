@@ -57,6 +57,7 @@ class DecodeCache:
         self._evictions: dict = {}
         self._rows = 0
         self._positions = self._tree = None
+        A.filled(self.lens.device)  # steps may run on another stream
 
     def _op(self, R: int) -> A.CacheAttention:
         """The attention of ``R`` rows per sequence.  Its calls are ordered by the
@@ -68,7 +69,7 @@ class DecodeCache:
             shape = self.B, R, self.heads, self.kv_heads, self.head_dim, self.capacity
             need, have = A.workspace_bytes(*shape, **kw), 0 if self._workspace is None else self._workspace.numel()
             if need > have:
-                self._workspace = torch.zeros(max(need, 2 * have), dtype=torch.uint8, device=self.lens.device)
+                self._workspace = A.zero_workspace(max(need, 2 * have), self.lens.device)
             self._ops[R] = A.CacheAttention(*shape, self.lens.device, workspace=self._workspace if need else None, **kw)
         return self._ops[R]
 

@@ -122,3 +122,15 @@ def test_given_workspaces():
             make(bad)
     with pytest.raises(ValueError, match="64 and 128"):
         A.workspace_bytes(2, 1, 8, 2, 96, 50)
+
+
+def test_building_waits_for_the_fill(monkeypatch):
+    """Every object that owns memory waits for the stream that fills it."""
+    waits = []
+    monkeypatch.setattr(A, "filled", lambda device: waits.append(str(device)))
+    A.CacheAttention(2, 1, 8, 2, 128, 5000, "cpu")
+    assert waits == ["cpu"]
+    c = C.DecodeCache(model(), 2, 5000)
+    assert len(waits) == 2
+    c.begin(1)
+    assert len(waits) == 3

@@ -87,3 +87,43 @@ def test_steps_of_many_sizes_share_a_workspace(device, model, kw):
             for a, b in zip(got, want):
                 assert torch.equal(a, b), (R_, n)
     assert len({op.workspace.data_ptr() for op in cache._ops.values() if op.workspace is not None}) < len(cache._ops)
+
+
+def test_first_calls_on_another_stream(device, model):
+    """Objects built on a stream that is busy, over memory that held other values,
+    and called at once on another: the counters are zero by then."""
+    g = gen(1110)
+    B, heads, kv, D, cap = 2, 32, 8, 128, 3000
+    k, v = rnd(g, B, cap, kv, D).to(device), rnd(g, B, cap, kv, D).to(device)
+    q = rnd(g, B, heads * D).to(device)
+    lens = torch.tensor([3000, 1700], dtype=torch.int32, device=device)
+    want = A.CacheAttention(B, 1, heads, kv, D, cap, device)(q, k, v, lens)
+    need = A.workspace_bytes(B, 1, heads, kv, D, cap)
+    busy = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    say("first call on another stream")
+    for _ in range(3):
+        with torch.cuda.stream(busy):
+            junk = torch.full((need,), 255, dtype=torch.uint8, device=device)
+            del junk
+            torch.cuda._sleep(20_000_000)
+            op = A.CacheAttention(B, 1, heads, kv, D, cap, device)
+        assert torch.equal(op(q, k, v, lens), want)
+        torch.cuda.synchronize()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(20_000_000)
+        cache = C.DecodeCache(model, 2, 40)
+    cache.begin(3)
+    assert cache.lens.tolist() == [3, 3] and cache._positions.tolist() == [0, 1, 2] * 2
+
+
+def test_no_workspace_while_a_graph_is_captured(device):
+    """Zeros that are only recorded would not be there for the next eager call."""
+    t = torch.zeros(4, device=device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            A.CacheAttention(2, 1, 32, 8, 128, 3000, device)
+    graph.replay()
+    assert t.tolist() == [1.0] * 4
