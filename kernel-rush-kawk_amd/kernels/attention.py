@@ -22,7 +22,8 @@ shorter than R, an idle one) are padding and give zeros.
 Calls launch on torch's current stream, never synchronise, and may be captured
 in a graph; an object's workspace is its own, so its calls are ordered on one
 stream.  Building an object waits until its workspace is filled (and is refused
-while a graph is captured), so its first call may come on any stream.  All compute runs in libkrk_attn.so; there is no fallback.
+while a graph is captured), so its first call may come on any stream; a graph that
+holds its calls needs the object as long as it is replayed.  All compute runs in libkrk_attn.so; there is no fallback.
 """
 
 from __future__ import annotations
@@ -264,6 +265,7 @@ class CacheAttention:
         elif workspace.device.type != self.device.type or self.device.index not in (None, workspace.device.index):
             raise ValueError(f"workspace on {workspace.device}; this object is built on {self.device}")
         self.workspace = workspace
+        self._streams: set = set()  # whose work the workspace outlives
 
     @property
     def plan(self) -> dict:
@@ -311,10 +313,20 @@ class CacheAttention:
         if ws is None:
             _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), args, 0, 0)
         elif ws.get_device() == index:
+            if _raw_stream(index) not in self._streams:
+                self._outlive(index)
             _launch(_lib.load().krk_attn_bf16, index, _byref(self._shape), args, ws.data_ptr(), ws.numel())
         else:
             raise ValueError(f"operands on {q.device}; this object was built on {self.device}")
         return out
+
+    def _outlive(self, index: int) -> None:
+        """The workspace's memory is not given to others before the current
+        stream is through with it, also where the object goes first.  (Of a
+        captured graph only its owner knows when it runs last.)"""
+        if not torch.cuda.is_current_stream_capturing():
+            self.workspace.record_stream(torch.cuda.current_stream(index))
+            self._streams.add(_raw_stream(index))
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, *,
                  prefix: tuple | None = None, tree: torch.Tensor | None = None, scores: torch.Tensor | None = None,

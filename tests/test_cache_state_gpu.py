@@ -127,3 +127,30 @@ def test_no_workspace_while_a_graph_is_captured(device):
             A.CacheAttention(2, 1, 32, 8, 128, 3000, device)
     graph.replay()
     assert t.tolist() == [1.0] * 4
+
+
+def test_an_object_that_goes_before_its_call_has_run(device):
+    """Its workspace is not given to another stream's tensors until then."""
+    g = gen(1120)
+    B, heads, kv, D, cap = 2, 32, 8, 128, 3000
+    k, v = rnd(g, B, cap, kv, D).to(device), rnd(g, B, cap, kv, D).to(device)
+    q = rnd(g, B, heads * D).to(device)
+    lens = torch.tensor([3000, 1700], dtype=torch.int32, device=device)
+    want = A.CacheAttention(B, 1, heads, kv, D, cap, device)(q, k, v, lens)
+    need = A.workspace_bytes(B, 1, heads, kv, D, cap)
+    out = torch.empty_like(want)
+    side = torch.cuda.Stream()
+    say("object gone")
+    for _ in range(3):
+        op = A.CacheAttention(B, 1, heads, kv, D, cap, device)
+        at = op.workspace.data_ptr()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            op.run(q, k, v, lens, out)
+        del op
+        other = torch.full((need,), 255, dtype=torch.uint8, device=device)
+        assert other.data_ptr() != at
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del other
