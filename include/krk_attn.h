@@ -96,7 +96,7 @@ typedef struct krk_attn_args {
     krk_cache k, v;    /* [B, capacity, kv_heads, head_dim] */
     krk_cache kp, vp;  /* [prefix, kv_heads, head_dim]; p NULL without a prefix */
     int prefix;        /* its keys in this call, 0 .. shape.prefix */
-    float scale;       /* > 0 and finite */
+    float scale;       /* > 0, at most 2.3e38 */
     const int32_t* lens;      /* [B] */
     const int64_t* tree;      /* [B, R] or NULL */
     void* out;                /* [B * R, heads * head_dim], row stride out_row (multiple of 8) */

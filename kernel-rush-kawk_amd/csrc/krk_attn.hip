@@ -347,7 +347,10 @@ int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* 
     krk_attn_args a = *args;
     if (int rc = check_shape(s)) return rc;
     if (a.prefix < 0 || a.prefix > s.prefix) return fail(KRK_ATTN_ERR_INVALID, "prefix=%d keys, the shape has 0 .. %d", a.prefix, s.prefix);
-    if (!(a.scale > 0.0f) || a.scale == __builtin_inff()) return fail(KRK_ATTN_ERR_INVALID, "scale=%g must be positive and finite", (double)a.scale);
+    // The kernels multiply by scale * log2(e).
+    const float scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+    if (!(a.scale > 0.0f) || scale_log2 == __builtin_inff())
+        return fail(KRK_ATTN_ERR_INVALID, "scale=%g must be positive and at most 2.3e38", (double)a.scale);
     if (!a.lens) return fail(KRK_ATTN_ERR_INVALID, "lens: null pointer");
     if (a.tree && (s.R > 64 || (s.window && s.window < s.R)))
         return fail(KRK_ATTN_ERR_INVALID, "tree masks need R <= 64 and a window of 0 or >= R, got R=%d window=%d", s.R, s.window);
@@ -422,7 +425,7 @@ int krk_attn_bf16(const krk_attn_shape* shape, const krk_attn_args* args, void* 
     p.raw = reinterpret_cast<float*>(take(plan.raw));
     p.raw_row = plan.raw_row;
     p.scale = a.scale;
-    p.c = (float)((double)a.scale * 1.4426950408889634);
+    p.c = scale_log2;
     p.B = s.B;
     p.R = s.R;
     p.heads = s.heads;

@@ -249,8 +249,8 @@ class CacheAttention:
                  window: int = 0, sinks: int = 0, prefix: int = 0, scored: bool = False, scale: float | None = None,
                  workspace: torch.Tensor | None = None):
         self._shape = _attn_shape(B, R, heads, kv_heads, head_dim, capacity, window, sinks, prefix, scored)
-        if scale is not None and not 0.0 < scale <= 3e38:
-            raise ValueError(f"scale={scale} must be positive and finite")
+        if scale is not None and not 1e-45 < scale <= 2.3e38:  # as an fp32, and times log2(e)
+            raise ValueError(f"scale={scale} must be positive and at most 2.3e38")
         self.B, self.R, self.heads, self.kv_heads, self.head_dim = B, R, heads, kv_heads, head_dim
         self.capacity, self.window, self.sinks, self.prefix, self.scored = capacity, window, sinks, prefix, bool(scored)
         self.device = torch.device(device)
