@@ -49,7 +49,9 @@ enum {
 
 /* A [.., slots, heads, head_dim] tensor of keys or values.  Strides in
  * elements, multiples of 8 and not negative; base 16-byte aligned; the
- * elements of a head are contiguous. */
+ * elements of a head are contiguous.  Rows of a written one may not share memory
+ * (sorted by size, each stride is at least the extent of what lies inside it);
+ * written k and v may be views of one tensor with the same strides. */
 typedef struct krk_cache {
     void* p;
     int64_t seq;  /* from sequence to sequence (ignored for a prefix) */

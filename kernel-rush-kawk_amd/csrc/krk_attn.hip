@@ -8,6 +8,7 @@
 #include <stdio.h>
 
 #include <atomic>
+#include <utility>
 
 #include "krk_attn.h"
 #include "krk_attn_split.h"
@@ -61,6 +62,21 @@ Span span(const void* p, uint64_t elems, size_t size) {
     return p ? Span{a, a + elems * size} : Span{0, 0};
 }
 
+// Whether no two elements of a written operand share memory: sorted by stride,
+// each is at least the extent of those inside it.  (Strides of extents of one
+// are 0.)
+bool nested(const int64_t (&stride)[3], const int64_t (&n)[3], int64_t inner) {
+    int at[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[at[j]] < stride[at[i]]) std::swap(at[i], at[j]);
+    for (int i : at) {
+        if (n[i] > 1 && stride[i] < inner) return false;
+        inner += (n[i] - 1) * stride[i];
+    }
+    return true;
+}
+
 // A cache of `seqs` sequences, `slots` keys, `heads` heads of `dim`.  Strides
 // of extents of one are of no matter and set to 0.
 int check_cache(const char* name, krk_cache& c, int64_t seqs, int64_t slots, int64_t heads, int dim, bool written,
@@ -76,9 +92,41 @@ int check_cache(const char* name, krk_cache& c, int64_t seqs, int64_t slots, int
             return fail(KRK_ATTN_ERR_INVALID, "%s is written: its strides must be at least head_dim=%d, got %lld", name, dim, (long long)st[i]);
         if (st[i] % 8) return fail(KRK_ATTN_ERR_ALIGN, "%s: strides must be multiples of 8 elements", name);
     }
+    if (written && !nested(st, n, dim))
+        return fail(KRK_ATTN_ERR_ALIAS, "%s is written: with strides of %lld, %lld and %lld its rows share memory", name, (long long)st[0], (long long)st[1], (long long)st[2]);
     if (reinterpret_cast<uintptr_t>(c.p) % 16) return fail(KRK_ATTN_ERR_ALIGN, "%s must be 16-byte aligned", name);
     *out = span(c.p, (uint64_t)((seqs - 1) * c.seq + (slots - 1) * c.slot + (heads - 1) * c.head + dim), 2);
     return KRK_ATTN_OK;
+}
+
+// Whether two written caches of one shape share memory.  Views whose spans meet
+// (k and v side by side in one tensor) have to have the same strides; they are
+// apart if no step from a row of one to a row of the other is shorter than a row.
+// A step's part along the largest stride is one of the two multiples next to it,
+// as what is left has to lie within the extent inside that stride.
+bool apart(int64_t d, const int64_t (&stride)[3], const int64_t (&n)[3], int dim, int level = 0) {
+    if (level == 3) return d <= -dim || d >= dim;
+    const int64_t s = stride[level];
+    if (s == 0) return apart(d, stride, n, dim, level + 1);
+    int64_t q = d / s;
+    if (q * s > d) --q;
+    for (int64_t i = q; i <= q + 1; ++i)
+        if (i > -n[level] && i < n[level] && !apart(d - i * s, stride, n, dim, level + 1)) return false;
+    return true;
+}
+bool share_memory(const krk_cache& x, const Span& xs, const krk_cache& y, const Span& ys, int64_t seqs, int64_t slots, int64_t heads,
+                  int dim) {
+    if (!overlaps(xs, ys)) return false;
+    if (x.seq != y.seq || x.slot != y.slot || x.head != y.head) return true;
+    const intptr_t bytes = reinterpret_cast<intptr_t>(y.p) - reinterpret_cast<intptr_t>(x.p);
+    int64_t stride[3] = {x.seq, x.slot, x.head}, n[3] = {seqs, slots, heads};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[j] > stride[i]) {
+                std::swap(stride[i], stride[j]);
+                std::swap(n[i], n[j]);
+            }
+    return !apart(bytes / 2, stride, n, dim);
 }
 
 // [rows, cols] operand; one row's stride is of no matter and set to its length.
@@ -101,6 +149,8 @@ int check_scores(const char* name, const void* p, int64_t& seq, int64_t& head, i
         return fail(KRK_ATTN_ERR_INVALID, "%s: strides out of range", name);
     if (written && ((seqs > 1 && seq < slots) || (heads > 1 && head < slots)))
         return fail(KRK_ATTN_ERR_INVALID, "%s is written: its strides must be at least its %lld slots", name, (long long)slots);
+    if (written && !nested({seq, head, 0}, {seqs, heads, 1}, slots))
+        return fail(KRK_ATTN_ERR_ALIAS, "%s is written: with strides of %lld and %lld its rows share memory", name, (long long)seq, (long long)head);
     if (reinterpret_cast<uintptr_t>(p) % 4) return fail(KRK_ATTN_ERR_ALIGN, "%s must be 4-byte aligned", name);
     *out = span(p, (uint64_t)((seqs - 1) * seq + (heads - 1) * head + slots), 4);
     return KRK_ATTN_OK;
@@ -467,7 +517,8 @@ int krk_qk_norm_rope_bf16(const krk_rope_args* args, void* stream) {
     const bool in_place = a.q_out == a.qkv && (M == 1 || a.q_row == a.qkv_row);
     const Span ins[5] = {span(a.q_norm, a.head_dim, 2), span(a.k_norm, a.head_dim, 2), span(a.table, (uint64_t)a.table_rows * a.head_dim, 4),
                          span(a.lens, a.B, 4), span(a.positions, M, 4)};
-    bool bad = (overlaps(q, qkv) && !in_place) || overlaps(k, qkv) || overlaps(v, qkv) || overlaps(q, k) || overlaps(q, v) || a.k.p == a.v.p;
+    bool bad = (overlaps(q, qkv) && !in_place) || overlaps(k, qkv) || overlaps(v, qkv) || overlaps(q, k) || overlaps(q, v) ||
+               share_memory(a.k, k, a.v, v, a.B, a.capacity, a.kv_heads, a.head_dim);
     for (const Span& i : ins) bad = bad || overlaps(q, i) || overlaps(k, i) || overlaps(v, i);
     if (bad) return fail(KRK_ATTN_ERR_ALIAS, "q_out (unless it is qkv in place), k and v may not share memory with each other or the inputs");
     krk::RopeParams p{static_cast<const uint16_t*>(a.qkv), a.qkv_row, static_cast<const uint16_t*>(a.q_norm),
@@ -500,9 +551,10 @@ int krk_cache_evict_bf16(const krk_evict_args* args, void* stream) {
     if (int rc = check_scores("scores", a.scores, a.sc_seq, a.sc_head, a.B, a.kv_heads, a.capacity, in_place, &in[2])) return rc;
     in[3] = span(a.lens, a.B, 4);
     const int64_t slots = in_place ? a.capacity : a.budget;
-    if (int rc = check_cache("k_out", a.k_out, a.B, slots, a.kv_heads, a.head_dim, true, &out[0])) return rc;
-    if (int rc = check_cache("v_out", a.v_out, a.B, slots, a.kv_heads, a.head_dim, true, &out[1])) return rc;
-    if (int rc = check_scores("scores_out", a.scores_out, a.so_seq, a.so_head, a.B, a.kv_heads, slots, true, &out[2])) return rc;
+    // In place the inputs were checked as written, and the outputs have to equal them.
+    if (int rc = check_cache("k_out", a.k_out, a.B, slots, a.kv_heads, a.head_dim, !in_place, &out[0])) return rc;
+    if (int rc = check_cache("v_out", a.v_out, a.B, slots, a.kv_heads, a.head_dim, !in_place, &out[1])) return rc;
+    if (int rc = check_scores("scores_out", a.scores_out, a.so_seq, a.so_head, a.B, a.kv_heads, slots, !in_place, &out[2])) return rc;
     out[3] = span(a.keep, (uint64_t)a.B * a.kv_heads * a.budget, 4);
     out[4] = span(a.lens_out, a.B, 4);
     if (a.k.p == a.v.p || a.k_out.p == a.v_out.p) return fail(KRK_ATTN_ERR_ALIAS, "k and v may not be one tensor");
@@ -512,13 +564,15 @@ int krk_cache_evict_bf16(const krk_evict_args* args, void* stream) {
                           a.scores == a.scores_out && a.sc_seq == a.so_seq && a.sc_head == a.so_head;
         if (!same) return fail(KRK_ATTN_ERR_ALIAS, "in place, k_out, v_out and scores_out are k, v and scores with their strides");
     }
+    // They may be interleaved views of one.
+    if (share_memory(a.k_out, out[0], a.v_out, out[1], a.B, slots, a.kv_heads, a.head_dim))
+        return fail(KRK_ATTN_ERR_ALIAS, "k_out and v_out may not share memory");
     for (int i = 0; i < 5; ++i)
         for (int j = 0; j < 4; ++j) {
             if (in_place && i < 3 && j < 3) continue;
             if (i == 4 && j == 3 && a.lens == a.lens_out) continue;
             if (overlaps(out[i], in[j])) return fail(KRK_ATTN_ERR_ALIAS, "the outputs may not share memory with the inputs (all in place, or lens_out == lens, aside)");
         }
-    // k_out and v_out may be interleaved views of one tensor.
     for (int i = 2; i < 5; ++i)
         for (int j = 0; j < i; ++j)
             if (overlaps(out[i], out[j])) return fail(KRK_ATTN_ERR_ALIAS, "the outputs may not overlap");
