@@ -43,6 +43,13 @@ class DecodeCache:
             raise ValueError(f"prefix: {len(prefix)} pairs for {len(m.layers)} layers")
         self.prefix = prefix
         self.prefix_keys = 0 if prefix is None else prefix[0][0].shape[0]
+        # What every step would be refused for is refused here.
+        A.workspace_bytes(B, 1, cfg.heads, cfg.kv_heads, cfg.head_dim, capacity, window=window, sinks=sinks,
+                          prefix=self.prefix_keys, scored=scored)
+        for i, pair in enumerate(prefix or ()):
+            run = (self.prefix_keys, cfg.kv_heads, cfg.head_dim)
+            if len(pair) != 2 or any(t.dtype is not _BF16 or t.shape != run or t.device.type != dev.type for t in pair):
+                raise ValueError(f"prefix of layer {i}: needs a bf16 k and v of shape {run} on {dev}, as layer 0 has")
         shape = (B, capacity, cfg.kv_heads, cfg.head_dim)
         self.k = [torch.zeros(shape, dtype=_BF16, device=dev) for _ in m.layers]
         self.v = [torch.zeros(shape, dtype=_BF16, device=dev) for _ in m.layers]

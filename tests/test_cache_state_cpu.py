@@ -134,3 +134,23 @@ def test_building_waits_for_the_fill(monkeypatch):
     assert len(waits) == 2
     c.begin(1)
     assert len(waits) == 3
+
+
+def pair(keys, kv=2, dim=128, dtype=BF):
+    return tuple(torch.zeros((keys, kv, dim), dtype=dtype) for _ in "kv")
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(scored=True, prefix=[pair(5)] * 2), "shared prefix"),
+    (dict(prefix=[pair(5), pair(6)]), "layer 1"),  # positions would differ from layer to layer
+    (dict(prefix=[pair(5), pair(5, kv=1)]), "layer 1"),
+    (dict(prefix=[pair(5, dim=64)] * 2), "layer 0"),
+    (dict(prefix=[pair(5, dtype=torch.float32)] * 2), "layer 0"),
+    (dict(prefix=[pair(5), (pair(5)[0], pair(4)[0])]), "layer 1"),
+    (dict(prefix=[pair(5), pair(5)[:1]]), "layer 1"),
+    (dict(prefix=[pair(5)]), "1 pairs for 2 layers"),
+    (dict(sinks=3), "sinks need a window"), (dict(window=-1), "negative"), (dict(capacity=0), ">= 1"), (dict(B=0), ">= 1"),
+])
+def test_caches_that_no_step_could_use(kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        C.DecodeCache(model(), **{**dict(B=2, capacity=20), **kw})
