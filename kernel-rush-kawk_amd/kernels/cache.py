@@ -51,8 +51,9 @@ class DecodeCache:
             if len(pair) != 2 or any(t.dtype is not _BF16 or t.shape != run or t.device.type != dev.type for t in pair):
                 raise ValueError(f"prefix of layer {i}: needs a bf16 k and v of shape {run} on {dev}, as layer 0 has")
         shape = (B, capacity, cfg.kv_heads, cfg.head_dim)
-        self.k = [torch.zeros(shape, dtype=_BF16, device=dev) for _ in m.layers]
-        self.v = [torch.zeros(shape, dtype=_BF16, device=dev) for _ in m.layers]
+        # One tensor, so that accept() moves the rows of all layers at once.
+        self._kv = torch.zeros((2, len(m.layers), *shape), dtype=_BF16, device=dev)
+        self.k, self.v = list(self._kv[0]), list(self._kv[1])
         self.scores = [torch.zeros((B, cfg.kv_heads, capacity), device=dev) for _ in m.layers] if scored else None
         self.lens = torch.zeros(B, dtype=torch.int32, device=dev)
         self.seen = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -160,9 +161,33 @@ class DecodeCache:
             c[0] = min(c[0], budget)
         return kept
 
+    def accept(self, R: int, paths: list) -> None:
+        """End a draft tree's step of ``R`` rows: of each sequence's last ``R``
+        slots the nodes ``paths[b]`` stay (ascending; from the root, each the
+        parent of the next) and become its next slots in every layer; the rest
+        is forgotten.  A node's position is its depth, so what stays is what a
+        step of those rows alone would have cached.  Until this or
+        :meth:`rollback`, later rows see every node."""
+        if self.scored:
+            raise ValueError("a scored cache takes no draft trees: rollback() forgets its last rows")
+        paths = [list(p) for p in paths]
+        if R < 1 or len(paths) != self.B or any(c[0] < R for c in self._host):
+            raise ValueError(f"accept needs a path for each of {self.B} sequences and {R} >= 1 slots in each")
+        for p in paths:
+            if any(not 0 <= i < R for i in p) or any(a >= b for a, b in zip(p, p[1:])):
+                raise ValueError(f"a path is ascending rows 0 .. {R - 1}, got {p}")
+        moves = [(b * self.capacity + c[0] - R + j, b * self.capacity + c[0] - R + i)
+                 for b, (c, p) in enumerate(zip(self._host, paths)) for j, i in enumerate(p) if i != j]
+        if moves:
+            to, at = torch.tensor(moves, device=self.lens.device).T
+            rows = self._kv.view(2 * len(self.k), self.B * self.capacity, self.kv_heads, self.head_dim)
+            rows[:, to] = rows[:, at]
+        self.rollback([R - len(p) for p in paths])
+
     def rollback(self, rows: list) -> None:
         """Forget the last ``rows[b]`` slots of each sequence: the rejected rows
-        of a verified draft, behind the accepted ones.  What they added to the
+        of a verified draft, behind the accepted ones (:meth:`accept` where the
+        accepted nodes of a tree are not its first).  What they added to the
         scores of the keys before them stays."""
         if len(rows) != self.B or any(not 0 <= n <= c[0] for n, c in zip(rows, self._host)):
             raise ValueError(f"rollback needs 0 .. slots rows for each of {self.B} sequences, got {list(rows)}")

@@ -154,3 +154,44 @@ def pair(keys, kv=2, dim=128, dtype=BF):
 def test_caches_that_no_step_could_use(kw, msg):
     with pytest.raises(ValueError, match=msg):
         C.DecodeCache(model(), **{**dict(B=2, capacity=20), **kw})
+
+
+def test_accepted_paths_of_a_draft_tree():
+    """Nodes that are not a tree's first move together in every layer; lengths and
+    positions go on from the path, as behind a step of its rows alone."""
+    c = C.DecodeCache(model(), 3, 30)
+    c.begin(4)
+    tree = torch.tensor([[1, 3, 5, 0b1001, 0b10101, 0b100101]] * 3)
+    c.begin(6, tree=tree)
+    assert c._positions.view(3, 6).tolist() == [[4, 5, 5, 5, 6, 6]] * 3
+    for i, t in enumerate(c.k + c.v):
+        t.copy_((torch.arange(30)[None, :] + 40 * torch.arange(3)[:, None] + i % 4)[:, :, None, None].expand(3, 30, 2, 128))
+    before = [t.clone() for t in c.k + c.v]
+    paths = [[0, 2, 5], [], [0, 1]]
+    c.accept(6, paths)
+    assert c.lens.tolist() == c.seen.tolist() == [7, 4, 6] and c._host == [[7, 7], [4, 4], [6, 6]]
+    for t, was in zip(c.k + c.v, before):
+        for b, p in enumerate(paths):
+            assert torch.equal(t[b, :4], was[b, :4]) and torch.equal(t[b, 4:4 + len(p)], was[b, [4 + i for i in p]])
+            assert torch.equal(t[b, 10:], was[b, 10:])
+    c.begin(1)
+    assert c._positions.tolist() == [7, 4, 6]
+
+
+@pytest.mark.parametrize("R,paths", [(6, [[0]]), (6, [[0], [6]]), (6, [[0], [-1]]), (6, [[0], [1, 1]]), (6, [[2, 1], [0]]),
+                                     (11, [[0], [0]]), (0, [[], []])])
+def test_paths_refused(R, paths):
+    c = C.DecodeCache(model(), 2, 30)
+    c.begin(10)
+    before = counts(c)
+    with pytest.raises(ValueError, match="path"):
+        c.accept(R, paths)
+    assert counts(c) == before
+
+
+def test_scored_caches_have_no_paths():
+    c = C.DecodeCache(model(), 2, 30, scored=True)
+    c.begin(3)
+    with pytest.raises(ValueError, match="rollback"):
+        c.accept(3, [[0], [0]])
+    assert counts(c)[0] == [3, 3]

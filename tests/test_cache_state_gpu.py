@@ -154,3 +154,32 @@ def test_an_object_that_goes_before_its_call_has_run(device):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         del other
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_decode_goes_on_from_an_accepted_path(device, model, captured):
+    """A tree step of which nodes 0, 2 and 5 (and 0 and 1) are accepted, then a
+    decode row: the cache holds the accepted nodes' rows in every layer, and that
+    row's attention, checked against the oracle, sees them and no others."""
+    from test_cache_step_gpu import Checked
+
+    B = 2
+    cache = (C.DecodeCache if captured else Checked)(model, B, 60)
+    S.GemmStep(model, B * 20, cache=cache).run(x_rows(device, model, B * 20, 71))
+    tree = torch.tensor([[1, 3, 5, 0b1001, 0b10101, 0b100101]] * B, device=device)
+    step = S.GemmStep(model, B * 6, cache=cache, tree=tree)
+    x = x_rows(device, model, B * 6, 72)
+    if captured:
+        step.capture(x)
+        step.replay()
+    else:
+        step.run(x)
+    before = [t.clone() for t in cache.k + cache.v]
+    say("accept", captured)
+    cache.accept(6, [[0, 2, 5], [0, 1]])
+    assert cache.lens.tolist() == cache.seen.tolist() == [23, 22]
+    for t, was in zip(cache.k + cache.v, before):
+        assert torch.equal(t[0, :20], was[0, :20]) and torch.equal(t[0, 20:23], was[0, [20, 22, 25]])
+        assert torch.equal(t[1, :22], was[1, :22])
+    S.GemmStep(model, B, cache=cache).run(x_rows(device, model, B, 73))
+    assert cache.lens.tolist() == [24, 23] and cache._positions.tolist() == [23, 22]
