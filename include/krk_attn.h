@@ -89,8 +89,10 @@ typedef struct krk_attn_shape {
  * Padding rows, and rows that see nothing (or whose scores are all -infinity),
  * give zeros in out and -infinity in lse.  Keys that a row does not see have no
  * part in its result, whatever they hold (NaN and infinities too).  Sums, maxima
- * and weights are held in 32 bits; the weights enter the products with v rounded to bf16 where 128
- * rows share a workgroup (krk_attn_plan tells), else as two bf16 parts.
+ * and weights are held in 32 bits.  The weights enter the products with v as two
+ * bf16 parts (off by 2^-16), or, where 128 rows share a workgroup (krk_attn_plan
+ * tells), rounded to one: an output is then off by up to 2^-8 of sum p |v| besides
+ * its own rounding.
  */
 typedef struct krk_attn_args {
     const void* q;     /* [B * R, heads * head_dim], row stride q_row (multiple of 8) */

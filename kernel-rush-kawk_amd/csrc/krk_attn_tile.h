@@ -1,12 +1,13 @@
 // Cache attention for many rows of a head (prompts, batches over a shared
 // prefix): one workgroup per tile of 128 rows, K and V through LDS.
 //
-// Bound by LDS and the matrix pipe alike: 64 keys of a wave's 32 rows are 1030
-// cycles of its SIMD's matrix pipe at head size 128 (2.1 MFLOP) and 32 KB of LDS
-// reads, 1030 cycles for a CU's four waves, and the keys' own 32 KB come on top.
-// The 2048 weights take about 750 cycles of the vector pipe.  Measured, two
-// waves of a SIMD need 3700 cycles for a step each, 880 TFLOP/s of an 8192-row
-// prompt with a window of 2048.
+// Bound by the matrix pipe, LDS and the vector pipe alike: 64 keys of a wave's 32
+// rows are 1024 cycles of its SIMD's matrix pipe at head size 128 (1.05 MFLOP), 32 KB
+// of LDS reads, 1030 cycles for a CU's four waves (the keys' own 32 KB come on
+// top), and 1260 cycles of the vector pipe for the 2048 weights, their maxima and
+// what goes with them (counted).  Two waves of a SIMD need 4200 cycles for a step
+// each, the first loads and the last stores included: 840-880 TFLOP/s of an 8192-row
+// prompt with a window of 2048, at the 2.1 GHz that the clock falls to under it.
 //
 // Work split.  Four waves, each with 32 rows of its own, all reading the same
 // 64-key steps of K and V from LDS.  S^T = K Q^T and O^T = V^T P^T on
@@ -28,9 +29,16 @@
 // barrier a step.  16-byte chunks of a row are permuted with the row's low
 // bits, so that neither kind of read meets bank conflicts.
 //
-// Weights are rounded to bf16 for the product with V (their sum is not): with
-// 8 bits of mantissa each, the error of a weighted mean of many values is that
-// of the final rounding again.
+// Weights are rounded to one bf16 for the product with V; their sum is not.  A
+// choice: with two parts, as the split kernel has them, the products take half as
+// many matrix instructions again (8192-row prompt 279 -> 366 us, 64 sequences over
+// 32768 shared keys 92 -> 101, 32 scored rows over 2 x 16000 keys 67 -> 73).  Each
+// weight is off by up to 2^-8 of itself, so an output by up to 2^-8 of sum p |v|
+// before its own rounding, whether its row sees many keys or few: measured, 0.0021
+// of the outputs' norm for rows of many keys and 0.0017-0.0020 for rows of 2 to 32
+// (rounding the exact result: 0.0017).  The sum of the rounded weights in its place
+// would help rows whose weight lies on a few keys (0.0019 -> 0.0017, the others
+// alike) and costs 3%.
 #pragma once
 
 #include <type_traits>
