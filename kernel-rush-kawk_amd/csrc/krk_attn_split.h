@@ -436,7 +436,10 @@ __global__ void __launch_bounds__(256) attn_weights_raw_kernel(AttnParams p) {
 // keys of a sequence and head, whose K stays in registers, over all R * G rows
 // in order (no atomics).  The rows come 32 at a time through LDS, shared by the
 // four waves, the next 32 loading meanwhile.  Bound by reading K once more and
-// by the weights themselves (20 VALU cycles a wave and 64 of them).
+// by the weights themselves (20 VALU cycles a wave and 64 of them): 26 us for 32
+// rows over 2 x 16000 keys.  All rows, also those that see none of the 32 keys: 2.7
+// ms for a prompt of 8192 rows, whose attention takes 0.56 ms (0.28 with a window of
+// 2048).
 constexpr int kWeightRows = 32;
 template <int D>
 __global__ void __launch_bounds__(256, 4) attn_weights_kernel(AttnParams p) {

@@ -242,7 +242,9 @@ class CacheAttention:
 
     The workspace (:func:`workspace_bytes`) belongs to the object, or is
     ``workspace``: zero-filled uint8 memory that objects of one B and kv_heads may
-    share if all their calls are ordered on one stream.  Results are deterministic.
+    share if all their calls are ordered on one stream.  A scored object without a
+    window keeps q.k there for up to 16 rows a key/value head: ``4 * B * R * heads
+    * capacity`` bytes.  Results are deterministic.
     """
 
     def __init__(self, B: int, R: int, heads: int, kv_heads: int, head_dim: int, capacity: int, device, *,
