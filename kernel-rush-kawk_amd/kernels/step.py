@@ -92,7 +92,7 @@ class GemmStep:
     adds the attention of the R rows of each sequence, sequence after sequence
     in x; each run or replay moves the cache on by R rows.  ``tree`` (int64
     ``[B, R]`` on the GPU, read at every run and replay) makes them a draft
-    tree's nodes."""
+    tree's nodes; ``cache.accept`` then keeps the accepted path."""
 
     def __init__(self, m, M: int, mm: dict | None = None, log=None, tune: bool = False,
                  select_k: int | None = None, cache=None, tree: torch.Tensor | None = None):
