@@ -1,9 +1,10 @@
 """Build libkrk_gemm.so (the C-ABI GEMM library), libkrk_attn.so (the cache
-operators between the qkv and o projections) and libkrk_probe.so (the pure-read
-floor probe bench.py measures against) for gfx950 with hipcc.
+operators between the qkv and o projections), libkrk_paged.so (the same over a
+paged cache), libkrk_adapter.so (low-rank adapters) and libkrk_probe.so (the
+pure-read floor probe bench.py measures against) for gfx950 with hipcc.
 
 Usage: ``python kernel-rush-kawk_amd/build_lib.py`` (or ``build()`` /
-``build_attn()`` / ``build_probe()`` from Python).  The libraries are written next to this file
+``build_attn()`` / ``build_paged()`` / ``build_adapter()`` / ``build_probe()`` from Python).  The libraries are written next to this file
 so they ship with the tree.  hipcc cross-compiles for gfx950 without a GPU
 present.
 """
@@ -22,6 +23,10 @@ LIB = HERE / "libkrk_gemm.so"
 SOURCES = [CSRC / "krk_gemm.hip"]
 ATTN_LIB = HERE / "libkrk_attn.so"
 ATTN_SOURCES = [CSRC / "krk_attn.hip"]
+PAGED_LIB = HERE / "libkrk_paged.so"
+PAGED_SOURCES = [CSRC / "krk_paged.hip"]
+ADAPTER_LIB = HERE / "libkrk_adapter.so"
+ADAPTER_SOURCES = [CSRC / "krk_adapter.hip"]
 PROBE_LIB = HERE / "libkrk_probe.so"
 PROBE_SOURCES = [CSRC / "krk_probe.hip"]
 HEADERS = sorted(CSRC.glob("*.h")) + [ROOT / "include" / "krk_gemm.h"]
@@ -70,6 +75,16 @@ def build_attn(verbose: bool = False) -> Path:
     return build(verbose, out=ATTN_LIB, sources=ATTN_SOURCES)
 
 
+def build_paged(verbose: bool = False) -> Path:
+    """Compile libkrk_paged.so (page tables, paged rotary embedding and attention); always recompiles."""
+    return build(verbose, out=PAGED_LIB, sources=PAGED_SOURCES)
+
+
+def build_adapter(verbose: bool = False) -> Path:
+    """Compile libkrk_adapter.so (low-rank adapters); always recompiles."""
+    return build(verbose, out=ADAPTER_LIB, sources=ADAPTER_SOURCES)
+
+
 def build_probe(verbose: bool = False) -> Path:
     """Compile libkrk_probe.so (bench.py's pure-read floor); always recompiles."""
     return build(verbose, out=PROBE_LIB, sources=PROBE_SOURCES)
@@ -79,5 +94,7 @@ if __name__ == "__main__":
     path = build(verbose=True)
     print(f"built {path}")
     print(f"built {build_attn(verbose=True)}")
+    print(f"built {build_paged(verbose=True)}")
+    print(f"built {build_adapter(verbose=True)}")
     print(f"built {build_probe(verbose=True)}")
     sys.exit(0)

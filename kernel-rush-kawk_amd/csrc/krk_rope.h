@@ -28,9 +28,12 @@ struct RopeParams {
     uint16_t *k, *v;
     int64_t k_seq, k_slot, k_head, v_seq, v_slot, v_head;
     int B, R, heads, kv_heads, capacity;
+    const int32_t* slots;  // paged: the rows' slots in a pool of `capacity` slots
+    int shift;             // paged: pages of 1 << shift slots, k_seq and v_seq from page to page
 };
 
-template <int D>
+// PAGED: B * R rows whose slots (and positions) are given, else those of lens.
+template <int D, bool PAGED = false>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeParams p) {
     constexpr int L = D / 8;  // lanes of a head
     const int all = p.heads + 2 * p.kv_heads;
@@ -40,12 +43,23 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeParams p) {
     const int64_t at = in ? row : 0;
     const int h = in ? (int)(unit - row * all) : 0;
     const int c = threadIdx.x % L;
-    const int b = (int)(at / p.R);
-    int len = p.lens[b];
-    len = len < 0 ? 0 : len > p.capacity ? p.capacity : len;
-    const int slot = len - p.R + (int)(at - (int64_t)b * p.R);
-    const int pos = p.positions ? p.positions[at] : slot;
-    const bool ok = in && slot >= 0 && pos >= 0 && pos < p.table_rows;
+    int b, slot, pos;
+    bool ok = in;
+    if constexpr (PAGED) {
+        const int s = p.slots[at];
+        b = s >> p.shift;  // the page
+        slot = s & ((1 << p.shift) - 1);
+        pos = p.positions[at];
+        ok = ok && s >= 0 && s < p.capacity;
+    } else {
+        b = (int)(at / p.R);
+        int len = p.lens[b];
+        len = len < 0 ? 0 : len > p.capacity ? p.capacity : len;
+        slot = len - p.R + (int)(at - (int64_t)b * p.R);
+        pos = p.positions ? p.positions[at] : slot;
+        ok = ok && slot >= 0;
+    }
+    ok = ok && pos >= 0 && pos < p.table_rows;
     const u32x4 x = load_stream16(p.qkv + at * p.qkv_row + (int64_t)h * D + 8 * c);
     if (h >= p.heads + p.kv_heads) {  // v: as it is
         if (ok)
