@@ -158,7 +158,7 @@ typedef struct krk_paged_shape {
  * row does not see have no part in its result, whatever they hold (NaN and infinities
  * too), and table entries of pages that no row sees are of no matter.  An entry
  * outside 0 .. pages - 1 for a page that is seen reads another page of the pool.
- * starts have to ascend; where they do not, some rows are not written.
+ * starts have to ascend; where they do not, rows may be left as they were.
  *
  * Sums, maxima and weights are held in 32 bits.  The weights enter the products with
  * v as two bf16 parts (off by 2^-16), or, where a request has more than

@@ -126,14 +126,26 @@ int check_shape(const krk_paged_shape& s) {
 // -------------------------------------------------------------------- plan
 struct Plan {
     int64_t blocks;
-    size_t bytes;
+    size_t ctr, part, ml, bytes;  // workspace: sizes of its parts and their sum
 };
 
 Plan make_plan(const krk_paged_shape& s) {
     Plan p{};
     const int64_t RG = (int64_t)s.rows * (s.heads / s.kv_heads);
-    // Each request with rows has one tile that is not full.
-    p.blocks = s.kv_heads * (RG / 16 + (s.B < s.rows ? s.B : s.rows));
+    // Tiles of 16 rows at least, and each request with rows has one that is not full.
+    const int64_t tiles = s.kv_heads * (RG / 16 + (s.B < s.rows ? s.B : s.rows));
+    // Their key ranges: as many as the longest request would have, and those of tiles
+    // that have several are limited.
+    const int64_t parts = cdiv(cdiv((int64_t)s.width * s.page_size, krk::kFewStep), krk::kFewLeast);
+    const int64_t split = tiles * parts < krk::kSplitJobs ? tiles * parts : krk::kSplitJobs;
+    p.blocks = tiles + (parts > 1 ? split : 0);
+    if (parts > 1) {
+        const size_t rows = (size_t)(32 * split);
+        p.ctr = align_up(krk::kCounters * sizeof(uint32_t), 256);
+        p.part = rows * s.head_dim * sizeof(float);
+        p.ml = rows * sizeof(float2);
+    }
+    p.bytes = p.ctr + p.part + p.ml;
     return p;
 }
 
@@ -144,7 +156,7 @@ int launch_attn(const krk::PagedParams& p, const Plan& plan, hipStream_t stream)
     const size_t shm = krk::few_lds_bytes<D>();
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "paged_attn_kernel LDS size");
     void* args[] = {(void*)&p};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)plan.blocks), dim3(krk::kFewThreads), args, shm, stream), "paged_attn_kernel launch");
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)plan.blocks), dim3(krk::kPagedThreads), args, shm, stream), "paged_attn_kernel launch");
 }
 
 krk::PageView view(const krk_pages& c) { return {static_cast<const uint16_t*>(c.p), c.page, c.slot, c.head}; }
@@ -334,6 +346,10 @@ int krk_paged_attn_bf16(const krk_paged_shape* shape, const krk_paged_attn_args*
     p.out = static_cast<uint16_t*>(a.out);
     p.out_row = a.out_row;
     p.lse = a.lse;
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    p.ctr = reinterpret_cast<uint32_t*>(w);
+    p.part = reinterpret_cast<float*>(w + plan.ctr);
+    p.ml = reinterpret_cast<float2*>(w + plan.ctr + plan.part);
     p.scale = a.scale;
     p.c = scale_log2;
     p.B = s.B;

@@ -1,20 +1,25 @@
 // Attention of many requests' new rows over their pages (gfx950): how a call is
-// cut into jobs, and the kernel for requests of few rows.
+// cut into jobs, and the jobs of requests of few rows.
 //
 // Rows.  A key/value head h serves G = heads / kv_heads query heads, so request b's
 // products have n * G rows per key/value head: row j is its new row j / G with
 // query head h * G + j % G.
 //
-// Jobs.  A call's lengths are on the device, so each workgroup works out from them
-// which job its number stands for: a lane takes one request in 64 of them (in order),
-// and a scan over the wave finds the request.  Every wave does so for itself: no
-// barrier, no launch in front, nothing kept from call to call.
+// Jobs.  A job is a tile of a request's rows of one head against one range of the
+// keys they see.  A call's lengths are on the device, so each workgroup works out from
+// them which job its number stands for: a lane takes one request in 64 of them (in
+// order), and scans over the wave find the request.  Every wave does so for itself: no
+// barrier, no launch in front, nothing kept from call to call.  Keys are cut by
+// length: into ranges that cost about what one of kTarget workgroups would take of
+// all of the call's work, so a long request beside short ones does not work on alone.
+// The workgroup that finishes the last range of a tile joins them, in order.
 //
 // Products, key order and the treatment of infinities and NaNs in masked places are
 // those of the contiguous caches' kernels.
 #pragma once
 
 #include "krk_attn_common.h"
+#include "krk_epilogue.h"
 #include "krk_page_step.h"
 
 namespace krk {
@@ -34,10 +39,29 @@ struct PagedParams {
     uint16_t* out;
     int64_t out_row;
     float* lse;
-    float scale;  // of q.k
-    float c;      // scale * log2(e)
+    uint32_t* ctr;  // [kCounters] finished ranges of a tile
+    float* part;    // [..][D] unnormalised outputs of ranges' rows
+    float2* ml;     // [..] their running maximum (of q.k) and sum
+    float scale;    // of q.k
+    float c;        // scale * log2(e)
     int B, rows, heads, kv_heads, G, pages, shift, width, window, sinks;
 };
+
+constexpr int kPagedThreads = 256;
+constexpr int kPagedWaves = kPagedThreads / 64;
+
+// Workgroups that the work is cut for: two a CU.
+constexpr int kTarget = 512;
+// Of more than one range each, tiles have less than twice as many ranges as there are
+// of the target's size: fewer than 2 * kTarget jobs.  A tile has two at least.
+constexpr int kSplitJobs = 2 * kTarget + 16;
+constexpr int kCounters = kSplitJobs;
+constexpr int kFewStep = 32 * kPagedWaves;  // keys of a step of a workgroup
+constexpr int kFewPairs = 64;               // rows of a head that jobs of few rows take
+// Least steps of a range.
+constexpr int kFewLeast = 2;
+// What a step costs, in us of one of two workgroups of a CU.
+constexpr float kFewCost = 1.0f;
 
 // A request: its first row, rows and keys, whatever the arrays hold.
 struct Request {
@@ -55,45 +79,109 @@ __device__ __forceinline__ Request request(const PagedParams& p, int b) {
     return x;
 }
 
-constexpr int kFewThreads = 256;
-constexpr int kFewWaves = kFewThreads / 64;
+// How a request's rows of one head are cut: tiles of `tile` rows, over `steps` steps of
+// keys at most.
+struct Tiling {
+    int tile, tiles, steps;
+};
+__device__ __forceinline__ Tiling tiling(const PagedParams& p, const Request& r) {
+    Tiling t;
+    const int rows = r.n * p.G;
+    t.tile = rows <= 16 ? 16 : 32;
+    t.tiles = (rows + t.tile - 1) / t.tile;
+    int keys = r.len;
+    if (p.window) {
+        const int near = p.window + p.sinks + r.n;
+        keys = near < keys ? near : keys;
+    }
+    t.steps = (keys + kFewStep - 1) / kFewStep;
+    return t;
+}
 
-// A tile of a request's rows of one key/value head.
+__device__ __forceinline__ float wave_total(float v) {
+    v += partner<1>(v);
+    v += partner<2>(v);
+    v += partner<4>(v);
+    v += partner<8>(v);
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(row_sum(v))));
+}
+
+// A tile of a request's rows of one key/value head, against one range of its keys.
 struct Job {
-    int b, h, tile;
+    int b, h, tile;     // tile: rows of a tile; < 0: no job
+    int row0;           // first row of the tile, of the head's row list
+    int part, parts;    // range, of how many
+    int slot, ctr;      // of parts > 1: row of the tile's first range's results; its counter
     Request req;
 };
 
-// The job that `id` stands for; tile < 0: none.
 __device__ __forceinline__ Job job_of(const PagedParams& p, int id) {
     const int lane = threadIdx.x & 63;
     const int per = (p.B + 63) / 64;
     const int b0 = lane * per, b1 = b0 + per < p.B ? b0 + per : p.B;
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (request(p, b).n * p.G + 15) / 16 * p.kv_heads;
-    const int end = wave_scan(mine);
-    int left = id - (end - mine);
-    const uint64_t who = __ballot(left >= 0 && left < mine);
+    const Request none = {0, 0, 0};
+    const Request first = b0 < b1 ? request(p, b0) : none;
+    float cost = 0.0f;
+    int all_rows = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Request r = b == b0 ? first : request(p, b);
+        const Tiling t = tiling(p, r);
+        all_rows += r.n;
+        cost += (float)t.tiles * (float)p.kv_heads * (float)t.steps * kFewCost;
+    }
+    const int most = (int)(wave_total(cost) * (1.0f / (kTarget * kFewCost))) + 1;  // steps of a range
+    const int few = most > kFewLeast ? most : kFewLeast;
+    // Jobs, tiles of several ranges and rows of their results.
+    auto cut = [&](const Tiling& t, int* parts, int* jobs, int* ctrs, int* rows) {
+        *parts = t.steps > few ? (t.steps + few - 1) / few : 1;
+        *ctrs = *parts > 1 ? t.tiles * p.kv_heads : 0;
+        *jobs = t.tiles * p.kv_heads * *parts;
+        *rows = *parts > 1 ? *jobs * t.tile : 0;
+    };
+    int jobs = 0, ctrs = 0, rows = 0;
+    for (int b = b0; b < b1; ++b) {
+        int parts, x, y, z;
+        cut(tiling(p, b == b0 ? first : request(p, b)), &parts, &x, &y, &z);
+        jobs += x;
+        ctrs += y;
+        rows += z;
+    }
+    int left = id - (wave_scan(jobs) - jobs), ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows;
+    const uint64_t who = __ballot(left >= 0 && left < jobs);
     Job j;
     j.tile = -1;
-    if (!who) return j;
+    // More rows than the call has, as starts do not ascend: the jobs' bounds would not hold.
+    if (!who || __builtin_amdgcn_readlane(wave_scan(all_rows), 63) > p.rows) return j;
     const int src = __ffsll((unsigned long long)who) - 1;
-    int b = b0;
-    Request r = {0, 0, 0};
+    int b = b0, parts = 1;
+    Request r = none;
     if (lane == src)
         for (; b < b1; ++b) {
-            r = request(p, b);
-            const int jobs = (r.n * p.G + 15) / 16 * p.kv_heads;
-            if (left < jobs) break;
-            left -= jobs;
+            r = b == b0 ? first : request(p, b);
+            int x, y, z;
+            cut(tiling(p, r), &parts, &x, &y, &z);
+            if (left < x) break;
+            left -= x;
+            ctr += y;
+            slot += z;
         }
     left = __builtin_amdgcn_readlane(left, src);
     j.b = __builtin_amdgcn_readlane(b, src);
     j.req.row = __builtin_amdgcn_readlane(r.row, src);
     j.req.n = __builtin_amdgcn_readlane(r.n, src);
     j.req.len = __builtin_amdgcn_readlane(r.len, src);
+    j.parts = __builtin_amdgcn_readlane(parts, src);
+    const Tiling t = tiling(p, j.req);
+    // Heads change fastest, then ranges, then tiles, those that see more keys first.
     j.h = left % p.kv_heads;
-    j.tile = left / p.kv_heads;
+    left /= p.kv_heads;
+    j.part = left % j.parts;
+    const int tile = t.tiles - 1 - left / j.parts;
+    j.tile = t.tile;
+    j.row0 = tile * t.tile;
+    const int at = tile * p.kv_heads + j.h;
+    j.ctr = __builtin_amdgcn_readlane(ctr, src) + at;
+    j.slot = __builtin_amdgcn_readlane(slot, src) + at * j.parts * t.tile;
     return j;
 }
 
@@ -153,109 +241,235 @@ struct PagedRun {
     }
 };
 
-template <int D>
-constexpr size_t few_lds_bytes() {
-    return (size_t)kFewWaves * 16 * ((D + 4) * sizeof(float) + sizeof(float2));
+// Where the rows of a tile are.
+struct TileRow {
+    int r, head, pos, lo;  // row of the request, query head, position and the first key of its window
+    __device__ __forceinline__ TileRow(const PagedParams& p, const Job& j, int row) {
+        r = row / p.G;
+        head = j.h * p.G + (row - r * p.G);
+        pos = j.req.len - j.req.n + r;
+        lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
+    }
+};
+
+// Four finished outputs of a tile's row, and with d = 0 the log of its sum: M the
+// maximum of q.k (-infinity: the row sees nothing), L the sum.
+__device__ __forceinline__ void finish_row(const PagedParams& p, const Job& j, int row, int D, int d, const f32x4& o, float M, float L) {
+    const TileRow t(p, j, row);
+    const int64_t at = j.req.row + t.r;
+    const bool none = L == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / L;
+    *reinterpret_cast<uint2*>(p.out + at * p.out_row + (int64_t)t.head * D + d) =
+        none ? make_uint2(0u, 0u) : make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+    if (d == 0 && p.lse) p.lse[at * p.heads + t.head] = none ? kNegInf : M * p.scale + logf(L);
 }
 
-// Requests of few rows: 16 rows of a head and all of the keys they see, the four
-// waves 32 keys at a time in turn.  Waves keep their own running maximum, sum and O
-// and meet in LDS once, at the end.  Bound by reading K and V once a tile (4 * D
-// bytes a key).  Weights go into the second product as two bf16 parts (p = hi + lo,
-// 16 bits of mantissa).
+// Outputs of one row over several ranges, put together.
+struct Merged {
+    float M = kNegInf, L = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    __device__ __forceinline__ void add(float c, float m, float l, const f32x4& x) {
+        const float mn = fmaxf(M, m);
+        const float ms = mn == kNegInf ? 0.0f : mn;
+        const float f0 = exp2_raw((M - ms) * c), f1 = exp2_raw((m - ms) * c);
+        L = L * f0 + f1 * l;
+        o = o * f0 + f1 * x;
+        M = mn;
+    }
+};
+
+// Joins all ranges of a tile with the whole workgroup: every four outputs of a row are
+// one thread's, or (few rows) several threads', each with every groups-th range,
+// which then meet in LDS in order: the result does not depend on which range finished
+// first.  kJoinLoads loads are in flight at a time, as each is a round trip beyond
+// this XCD's L2.
+constexpr int kJoinLoads = 8;
 template <int D>
-__global__ void __launch_bounds__(kFewThreads, 2) paged_attn_kernel(PagedParams p) {
-    extern __shared__ __align__(16) unsigned char lds[];
+__device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, unsigned char* lds) {
+    const int left = j.req.n * p.G - j.row0;
+    const int units = (left < j.tile ? left : j.tile) * (D / 4);
+    auto join = [&](int e, int from, int step) {
+        const int row = e / (D / 4), d = 4 * (e % (D / 4));
+        Merged y;
+        for (int s0 = from; s0 < j.parts; s0 += kJoinLoads * step) {
+            float2 ml[kJoinLoads];
+            f32x4 x[kJoinLoads];
+#pragma unroll
+            for (int s = 0; s < kJoinLoads; ++s) {
+                const int at = s0 + s * step;
+                const int64_t g = j.slot + (int64_t)(at < j.parts ? at : s0) * j.tile + row;
+                ml[s] = get_agent(p.ml + g);
+                x[s] = get_agent(p.part + g * D + d);
+            }
+#pragma unroll
+            for (int s = 0; s < kJoinLoads; ++s)
+                if (s0 + s * step < j.parts) y.add(p.c, ml[s].x, ml[s].y, x[s]);
+        }
+        return y;
+    };
+    int groups = 1;
+    while (2 * groups * units <= kPagedThreads && groups < 8) groups *= 2;
+    if (groups > 1) {
+        const int g = threadIdx.x / units, e = threadIdx.x - g * units;
+        Merged y;
+        if (g < groups) y = join(e, g, groups);
+        f32x4* lo = reinterpret_cast<f32x4*>(lds);
+        float2* lml = reinterpret_cast<float2*>(lds + kPagedThreads * sizeof(f32x4));
+        __syncthreads();
+        lo[threadIdx.x] = y.o;
+        lml[threadIdx.x] = make_float2(y.M, y.L);
+        __syncthreads();
+        if (g == 0) {
+            for (int k = 1; k < groups; ++k) y.add(p.c, lml[e + k * units].x, lml[e + k * units].y, lo[e + k * units]);
+            finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+        }
+        return;
+    }
+    for (int e = threadIdx.x; e < units; e += kPagedThreads) {
+        const Merged y = join(e, 0, 1);
+        finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+    }
+}
+
+template <int D>
+constexpr size_t few_lds_bytes() {
+    return (size_t)kPagedWaves * 32 * ((D + 4) * sizeof(float) + sizeof(float2));
+}
+
+// Jobs of few rows: 16 * MT rows of a head against one range of keys, the four waves 32
+// keys at a time in turn.  Waves keep their own running maximum, sum and O and meet in
+// LDS once, at the end.  Bound by reading K and V once a tile (4 * D bytes a key), so
+// a wave's loads run ahead: K's registers are loaded again as soon as the scores are
+// taken, V's as soon as the products are, and the page numbers of the step behind
+// those are on their way meanwhile.  Weights go into the second product as two bf16
+// parts (p = hi + lo, 16 bits of mantissa).
+template <int D, int MT>
+__device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, unsigned char* lds) {
+    constexpr int TR = 16 * MT;
     constexpr int KS = D / 32;
     constexpr int VD = D / 16;
-    const Job job = job_of(p, (int)blockIdx.x);
-    if (job.tile < 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
-    const int rows = job.req.n * p.G, row0 = 16 * job.tile;
+    const int rows = job.req.n * p.G, row0 = job.row0;
     const int pos0 = job.req.len - job.req.n;  // of the request's first row
-    const int last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
+    const int last_row = row0 + TR - 1 < rows ? row0 + TR - 1 : rows - 1;
     const KeySpan<32> span(p, job.req.len, pos0 + row0 / p.G, pos0 + last_row / p.G);
     const PagedRun kr(p, p.k, job, span.end), vr(p, p.v, job, span.end);
+    const int t1 = (int)((int64_t)span.steps * (job.part + 1) / job.parts);
+    int t = (int)((int64_t)span.steps * job.part / job.parts) + wave;
 
-    // This lane's row (the last one again behind the end).
-    const int mine = row0 + n16 < rows ? row0 + n16 : rows - 1;
-    const int r = mine / p.G;
-    const int head = job.h * p.G + (mine - r * p.G);
-    const int pos = pos0 + r;
-    const int lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
-    u32x4 qf[KS];
-    {
-        const uint16_t* qr = p.q + (int64_t)(job.req.row + r) * p.q_row + (int64_t)head * D + 8 * q4;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_cached16(qr + 32 * s);
-    }
-    f32x4 acc[VD];
-    float m = kNegInf, l = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VD; ++j) acc[j] = f32x4{0, 0, 0, 0};
-    bool any_odd = false;
-    for (int t = wave; t < span.steps; t += kFewWaves) {
-        const int kb = span.key(t);
-        KeyFrag<D> kf;
-        ValueFrag<D> vf;
-        {
-            const int group = kb + 8 * (n16 >> 2);
-            const unsigned page = kr.page_of(group);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint16_t* x = kr.row(kb + tile_key(u, n16), page) + 8 * q4;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) kf.f[u][s] = load_cached16(x + 32 * s);
-            }
-            const unsigned vpage = vr.page_of(kb + 8 * q4);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                vf.f[i] = __builtin_nontemporal_load(
-                    reinterpret_cast<const typename ValueFrag<D>::vec*>(vr.row(kb + 8 * q4 + i, vpage) + VD * n16));
-        }
-        f32x4 s[2];
+    KeyFrag<D> kf;
+    ValueFrag<D> vf;
+    auto load_k = [&](int kb, unsigned page) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            s[u] = f32x4{0, 0, 0, 0};
+            const uint16_t* x = kr.row(kb + tile_key(u, n16), page) + 8 * q4;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[u] = mfma16(kf.f[u][ks], qf[ks], s[u]);
+            for (int s = 0; s < KS; ++s) kf.f[u][s] = load_cached16(x + 32 * s);
         }
+    };
+    auto load_v = [&](int kb, unsigned page) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            vf.f[i] = __builtin_nontemporal_load(
+                reinterpret_cast<const typename ValueFrag<D>::vec*>(vr.row(kb + 8 * q4 + i, page) + VD * n16));
+    };
+    // Page numbers of the keys that this lane loads of the wave's next step and of the
+    // one behind it (behind the range: of some step in it).
+    auto k_page = [&](int t) { return kr.page_of(span.key(t < t1 ? t : t1 - 1) + 8 * (n16 >> 2)); };
+    auto v_page = [&](int t) { return vr.page_of(span.key(t < t1 ? t : t1 - 1) + 8 * q4); };
+    unsigned kp = 0, vp = 0;
+    if (t < t1) {
+        const unsigned kp0 = k_page(t), vp0 = v_page(t);
+        kp = k_page(t + kPagedWaves);
+        vp = v_page(t + kPagedWaves);
+        load_k(span.key(t), kp0);
+        load_v(span.key(t), vp0);
+    }
+    const int t_first = t;
+
+    // This lane's rows (the last one again behind the end), and their q.
+    u32x4 qf[MT][KS];
+    int pos[MT], lo[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int row = row0 + 16 * i + n16;
+        const TileRow x(p, job, row < rows ? row : rows - 1);
+        pos[i] = x.pos;
+        lo[i] = x.lo;
+        const uint16_t* qr = p.q + (int64_t)(job.req.row + x.r) * p.q_row + (int64_t)x.head * D + 8 * q4;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[i][s] = load_cached16(qr + 32 * s);
+    }
+    f32x4 acc[MT][VD];
+    float m[MT], l[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        m[i] = kNegInf;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VD; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    }
+    // An infinity or a NaN times a zero weight would reach rows that do not see
+    // it: the products run on zeros in their place, and the rows that see them
+    // get them behind the last step.
+    bool any_odd = false;
+    for (; t < t1; t += kPagedWaves) {
+        const int kb = span.key(t);
+        const int next = t + kPagedWaves;
+        const unsigned kp2 = k_page(next + kPagedWaves), vp2 = v_page(next + kPagedWaves);
+        f32x4 s[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[i][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s[i][u] = mfma16(kf.f[u][ks], qf[i][ks], s[i][u]);
+            }
+        if (next < t1) load_k(span.key(next), kp);
+        // What each row does not see gets no weight.
         if (!span.whole(kb, p.sinks)) {
 #pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = kb + 8 * q4 + e;
+                    s[i][e >> 2][e & 3] = row_sees(pos[i], lo[i], p.sinks, key) ? s[i][e >> 2][e & 3] : kNegInf;
+                }
+        }
+        bf16x8 hi[MT], low[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            float mx = s[i][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[i][e >> 2][e & 3]);
+            const float mn = fmaxf(m[i], row_max(mx));
+            const float ms = mn == kNegInf ? 0.0f : mn;  // nothing seen yet: weights exp2(-inf) = 0
+            const float alpha = exp2_raw((m[i] - ms) * p.c);
+            m[i] = mn;
+            float w[8], sum = 0.0f;
+#pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int key = kb + 8 * q4 + e;
-                s[e >> 2][e & 3] = row_sees(pos, lo, p.sinks, key) ? s[e >> 2][e & 3] : kNegInf;
+                w[e] = exp2_raw((s[i][e >> 2][e & 3] - ms) * p.c);
+                sum += w[e];
+            }
+            l[i] = l[i] * alpha + sum;
+            u32x4 ph, pl;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ph[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
+                const uint32_t x = ph[e];
+                pl[e] = pack_bf16(w[2 * e] - bf16_to_f32(x & 0xffffu), w[2 * e + 1] - __uint_as_float(x & 0xffff0000u));
+            }
+            hi[i] = __builtin_bit_cast(bf16x8, ph);
+            low[i] = __builtin_bit_cast(bf16x8, pl);
+            if (__any(alpha != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < VD; ++j) acc[i][j] *= alpha;
             }
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
-        const float mn = fmaxf(m, row_max(mx));
-        const float ms = mn == kNegInf ? 0.0f : mn;  // nothing seen yet: weights exp2(-inf) = 0
-        const float alpha = exp2_raw((m - ms) * p.c);
-        m = mn;
-        float w[8], sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            w[e] = exp2_raw((s[e >> 2][e & 3] - ms) * p.c);
-            sum += w[e];
-        }
-        l = l * alpha + sum;
-        u32x4 ph, pl;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            ph[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
-            const uint32_t x = ph[e];
-            pl[e] = pack_bf16(w[2 * e] - bf16_to_f32(x & 0xffffu), w[2 * e + 1] - __uint_as_float(x & 0xffff0000u));
-        }
-        const bf16x8 hi = __builtin_bit_cast(bf16x8, ph), low = __builtin_bit_cast(bf16x8, pl);
-#pragma unroll
-        for (int j = 0; j < VD; ++j) acc[j] *= alpha;
-        // An infinity or a NaN times a zero weight would reach rows that do not see
-        // it: the products run on zeros in their place, and the rows that see them
-        // get them behind the last step.
         if (__any(vf.odd())) {
             vf.tame();
             any_odd = true;
@@ -263,24 +477,31 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attn_kernel(PagedParams 
 #pragma unroll
         for (int j = 0; j < VD; ++j) {
             const bf16x8 a = vf.operand(j);
-            acc[j] = mfma16(a, hi, mfma16(a, low, acc[j]));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, low[i], acc[i][j]));
         }
+        if (next < t1) load_v(span.key(next), vp);
+        kp = kp2;
+        vp = vp2;
     }
     if (any_odd) {  // rare, so key by key
 #pragma unroll 1
-        for (int t = wave; t < span.steps; t += kFewWaves) {
+        for (t = t_first; t < t1; t += kPagedWaves) {
             const int kb = span.key(t);
 #pragma unroll 1
             for (int key = kb; key < kb + 32 && key < span.end; ++key) {
                 const uint16_t* x = vr.row(key, vr.page_of(key)) + 4 * q4 * VD;
-                const bool ok = row_sees(pos, lo, p.sinks, key);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int j = 0; j < VD; j += 2) {
                         const uint32_t y = *reinterpret_cast<const uint32_t*>(x + e * VD + j);
-                        acc[j][e] += ok ? odd_or_zero(y << 16) : 0.0f;
-                        acc[j + 1][e] += ok ? odd_or_zero(y & 0xffff0000u) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            const bool ok = row_sees(pos[i], lo[i], p.sinks, key);
+                            acc[i][j][e] += ok ? odd_or_zero(y << 16) : 0.0f;
+                            acc[i][j + 1][e] += ok ? odd_or_zero(y & 0xffff0000u) : 0.0f;
+                        }
                     }
             }
         }
@@ -290,45 +511,72 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attn_kernel(PagedParams 
     // sums behind.
     constexpr int LD = D + 4;
     float* lo_o = reinterpret_cast<float*>(lds);
-    float2* lo_ml = reinterpret_cast<float2*>(lds + (size_t)kFewWaves * 16 * LD * sizeof(float));
-    const float ls = row_sum(l);
-    if (q4 == 0) lo_ml[wave * 16 + n16] = make_float2(m, ls);
-    float* o = lo_o + (wave * 16 + n16) * LD;
+    float2* lo_ml = reinterpret_cast<float2*>(lds + (size_t)kPagedWaves * TR * LD * sizeof(float));
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int i = 0; i < MT; ++i) {
+        const float ls = row_sum(l[i]);
+        if (q4 == 0) lo_ml[wave * TR + 16 * i + n16] = make_float2(m[i], ls);
+        float* o = lo_o + ((size_t)wave * TR + 16 * i + n16) * LD;
 #pragma unroll
-        for (int j = 0; j < VD; j += 4)
-            *reinterpret_cast<f32x4*>(o + (4 * q4 + e) * VD + j) = f32x4{acc[j][e], acc[j + 1][e], acc[j + 2][e], acc[j + 3][e]};
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < VD; j += 4)
+                *reinterpret_cast<f32x4*>(o + (4 * q4 + e) * VD + j) =
+                    f32x4{acc[i][j][e], acc[i][j + 1][e], acc[i][j + 2][e], acc[i][j + 3][e]};
+    }
     __syncthreads();
-    constexpr int PER_ROW = D / 4, ROWS = kFewThreads / PER_ROW;
+    constexpr int PER_ROW = D / 4, ROWS = kPagedThreads / PER_ROW;
     const int d = 4 * (threadIdx.x % PER_ROW);
 #pragma unroll
-    for (int i = 0; i < 16 / ROWS; ++i) {
+    for (int i = 0; i < TR / ROWS; ++i) {
         const int n = i * ROWS + threadIdx.x / PER_ROW;
-        if (row0 + n >= rows) continue;
-        float mw[kFewWaves], M = kNegInf, L = 0.0f;
+        float mw[kPagedWaves], M = kNegInf, L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) {
-            mw[w] = lo_ml[w * 16 + n].x;
+        for (int w = 0; w < kPagedWaves; ++w) {
+            mw[w] = lo_ml[w * TR + n].x;
             M = fmaxf(M, mw[w]);
         }
         const float ms = M == kNegInf ? 0.0f : M;
         f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) {
+        for (int w = 0; w < kPagedWaves; ++w) {
             const float f = exp2_raw((mw[w] - ms) * p.c);
-            L += f * lo_ml[w * 16 + n].y;
-            x += f * *reinterpret_cast<const f32x4*>(lo_o + (w * 16 + n) * LD + d);
+            L += f * lo_ml[w * TR + n].y;
+            x += f * *reinterpret_cast<const f32x4*>(lo_o + ((size_t)w * TR + n) * LD + d);
         }
-        const int rr = (row0 + n) / p.G;
-        const int64_t at = job.req.row + rr;
-        const int hd = job.h * p.G + (row0 + n - rr * p.G);
-        const bool none = L == 0.0f;
-        const float inv = none ? 0.0f : 1.0f / L;
-        *reinterpret_cast<uint2*>(p.out + at * p.out_row + (int64_t)hd * D + d) =
-            none ? make_uint2(0u, 0u) : make_uint2(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv));
-        if (d == 0 && p.lse) p.lse[at * p.heads + hd] = none ? kNegInf : M * p.scale + logf(L);
+        if (row0 + n >= rows) continue;
+        if (job.parts == 1) {
+            finish_row(p, job, row0 + n, D, d, x, M, L);
+        } else {  // for a workgroup of this launch, maybe on another XCD
+            const int64_t g = job.slot + (int64_t)job.part * TR + n;
+            put_agent(p.part + g * D + d, x);
+            if (d == 0) put_agent(p.ml + g, make_float2(M, L));
+        }
     }
+}
+
+// Whether this workgroup's was the last range of its tile.
+__device__ __forceinline__ bool last_range(const PagedParams& p, const Job& job) {
+    __shared__ int last;
+    drain_memory();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(p.ctr + job.ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = before == (uint32_t)job.parts - 1;
+        if (last) __hip_atomic_store(p.ctr + job.ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPagedThreads, 2) paged_attn_kernel(PagedParams p) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    const Job job = job_of(p, (int)blockIdx.x);
+    if (job.tile < 0) return;
+    if (job.tile == 16) few_rows<D, 1>(p, job, lds);
+    else few_rows<D, 2>(p, job, lds);
+    if (job.parts > 1 && last_range(p, job)) join_tile<D>(p, job, lds);
 }
 
 }  // namespace krk
