@@ -89,7 +89,7 @@ typedef struct krk_page_step_args {
 int krk_page_step(const krk_page_step_args* args, void* stream);
 
 /* A [pages, page_size, heads, head_dim] tensor of keys or values.  Strides in
- * elements, multiples of 8 and not negative (page at most 2^31); base 16-byte aligned;
+ * elements, multiples of 8 and not negative (below 2^31, slot below 2^25); base 16-byte aligned;
  * the elements of a head are contiguous.  Rows of a written one may not share memory
  * (sorted by size, each stride is at least the extent of what lies inside it); written
  * k and v may be views of one tensor with the same strides. */

@@ -5,7 +5,7 @@
 #include "krk_host.h"
 #include "krk_page_step.h"
 #include "krk_paged.h"
-#include "krk_paged_attn.h"
+#include "krk_paged_many.h"
 #include "krk_rope.h"
 
 namespace {
@@ -63,11 +63,12 @@ int check_pages(const char* name, krk_pages& c, int64_t pages, int64_t slots, in
     if (heads == 1) c.head = 0;
     const int64_t st[3] = {c.page, c.slot, c.head}, n[3] = {pages, slots, heads};
     for (int i = 0; i < 3; ++i) {
-        if (st[i] < 0 || st[i] > (int64_t)1 << 31)
-            return fail(kErrInvalid, "%s: stride %lld out of range (0 .. 2^31)", name, (long long)st[i]);
+        if (st[i] < 0 || st[i] >= (int64_t)1 << 31)
+            return fail(kErrInvalid, "%s: stride %lld out of range (below 2^31)", name, (long long)st[i]);
         if (st[i] % 8) return fail(kErrAlign, "%s: strides must be multiples of 8 elements", name);
     }
-    if (c.slot >= (int64_t)1 << 31) return fail(kErrInvalid, "%s: stride %lld from key to key out of range", name, (long long)c.slot);
+    // Offsets among the 64 keys of a step are 32 bits of bytes.
+    if (c.slot >= (int64_t)1 << 25) return fail(kErrInvalid, "%s: stride %lld from key to key out of range (below 2^25)", name, (long long)c.slot);
     if (written && !nested(st, n, dim))
         return fail(kErrAlias, "%s is written: with strides of %lld, %lld and %lld its rows share memory", name, (long long)st[0], (long long)st[1], (long long)st[2]);
     if (!aligned(c.p, 16)) return fail(kErrAlign, "%s must be 16-byte aligned", name);
@@ -125,6 +126,7 @@ int check_shape(const krk_paged_shape& s) {
 
 // -------------------------------------------------------------------- plan
 struct Plan {
+    bool many;  // some request may have more than kFewPairs rows of a head
     int64_t blocks;
     size_t ctr, part, ml, bytes;  // workspace: sizes of its parts and their sum
 };
@@ -132,15 +134,18 @@ struct Plan {
 Plan make_plan(const krk_paged_shape& s) {
     Plan p{};
     const int64_t RG = (int64_t)s.rows * (s.heads / s.kv_heads);
+    p.many = RG > krk::kFewPairs;
     // Tiles of 16 rows at least, and each request with rows has one that is not full.
     const int64_t tiles = s.kv_heads * (RG / 16 + (s.B < s.rows ? s.B : s.rows));
-    // Their key ranges: as many as the longest request would have, and those of tiles
+    // Their key ranges: as many as the longest request could have, and those of tiles
     // that have several are limited.
-    const int64_t parts = cdiv(cdiv((int64_t)s.width * s.page_size, krk::kFewStep), krk::kFewLeast);
+    const int64_t keys = (int64_t)s.width * s.page_size;
+    int64_t parts = cdiv(keys, krk::kFewStep * krk::kFewLeast);
+    if (p.many) parts = parts > cdiv(keys, krk::kManyStep * krk::kManyLeast) ? parts : cdiv(keys, krk::kManyStep * krk::kManyLeast);
     const int64_t split = tiles * parts < krk::kSplitJobs ? tiles * parts : krk::kSplitJobs;
     p.blocks = tiles + (parts > 1 ? split : 0);
     if (parts > 1) {
-        const size_t rows = (size_t)(32 * split);
+        const size_t rows = (size_t)split * (p.many ? krk::kManyRows : 32);
         p.ctr = align_up(krk::kCounters * sizeof(uint32_t), 256);
         p.part = rows * s.head_dim * sizeof(float);
         p.ml = rows * sizeof(float2);
@@ -149,11 +154,12 @@ Plan make_plan(const krk_paged_shape& s) {
     return p;
 }
 
-template <int D>
+template <int D, bool MANY>
 int launch_attn(const krk::PagedParams& p, const Plan& plan, hipStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    const void* fn = reinterpret_cast<const void*>(&krk::paged_attn_kernel<D>);
-    const size_t shm = krk::few_lds_bytes<D>();
+    const void* fn = reinterpret_cast<const void*>(&krk::paged_attn_kernel<D, MANY>);
+    constexpr size_t few = krk::few_lds_bytes<D>(), many = krk::tile_lds_bytes<D>();
+    constexpr size_t shm = MANY && many > few ? many : few;
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "paged_attn_kernel LDS size");
     void* args[] = {(void*)&p};
     return hip_status(hipLaunchKernel(fn, dim3((unsigned)plan.blocks), dim3(krk::kPagedThreads), args, shm, stream), "paged_attn_kernel launch");
@@ -363,7 +369,8 @@ int krk_paged_attn_bf16(const krk_paged_shape* shape, const krk_paged_attn_args*
     p.window = s.window;
     p.sinks = s.sinks;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    return s.head_dim == 128 ? launch_attn<128>(p, plan, st) : launch_attn<64>(p, plan, st);
+    if (s.head_dim == 128) return plan.many ? launch_attn<128, true>(p, plan, st) : launch_attn<128, false>(p, plan, st);
+    return plan.many ? launch_attn<64, true>(p, plan, st) : launch_attn<64, false>(p, plan, st);
 }
 
 }  // extern "C"

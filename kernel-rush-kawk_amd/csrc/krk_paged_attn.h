@@ -52,16 +52,17 @@ constexpr int kPagedWaves = kPagedThreads / 64;
 
 // Workgroups that the work is cut for: two a CU.
 constexpr int kTarget = 512;
-// Of more than one range each, tiles have less than twice as many ranges as there are
-// of the target's size: fewer than 2 * kTarget jobs.  A tile has two at least.
+// Tiles of more than one range have less than twice as many ranges as there are of the
+// target's size: fewer than 2 * kTarget jobs.  A tile has two at least.
 constexpr int kSplitJobs = 2 * kTarget + 16;
 constexpr int kCounters = kSplitJobs;
-constexpr int kFewStep = 32 * kPagedWaves;  // keys of a step of a workgroup
 constexpr int kFewPairs = 64;               // rows of a head that jobs of few rows take
-// Least steps of a range.
-constexpr int kFewLeast = 2;
-// What a step costs, in us of one of two workgroups of a CU.
-constexpr float kFewCost = 1.0f;
+constexpr int kManyRows = 128;              // rows of a job of many
+// Keys of a step of a workgroup, least steps of a range, and what a step costs, in us of
+// one of two workgroups of a CU (head size 128; only their proportion is of matter).
+constexpr int kFewStep = 32 * kPagedWaves, kManyStep = 64;
+constexpr int kFewLeast = 2, kManyLeast = 4;
+constexpr float kFewCost = 5.0f, kManyCost = 2.0f;
 
 // A request: its first row, rows and keys, whatever the arrays hold.
 struct Request {
@@ -82,19 +83,23 @@ __device__ __forceinline__ Request request(const PagedParams& p, int b) {
 // How a request's rows of one head are cut: tiles of `tile` rows, over `steps` steps of
 // keys at most.
 struct Tiling {
+    bool many;
     int tile, tiles, steps;
 };
 __device__ __forceinline__ Tiling tiling(const PagedParams& p, const Request& r) {
     Tiling t;
     const int rows = r.n * p.G;
-    t.tile = rows <= 16 ? 16 : 32;
+    t.many = rows > kFewPairs;
+    t.tile = t.many ? kManyRows : rows <= 16 ? 16 : 32;
     t.tiles = (rows + t.tile - 1) / t.tile;
     int keys = r.len;
     if (p.window) {
-        const int near = p.window + p.sinks + r.n;
+        const int of_tile = t.tile / p.G + 2;  // positions of a tile's rows
+        const int near = p.window + p.sinks + (r.n < of_tile ? r.n : of_tile) + kManyStep;
         keys = near < keys ? near : keys;
     }
-    t.steps = (keys + kFewStep - 1) / kFewStep;
+    const int step = t.many ? kManyStep : kFewStep;
+    t.steps = (keys + step - 1) / step;
     return t;
 }
 
@@ -127,27 +132,37 @@ __device__ __forceinline__ Job job_of(const PagedParams& p, int id) {
         const Request r = b == b0 ? first : request(p, b);
         const Tiling t = tiling(p, r);
         all_rows += r.n;
-        cost += (float)t.tiles * (float)p.kv_heads * (float)t.steps * kFewCost;
+        cost += (float)t.tiles * (float)p.kv_heads * (float)t.steps * (t.many ? kManyCost : kFewCost);
     }
-    const int most = (int)(wave_total(cost) * (1.0f / (kTarget * kFewCost))) + 1;  // steps of a range
-    const int few = most > kFewLeast ? most : kFewLeast;
+    const float share = wave_total(cost) * (1.0f / kTarget);  // of a workgroup
+    auto range = [&](float of_step, int least) {
+        const int steps = (int)(share / of_step) + 1;
+        return steps > least ? steps : least;
+    };
+    const int few = range(kFewCost, kFewLeast), many = range(kManyCost, kManyLeast);
     // Jobs, tiles of several ranges and rows of their results.
     auto cut = [&](const Tiling& t, int* parts, int* jobs, int* ctrs, int* rows) {
-        *parts = t.steps > few ? (t.steps + few - 1) / few : 1;
+        const int most = t.many ? many : few;
+        *parts = t.steps > most ? (t.steps + most - 1) / most : 1;
         *ctrs = *parts > 1 ? t.tiles * p.kv_heads : 0;
         *jobs = t.tiles * p.kv_heads * *parts;
         *rows = *parts > 1 ? *jobs * t.tile : 0;
     };
-    int jobs = 0, ctrs = 0, rows = 0;
+    int jobs[2] = {0, 0}, ctrs = 0, rows = 0;
     for (int b = b0; b < b1; ++b) {
+        const Tiling t = tiling(p, b == b0 ? first : request(p, b));
         int parts, x, y, z;
-        cut(tiling(p, b == b0 ? first : request(p, b)), &parts, &x, &y, &z);
-        jobs += x;
+        cut(t, &parts, &x, &y, &z);
+        jobs[t.many ? 0 : 1] += x;
         ctrs += y;
         rows += z;
     }
-    int left = id - (wave_scan(jobs) - jobs), ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows;
-    const uint64_t who = __ballot(left >= 0 && left < jobs);
+    // Jobs of many rows first: they take longest.
+    const int upto_many = wave_scan(jobs[0]), all_many = __builtin_amdgcn_readlane(upto_many, 63);
+    const bool want_many = id < all_many;
+    const int before = want_many ? upto_many - jobs[0] : all_many + wave_scan(jobs[1]) - jobs[1];
+    int left = id - before, ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows;
+    const uint64_t who = __ballot(left >= 0 && left < (want_many ? jobs[0] : jobs[1]));
     Job j;
     j.tile = -1;
     // More rows than the call has, as starts do not ascend: the jobs' bounds would not hold.
@@ -158,10 +173,13 @@ __device__ __forceinline__ Job job_of(const PagedParams& p, int id) {
     if (lane == src)
         for (; b < b1; ++b) {
             r = b == b0 ? first : request(p, b);
+            const Tiling t = tiling(p, r);
             int x, y, z;
-            cut(tiling(p, r), &parts, &x, &y, &z);
-            if (left < x) break;
-            left -= x;
+            cut(t, &parts, &x, &y, &z);
+            if (t.many == want_many) {
+                if (left < x) break;
+                left -= x;
+            }
             ctr += y;
             slot += z;
         }
@@ -555,28 +573,22 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
     }
 }
 
-// Whether this workgroup's was the last range of its tile.
-__device__ __forceinline__ bool last_range(const PagedParams& p, const Job& job) {
-    __shared__ int last;
+// Whether this workgroup's was the last range of its tile.  (Through the front of lds,
+// which nobody uses any more: the tile kernel's 80 KB are all that two workgroups of a
+// CU can have.)
+__device__ __forceinline__ bool last_range(const PagedParams& p, const Job& job, unsigned char* lds) {
+    int* last = reinterpret_cast<int*>(lds);
     drain_memory();
     __syncthreads();
     if (threadIdx.x == 0) {
         const uint32_t before = __hip_atomic_fetch_add(p.ctr + job.ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = before == (uint32_t)job.parts - 1;
-        if (last) __hip_atomic_store(p.ctr + job.ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = before == (uint32_t)job.parts - 1;
+        if (*last) __hip_atomic_store(p.ctr + job.ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    return last;
-}
-
-template <int D>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_attn_kernel(PagedParams p) {
-    extern __shared__ __align__(16) unsigned char lds[];
-    const Job job = job_of(p, (int)blockIdx.x);
-    if (job.tile < 0) return;
-    if (job.tile == 16) few_rows<D, 1>(p, job, lds);
-    else few_rows<D, 2>(p, job, lds);
-    if (job.parts > 1 && last_range(p, job)) join_tile<D>(p, job, lds);
+    const bool yes = *last;
+    __syncthreads();
+    return yes;
 }
 
 }  // namespace krk
