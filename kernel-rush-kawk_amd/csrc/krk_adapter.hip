@@ -35,17 +35,38 @@ struct Plan {
     size_t bytes;
 };
 
+// Rows up to kByRow: a workgroup per row, which takes the rows of its tile of 16 that
+// have its adapter, if it is their first.  More: tiles of 64 rows, adapter by adapter.
+constexpr int kByRow = 256;
+// Steps of 32 of K that a wave of the first launch has in flight.
+constexpr int kFewAhead = 4, kManyAhead = 2;
+
 Plan make_plan(const krk_adapter_shape& s) {
     Plan p{};
-    p.by_row = s.rows <= 256;
-    p.blocks = p.by_row ? s.rows : (int)cdiv(s.rows, 16);
+    p.by_row = s.rows <= kByRow;
+    p.blocks = p.by_row ? s.rows : (int)cdiv(s.rows, 64);
     p.groups = (int)cdiv((int64_t)s.slices * s.rank, 16 * krk::kAdapterTiles);
     const int64_t want = cdiv(2 * kCuCount, (int64_t)p.blocks * p.groups);
-    const int64_t most = cdiv(s.K, krk::kAdapterChunk * krk::kAdapterWaves);
+    const int64_t most = cdiv(s.K, 32 * (p.by_row ? kFewAhead : kManyAhead) * krk::kAdapterWaves);
     p.splits = (int)(want < most ? want : most);
-    p.splits = p.splits < 8 ? p.splits : 8;
+    p.splits = p.splits < krk::kAdapterSplits ? p.splits : krk::kAdapterSplits;
     p.bytes = align_up((size_t)p.splits * s.rows * s.slices * s.rank * sizeof(float), 256);
     return p;
+}
+
+template <int MT, int U>
+int launch(const krk::AdapterParams& p, const Plan& plan, bool silu, int col_blocks, hipStream_t st) {
+    void* kargs[] = {(void*)&p};
+    hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_shrink_kernel<MT, U>),
+                                   dim3(plan.blocks, plan.splits, plan.groups), dim3(krk::kAdapterThreads), kargs, 0, st);
+    if (int rc = hip_status(e, "adapter_shrink_kernel launch")) return rc;
+    const void* fn = silu ? reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, true>)
+                          : reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, false>);
+    static std::atomic<uint64_t> done[2];
+    const size_t row = 16 * MT * (silu ? 2 : 1);
+    if (hipError_t x = ensure_lds_limit(fn, row * krk::adapter_row_bytes(128), done[silu])) return hip_status(x, "adapter_expand_kernel LDS size");
+    e = hipLaunchKernel(fn, dim3(plan.blocks, col_blocks), dim3(krk::kAdapterThreads), kargs, row * krk::adapter_row_bytes(p.rank), st);
+    return hip_status(e, "adapter_expand_kernel launch");
 }
 
 // A factor of each adapter: [adapters, rows, cols].
@@ -145,18 +166,11 @@ int krk_adapter_bf16(const krk_adapter_shape* shape, const krk_adapter_args* arg
     for (int i = 0; i < s.slices; ++i) {
         p.width[i] = s.widths[i];
         p.first[i] = i ? p.first[i - 1] + s.widths[i - 1] : 0;
-        p.group[i + 1] = p.group[i] + (int)cdiv(s.widths[i], krk::kAdapterCols);
+        p.block[i + 1] = p.block[i] + (int)cdiv(s.widths[i], krk::kAdapterWaves * krk::kAdapterCols);
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    void* kargs[] = {(void*)&p};
-    hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_shrink_kernel), dim3(plan.blocks, plan.splits, plan.groups),
-                                   dim3(krk::kAdapterThreads), kargs, 0, st);
-    if (int rc = hip_status(e, "adapter_shrink_kernel launch")) return rc;
-    const void* fn = s.silu ? reinterpret_cast<const void*>(&krk::adapter_expand_kernel<true>)
-                            : reinterpret_cast<const void*>(&krk::adapter_expand_kernel<false>);
-    const int64_t groups = s.silu ? cdiv(out_cols, krk::kAdapterCols) : p.group[s.slices];
-    return hip_status(hipLaunchKernel(fn, dim3(plan.blocks, (unsigned)cdiv(groups, krk::kAdapterWaves)), dim3(krk::kAdapterThreads), kargs, 0, st),
-                      "adapter_expand_kernel launch");
+    const int col_blocks = s.silu ? (int)cdiv(out_cols, krk::kAdapterWaves * krk::kAdapterCols) : p.block[s.slices];
+    return plan.by_row ? launch<1, kFewAhead>(p, plan, s.silu, col_blocks, st) : launch<4, kManyAhead>(p, plan, s.silu, col_blocks, st);
 }
 
 }  // extern "C"
