@@ -30,43 +30,79 @@ int check_shape(const krk_adapter_shape& s) {
 }
 
 struct Plan {
-    bool by_row;
-    int blocks, groups, splits;  // of rows; of 64 rows of A; ranges of K
-    size_t bytes;
+    bool many;              // tiles of 64 rows, else of 16
+    int tiles, groups;      // of rows; of 64 rows of A
+    int splits;             // ranges of K
+    int shrink_slots, expand_slots;
+    int col_blocks;
+    size_t h, joined, bytes;  // workspace: sizes of its parts and their sum
 };
 
-// Rows up to kByRow: a workgroup per row, which takes the rows of its tile of 16 that
-// have its adapter, if it is their first.  More: tiles of 64 rows, adapter by adapter.
-constexpr int kByRow = 256;
-// Steps of 32 of K that a wave of the first launch has in flight.
-constexpr int kFewAhead = 4, kManyAhead = 2;
+constexpr int kFewRows = 256;
+// Workgroups that the slots of a tile's adapters may come to: those without one cost 9 ns
+// each (64 rows of 4 runs, 38 blocks of columns: a workgroup for every row took 25 us).
+constexpr int kSlotBlocks = 1024;
+
+int slots(int64_t blocks, int rows) {
+    const int64_t s = kSlotBlocks / blocks;
+    return (int)(s < 1 ? 1 : s < rows ? s : rows);
+}
 
 Plan make_plan(const krk_adapter_shape& s) {
     Plan p{};
-    p.by_row = s.rows <= kByRow;
-    p.blocks = p.by_row ? s.rows : (int)cdiv(s.rows, 64);
+    p.many = s.rows > kFewRows;
+    const int tile = p.many ? 64 : 16, most_sets = tile < s.rows ? tile : s.rows;
+    p.tiles = (int)cdiv(s.rows, tile);
     p.groups = (int)cdiv((int64_t)s.slices * s.rank, 16 * krk::kAdapterTiles);
-    const int64_t want = cdiv(2 * kCuCount, (int64_t)p.blocks * p.groups);
-    const int64_t most = cdiv(s.K, 32 * (p.by_row ? kFewAhead : kManyAhead) * krk::kAdapterWaves);
+    const int64_t want = cdiv(2 * kCuCount, (int64_t)p.tiles * p.groups);
+    const int64_t most = p.many ? cdiv(s.K, 4 * krk::kAdapterManyStep) : cdiv(s.K, krk::kAdapterWaves * krk::kAdapterFewStep);
     p.splits = (int)(want < most ? want : most);
     p.splits = p.splits < krk::kAdapterSplits ? p.splits : krk::kAdapterSplits;
-    p.bytes = align_up((size_t)p.splits * s.rows * s.slices * s.rank * sizeof(float), 256);
+    p.shrink_slots = slots((int64_t)p.tiles * p.groups * p.splits, most_sets);
+    for (int i = 0; i < s.slices; ++i) p.col_blocks += (int)cdiv(s.widths[i], krk::kAdapterWaves * krk::kAdapterCols);
+    if (s.silu) p.col_blocks = (int)cdiv(s.N / 2, krk::kAdapterWaves * krk::kAdapterCols);
+    const int expand_tiles = p.many ? (int)cdiv(s.rows, 32) : p.tiles;
+    p.expand_slots = slots((int64_t)expand_tiles * p.col_blocks, most_sets);
+    const size_t values = (size_t)s.rows * s.slices * s.rank;
+    p.h = align_up(p.splits * values * sizeof(float), 256);
+    p.joined = p.many ? align_up(2 * values * sizeof(uint16_t), 256) : 0;
+    p.bytes = p.h + p.joined;
     return p;
 }
 
-template <int MT, int U>
-int launch(const krk::AdapterParams& p, const Plan& plan, bool silu, int col_blocks, hipStream_t st) {
+int launch_shrink(krk::AdapterParams p, const Plan& plan, hipStream_t st) {
+    p.slots = plan.shrink_slots;
     void* kargs[] = {(void*)&p};
-    hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_shrink_kernel<MT, U>),
-                                   dim3(plan.blocks, plan.splits, plan.groups), dim3(krk::kAdapterThreads), kargs, 0, st);
-    if (int rc = hip_status(e, "adapter_shrink_kernel launch")) return rc;
-    const void* fn = silu ? reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, true>)
-                          : reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, false>);
-    static std::atomic<uint64_t> done[2];
-    const size_t row = 16 * MT * (silu ? 2 : 1);
-    if (hipError_t x = ensure_lds_limit(fn, row * krk::adapter_row_bytes(128), done[silu])) return hip_status(x, "adapter_expand_kernel LDS size");
-    e = hipLaunchKernel(fn, dim3(plan.blocks, col_blocks), dim3(krk::kAdapterThreads), kargs, row * krk::adapter_row_bytes(p.rank), st);
+    const void* fn = plan.many ? reinterpret_cast<const void*>(&krk::adapter_shrink64_kernel) : reinterpret_cast<const void*>(&krk::adapter_shrink_kernel);
+    const hipError_t e = hipLaunchKernel(fn, dim3(plan.splits, plan.tiles * p.slots, plan.groups), dim3(krk::kAdapterThreads), kargs, 0, st);
+    return hip_status(e, "adapter_shrink_kernel launch");
+}
+
+template <int MT, bool SILU, bool JOINED>
+int launch_expand(krk::AdapterParams p, const Plan& plan, hipStream_t st) {
+    p.slots = plan.expand_slots;
+    void* kargs[] = {(void*)&p};
+    const void* fn = reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, SILU, JOINED>);
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t rows = JOINED ? 0 : 16 * MT * (SILU ? 2 : 1);
+    if (rows)
+        if (hipError_t x = ensure_lds_limit(fn, rows * krk::adapter_row_bytes(128), done)) return hip_status(x, "adapter_expand_kernel LDS size");
+    const hipError_t e = hipLaunchKernel(fn, dim3(plan.col_blocks, (unsigned)cdiv(p.rows, 16 * MT) * p.slots), dim3(krk::kAdapterThreads), kargs,
+                                         rows * krk::adapter_row_bytes(p.rank), st);
     return hip_status(e, "adapter_expand_kernel launch");
+}
+
+template <bool SILU>
+int launch(const krk::AdapterParams& p, const Plan& plan, hipStream_t st) {
+    if (int rc = launch_shrink(p, plan, st)) return rc;
+    if (!plan.many) return launch_expand<1, SILU, false>(p, plan, st);
+    krk::AdapterParams q = p;
+    void* kargs[] = {(void*)&q};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_join_kernel), dim3((unsigned)cdiv((int64_t)p.rows * (p.HN / 4), 256)),
+                                         dim3(256), kargs, 0, st);
+    if (int rc = hip_status(e, "adapter_join_kernel launch")) return rc;
+    // 32 rows: with 64 few workgroups are left (4096 rows of 2560 columns: 31 us against 23).
+    return launch_expand<2, SILU, true>(p, plan, st);
 }
 
 // A factor of each adapter: [adapters, rows, cols].
@@ -161,7 +197,7 @@ int krk_adapter_bf16(const krk_adapter_shape* shape, const krk_adapter_args* arg
     p.adapters = a.adapters;
     p.splits = plan.splits;
     p.slices = s.slices;
-    p.by_row = plan.by_row;
+    p.joined = plan.joined ? reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(workspace) + plan.h) : nullptr;
     p.same = same;
     for (int i = 0; i < s.slices; ++i) {
         p.width[i] = s.widths[i];
@@ -169,8 +205,7 @@ int krk_adapter_bf16(const krk_adapter_shape* shape, const krk_adapter_args* arg
         p.block[i + 1] = p.block[i] + (int)cdiv(s.widths[i], krk::kAdapterWaves * krk::kAdapterCols);
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int col_blocks = s.silu ? (int)cdiv(out_cols, krk::kAdapterWaves * krk::kAdapterCols) : p.block[s.slices];
-    return plan.by_row ? launch<1, kFewAhead>(p, plan, s.silu, col_blocks, st) : launch<4, kManyAhead>(p, plan, s.silu, col_blocks, st);
+    return s.silu ? launch<true>(p, plan, st) : launch<false>(p, plan, st);
 }
 
 }  // extern "C"

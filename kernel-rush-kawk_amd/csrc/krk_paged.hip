@@ -135,8 +135,10 @@ Plan make_plan(const krk_paged_shape& s) {
     Plan p{};
     const int64_t RG = (int64_t)s.rows * (s.heads / s.kv_heads);
     p.many = RG > krk::kFewPairs;
-    // Tiles of 16 rows at least, and each request with rows has one that is not full.
-    const int64_t tiles = s.kv_heads * (RG / 16 + (s.B < s.rows ? s.B : s.rows));
+    // A request with rows has up to two tiles where they are few, of 16 rows or more but
+    // for the last; else tiles of 128.
+    const int64_t live = s.B < s.rows ? s.B : s.rows;
+    const int64_t tiles = s.kv_heads * (RG / krk::kManyRows + (live < RG / 16 ? 2 * live : live + RG / 16));
     // Their key ranges: as many as the longest request could have, and those of tiles
     // that have several are limited.
     const int64_t keys = (int64_t)s.width * s.page_size;
