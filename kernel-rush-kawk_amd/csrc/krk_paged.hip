@@ -142,12 +142,15 @@ Plan make_plan(const krk_paged_shape& s) {
     // Their key ranges: as many as the longest request could have, and those of tiles
     // that have several are limited.
     const int64_t keys = (int64_t)s.width * s.page_size;
-    int64_t parts = cdiv(keys, krk::kFewStep * krk::kFewLeast);
-    if (p.many) parts = parts > cdiv(keys, krk::kManyStep * krk::kManyLeast) ? parts : cdiv(keys, krk::kManyStep * krk::kManyLeast);
-    const int64_t split = tiles * parts < krk::kSplitJobs ? tiles * parts : krk::kSplitJobs;
-    p.blocks = tiles + (parts > 1 ? split : 0);
-    if (parts > 1) {
-        const size_t rows = (size_t)split * (p.many ? krk::kManyRows : 32);
+    auto splits = [&](int64_t least, int64_t most) {
+        const int64_t parts = cdiv(keys, least);
+        return parts < 2 ? 0 : tiles * parts < most ? tiles * parts : most;
+    };
+    const int64_t few = splits(krk::kFewStep * krk::kFewLeast, krk::kFewSplits);
+    const int64_t many = p.many ? splits(krk::kManyStep * krk::kManyLeast, krk::kManySplits) : 0;
+    p.blocks = tiles + few + many;
+    if (few + many) {
+        const size_t rows = (size_t)(few * 32 + many * krk::kManyRows);
         p.ctr = align_up(krk::kCounters * sizeof(uint32_t), 256);
         p.part = rows * s.head_dim * sizeof(float);
         p.ml = rows * sizeof(float2);
@@ -365,6 +368,8 @@ int krk_paged_attn_bf16(const krk_paged_shape* shape, const krk_paged_attn_args*
     p.heads = s.heads;
     p.kv_heads = s.kv_heads;
     p.G = s.heads / s.kv_heads;
+    p.inv_G = 1.0f / (float)p.G;
+    p.inv_kv = 1.0f / (float)s.kv_heads;
     p.pages = a.pages;
     p.shift = page_shift(s.page_size);
     p.width = s.width;

@@ -45,24 +45,38 @@ struct PagedParams {
     float scale;    // of q.k
     float c;        // scale * log2(e)
     int B, rows, heads, kv_heads, G, pages, shift, width, window, sinks;
+    float inv_G, inv_kv;  // 1 / G, 1 / kv_heads
 };
 
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 
-// Workgroups that the work is cut for: two a CU.
-constexpr int kTarget = 512;
-// Tiles of more than one range have less than twice as many ranges as there are of the
-// target's size: fewer than 2 * kTarget jobs.  A tile has two at least.
-constexpr int kSplitJobs = 2 * kTarget + 16;
-constexpr int kCounters = kSplitJobs;
-constexpr int kFewPairs = 64;               // rows of a head that jobs of few rows take
-constexpr int kManyRows = 128;              // rows of a job of many
+// Workgroups that the work is cut for: one a CU, though two run at once (ranges half as
+// long: 4 drafts of 8 rows 21 -> 30 us, 100 rows over 16000 keys 86 -> 118, 32 requests of
+// 4000 keys 88 -> 98).
+constexpr int kTarget = 256;
+constexpr int kFewPairs = 64;   // rows of a head that tiles of few rows (16 or 32) take
+constexpr int kManyRows = 128;  // rows of a job of many
 // Keys of a step of a workgroup, least steps of a range, and what a step costs, in us of
 // one of two workgroups of a CU (head size 128; only their proportion is of matter).
 constexpr int kFewStep = 32 * kPagedWaves, kManyStep = 64;
-constexpr int kFewLeast = 2, kManyLeast = 4;
+constexpr int kFewLeast = 1, kManyLeast = 4;
 constexpr float kFewCost = 5.0f, kManyCost = 2.0f;
+// Jobs that do not all run at once: where a share of the work is long, ranges of few
+// rows are cut finer, into up to kRounds a workgroup of at least kGrain us each.
+constexpr int kRounds = 4;
+constexpr float kGrain = 25.0f;
+// Tiles of more than one range have less than twice as many ranges as there are of the
+// target's size.  A tile has two at least.
+constexpr int kFewSplits = 2 * kRounds * kTarget + 64, kManySplits = 2 * kTarget + 64;
+constexpr int kCounters = (kFewSplits + kManySplits) / 2;
+
+// n / d by its reciprocal (off by one at most), then put right.
+__device__ __forceinline__ int quotient(int n, int d, float inv) {
+    int q = (int)((float)n * inv);
+    const int r = n - q * d;
+    return q + (r >= d) - (r < 0);
+}
 
 // A request: its first row, rows and keys, whatever the arrays hold.
 struct Request {
@@ -80,26 +94,25 @@ __device__ __forceinline__ Request request(const PagedParams& p, int b) {
     return x;
 }
 
-// How a request's rows of one head are cut: tiles of `tile` rows, over `steps` steps of
-// keys at most.
+// How a request's rows of one head are cut: tiles of 1 << shift rows, over `steps` steps
+// of keys at most.
 struct Tiling {
     bool many;
-    int tile, tiles, steps;
+    int shift, tiles, steps;
 };
 __device__ __forceinline__ Tiling tiling(const PagedParams& p, const Request& r) {
     Tiling t;
     const int rows = r.n * p.G;
     t.many = rows > kFewPairs;
-    t.tile = t.many ? kManyRows : rows <= 16 ? 16 : 32;
-    t.tiles = (rows + t.tile - 1) / t.tile;
+    t.shift = t.many ? 7 : rows <= 16 ? 4 : 5;
+    t.tiles = (rows + (1 << t.shift) - 1) >> t.shift;
     int keys = r.len;
     if (p.window) {
-        const int of_tile = t.tile / p.G + 2;  // positions of a tile's rows
+        const int of_tile = quotient(1 << t.shift, p.G, p.inv_G) + 2;  // positions of a tile's rows
         const int near = p.window + p.sinks + (r.n < of_tile ? r.n : of_tile) + kManyStep;
         keys = near < keys ? near : keys;
     }
-    const int step = t.many ? kManyStep : kFewStep;
-    t.steps = (keys + step - 1) / step;
+    t.steps = t.many ? (keys + kManyStep - 1) / kManyStep : (keys + kFewStep - 1) / kFewStep;
     return t;
 }
 
@@ -120,86 +133,139 @@ struct Job {
     Request req;
 };
 
+// Requests of a lane that stay in registers (of calls of up to 256).
+constexpr int kHeld = 4;
+
 __device__ __forceinline__ Job job_of(const PagedParams& p, int id) {
     const int lane = threadIdx.x & 63;
     const int per = (p.B + 63) / 64;
-    const int b0 = lane * per, b1 = b0 + per < p.B ? b0 + per : p.B;
-    const Request none = {0, 0, 0};
-    const Request first = b0 < b1 ? request(p, b0) : none;
+    const int b0 = lane * per;
+    int n = p.B - b0;
+    n = n < 0 ? 0 : n < per ? n : per;
+    Request held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        held[i] = Request{0, 0, 0};
+        if (i < per) {  // the same for all lanes
+            held[i] = request(p, i < n ? b0 + i : p.B - 1);
+            if (i >= n) held[i].n = 0;
+        }
+    }
+    // f(i, request) of this lane's requests in order, those of no rows too.
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (i < per) f(i, held[i]);
+        for (int i = kHeld; i < n; ++i) f(i, request(p, b0 + i));
+    };
     float cost = 0.0f;
     int all_rows = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Request r = b == b0 ? first : request(p, b);
+    each([&](int, const Request& r) {
         const Tiling t = tiling(p, r);
         all_rows += r.n;
-        cost += (float)t.tiles * (float)p.kv_heads * (float)t.steps * (t.many ? kManyCost : kFewCost);
-    }
-    const float share = wave_total(cost) * (1.0f / kTarget);  // of a workgroup
-    auto range = [&](float of_step, int least) {
-        const int steps = (int)(share / of_step) + 1;
-        return steps > least ? steps : least;
+        cost += (float)(t.tiles * t.steps) * (t.many ? kManyCost : kFewCost);
+    });
+    const float share = wave_total(cost) * (float)p.kv_heads * (1.0f / kTarget);  // of a workgroup
+    // Steps of a range.
+    auto at_least = [](float steps, int least) { return (int)steps + 1 > least ? (int)steps + 1 : least; };
+    int few = at_least(share * (1.0f / kFewCost), kFewLeast);
+    const int many = at_least(share * (1.0f / kManyCost), kManyLeast);
+    float inv_few = __builtin_amdgcn_rcpf((float)few);
+    const float inv_many = __builtin_amdgcn_rcpf((float)many);
+    // Ranges, jobs, tiles of several ranges and rows of their results.
+    struct Cut {
+        int parts, jobs, ctrs, rows;
     };
-    const int few = range(kFewCost, kFewLeast), many = range(kManyCost, kManyLeast);
-    // Jobs, tiles of several ranges and rows of their results.
-    auto cut = [&](const Tiling& t, int* parts, int* jobs, int* ctrs, int* rows) {
-        const int most = t.many ? many : few;
-        *parts = t.steps > most ? (t.steps + most - 1) / most : 1;
-        *ctrs = *parts > 1 ? t.tiles * p.kv_heads : 0;
-        *jobs = t.tiles * p.kv_heads * *parts;
-        *rows = *parts > 1 ? *jobs * t.tile : 0;
+    auto cut = [&](const Tiling& t) {
+        Cut c;
+        c.parts = t.steps > (t.many ? many : few) ? (int)((float)(t.steps - 1) * (t.many ? inv_many : inv_few)) + 1 : 1;
+        const int tiles = t.tiles * p.kv_heads;
+        c.ctrs = c.parts > 1 ? tiles : 0;
+        c.jobs = tiles * c.parts;
+        c.rows = c.parts > 1 ? c.jobs << t.shift : 0;
+        return c;
     };
-    int jobs[2] = {0, 0}, ctrs = 0, rows = 0;
-    for (int b = b0; b < b1; ++b) {
-        const Tiling t = tiling(p, b == b0 ? first : request(p, b));
-        int parts, x, y, z;
-        cut(t, &parts, &x, &y, &z);
-        jobs[t.many ? 0 : 1] += x;
-        ctrs += y;
-        rows += z;
+    int jobs_many, jobs_few, ctrs, rows, upto_many, upto_few, all_many, all_few;
+    auto count = [&]() {
+        jobs_many = jobs_few = ctrs = rows = 0;
+        each([&](int, const Request& r) {
+            const Tiling t = tiling(p, r);
+            const Cut c = cut(t);
+            jobs_many += t.many ? c.jobs : 0;
+            jobs_few += t.many ? 0 : c.jobs;
+            ctrs += c.ctrs;
+            rows += c.rows;
+        });
+        upto_many = wave_scan(jobs_many);
+        upto_few = wave_scan(jobs_few);
+        all_many = __builtin_amdgcn_readlane(upto_many, 63);
+        all_few = __builtin_amdgcn_readlane(upto_few, 63);
+    };
+    count();
+    if (all_many + all_few > kTarget && all_few) {
+        // A few jobs too many would run by themselves behind the others: either ranges
+        // that long that all run at once, or, where they are long, short ones.
+        float rounds = floorf(share * (1.0f / kGrain));
+        rounds = rounds > (float)kRounds ? (float)kRounds : rounds;
+        few = rounds >= 2.0f ? at_least(share / (kFewCost * rounds), kFewLeast)
+                             : at_least((float)few * (float)(all_many + all_few) * (1.0f / kTarget), kFewLeast);
+        inv_few = __builtin_amdgcn_rcpf((float)few);
+        count();
     }
-    // Jobs of many rows first: they take longest.
-    const int upto_many = wave_scan(jobs[0]), all_many = __builtin_amdgcn_readlane(upto_many, 63);
-    const bool want_many = id < all_many;
-    const int before = want_many ? upto_many - jobs[0] : all_many + wave_scan(jobs[1]) - jobs[1];
-    int left = id - before, ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows;
-    const uint64_t who = __ballot(left >= 0 && left < (want_many ? jobs[0] : jobs[1]));
+    // Which kind, and which of its jobs: 256 of many rows, which keep the matrix pipe
+    // busy, and 256 of few, which read, in turn, so that a CU has one of each; then what
+    // is left of the many and of the few.
+    const int both = (all_many < all_few ? all_many : all_few) >> 8;
+    bool want_many = !(id >> 8 & 1);
+    int nth = (id >> 9 << 8) + (id & 255);
+    if (id >= both << 9) {
+        nth = id - (both << 8);
+        want_many = nth < all_many;
+        nth = want_many ? nth : id - all_many;
+    }
+    int left = nth - (want_many ? upto_many - jobs_many : upto_few - jobs_few);
+    const uint64_t who = __ballot(left >= 0 && left < (want_many ? jobs_many : jobs_few));
     Job j;
     j.tile = -1;
     // More rows than the call has, as starts do not ascend: the jobs' bounds would not hold.
     if (!who || __builtin_amdgcn_readlane(wave_scan(all_rows), 63) > p.rows) return j;
     const int src = __ffsll((unsigned long long)who) - 1;
-    int b = b0, parts = 1;
-    Request r = none;
-    if (lane == src)
-        for (; b < b1; ++b) {
-            r = b == b0 ? first : request(p, b);
-            const Tiling t = tiling(p, r);
-            int x, y, z;
-            cut(t, &parts, &x, &y, &z);
-            if (t.many == want_many) {
-                if (left < x) break;
-                left -= x;
+    int ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows, at = -1, parts = 1, place = 0;
+    Request r = {0, 0, 0};
+    each([&](int i, const Request& x) {
+        const Tiling t = tiling(p, x);
+        const Cut c = cut(t);
+        if (at < 0) {
+            if (t.many == want_many && left < c.jobs) {
+                at = i;
+                r = x;
+                parts = c.parts;
+                place = left;
+            } else {
+                left -= t.many == want_many ? c.jobs : 0;
+                ctr += c.ctrs;
+                slot += c.rows;
             }
-            ctr += y;
-            slot += z;
         }
-    left = __builtin_amdgcn_readlane(left, src);
-    j.b = __builtin_amdgcn_readlane(b, src);
+    });
+    j.b = __builtin_amdgcn_readlane(b0 + at, src);
     j.req.row = __builtin_amdgcn_readlane(r.row, src);
     j.req.n = __builtin_amdgcn_readlane(r.n, src);
     j.req.len = __builtin_amdgcn_readlane(r.len, src);
     j.parts = __builtin_amdgcn_readlane(parts, src);
+    place = __builtin_amdgcn_readlane(place, src);
     const Tiling t = tiling(p, j.req);
     // Heads change fastest, then ranges, then tiles, those that see more keys first.
-    j.h = left % p.kv_heads;
-    left /= p.kv_heads;
-    j.part = left % j.parts;
-    const int tile = t.tiles - 1 - left / j.parts;
-    j.tile = t.tile;
-    j.row0 = tile * t.tile;
-    const int at = tile * p.kv_heads + j.h;
-    j.ctr = __builtin_amdgcn_readlane(ctr, src) + at;
-    j.slot = __builtin_amdgcn_readlane(slot, src) + at * j.parts * t.tile;
+    const int over_heads = __builtin_amdgcn_readfirstlane(quotient(place, p.kv_heads, p.inv_kv));
+    j.h = place - over_heads * p.kv_heads;
+    const int over_parts = __builtin_amdgcn_readfirstlane(quotient(over_heads, j.parts, __builtin_amdgcn_rcpf((float)j.parts)));
+    j.part = over_heads - over_parts * j.parts;
+    const int tile = t.tiles - 1 - over_parts;
+    j.tile = 1 << t.shift;
+    j.row0 = tile << t.shift;
+    const int tile_head = tile * p.kv_heads + j.h;
+    j.ctr = __builtin_amdgcn_readlane(ctr, src) + tile_head;
+    j.slot = __builtin_amdgcn_readlane(slot, src) + (tile_head * j.parts << t.shift);
     return j;
 }
 
@@ -263,7 +329,7 @@ struct PagedRun {
 struct TileRow {
     int r, head, pos, lo;  // row of the request, query head, position and the first key of its window
     __device__ __forceinline__ TileRow(const PagedParams& p, const Job& j, int row) {
-        r = row / p.G;
+        r = quotient(row, p.G, p.inv_G);
         head = j.h * p.G + (row - r * p.G);
         pos = j.req.len - j.req.n + r;
         lo = p.window && pos >= p.window ? pos - p.window + 1 : 0;
@@ -299,53 +365,66 @@ struct Merged {
 // Joins all ranges of a tile with the whole workgroup: every four outputs of a row are
 // one thread's, or (few rows) several threads', each with every groups-th range,
 // which then meet in LDS in order: the result does not depend on which range finished
-// first.  kJoinLoads loads are in flight at a time, as each is a round trip beyond
-// this XCD's L2.
-constexpr int kJoinLoads = 8;
+// first.  A thread has loads of up to kJoinUnits of its outputs and kJoinParts ranges in
+// flight at a time, as each is a round trip beyond this XCD's L2.
+constexpr int kJoinUnits = 4, kJoinParts = 4;
 template <int D>
 __device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, unsigned char* lds) {
     const int left = j.req.n * p.G - j.row0;
     const int units = (left < j.tile ? left : j.tile) * (D / 4);
-    auto join = [&](int e, int from, int step) {
-        const int row = e / (D / 4), d = 4 * (e % (D / 4));
-        Merged y;
-        for (int s0 = from; s0 < j.parts; s0 += kJoinLoads * step) {
-            float2 ml[kJoinLoads];
-            f32x4 x[kJoinLoads];
+    // Outputs first, first + kPagedThreads, ... (of `units`), over ranges from, from + step, ...
+    auto join = [&](Merged (&y)[kJoinUnits], int first, int from, int step) {
+        for (int s0 = from; s0 < j.parts; s0 += kJoinParts * step) {
+            float2 ml[kJoinUnits][kJoinParts];
+            f32x4 x[kJoinUnits][kJoinParts];
 #pragma unroll
-            for (int s = 0; s < kJoinLoads; ++s) {
-                const int at = s0 + s * step;
-                const int64_t g = j.slot + (int64_t)(at < j.parts ? at : s0) * j.tile + row;
-                ml[s] = get_agent(p.ml + g);
-                x[s] = get_agent(p.part + g * D + d);
+            for (int u = 0; u < kJoinUnits; ++u) {
+                const int e = first + u * kPagedThreads;
+                if (u && e >= units) break;
+#pragma unroll
+                for (int s = 0; s < kJoinParts; ++s) {
+                    const int at = s0 + s * step;
+                    const int64_t g = j.slot + (int64_t)(at < j.parts ? at : s0) * j.tile + e / (D / 4);
+                    ml[u][s] = get_agent(p.ml + g);
+                    x[u][s] = get_agent(p.part + g * D + 4 * (e % (D / 4)));
+                }
             }
 #pragma unroll
-            for (int s = 0; s < kJoinLoads; ++s)
-                if (s0 + s * step < j.parts) y.add(p.c, ml[s].x, ml[s].y, x[s]);
+            for (int u = 0; u < kJoinUnits; ++u) {
+                if (u && first + u * kPagedThreads >= units) break;
+#pragma unroll
+                for (int s = 0; s < kJoinParts; ++s)
+                    if (s0 + s * step < j.parts) y[u].add(p.c, ml[u][s].x, ml[u][s].y, x[u][s]);
+            }
         }
-        return y;
+    };
+    auto finish = [&](const Merged& y, int e) {
+        finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
     };
     int groups = 1;
     while (2 * groups * units <= kPagedThreads && groups < 8) groups *= 2;
     if (groups > 1) {
         const int g = threadIdx.x / units, e = threadIdx.x - g * units;
-        Merged y;
-        if (g < groups) y = join(e, g, groups);
+        Merged y[kJoinUnits];
+        if (g < groups) join(y, e, g, groups);
         f32x4* lo = reinterpret_cast<f32x4*>(lds);
         float2* lml = reinterpret_cast<float2*>(lds + kPagedThreads * sizeof(f32x4));
         __syncthreads();
-        lo[threadIdx.x] = y.o;
-        lml[threadIdx.x] = make_float2(y.M, y.L);
+        lo[threadIdx.x] = y[0].o;
+        lml[threadIdx.x] = make_float2(y[0].M, y[0].L);
         __syncthreads();
         if (g == 0) {
-            for (int k = 1; k < groups; ++k) y.add(p.c, lml[e + k * units].x, lml[e + k * units].y, lo[e + k * units]);
-            finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+            for (int k = 1; k < groups; ++k) y[0].add(p.c, lml[e + k * units].x, lml[e + k * units].y, lo[e + k * units]);
+            finish(y[0], e);
         }
         return;
     }
-    for (int e = threadIdx.x; e < units; e += kPagedThreads) {
-        const Merged y = join(e, 0, 1);
-        finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+    for (int e = threadIdx.x; e < units; e += kJoinUnits * kPagedThreads) {
+        Merged y[kJoinUnits];
+        join(y, e, 0, 1);
+#pragma unroll
+        for (int u = 0; u < kJoinUnits; ++u)
+            if (e + u * kPagedThreads < units) finish(y[u], e + u * kPagedThreads);
     }
 }
 
@@ -372,7 +451,8 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
     const int rows = job.req.n * p.G, row0 = job.row0;
     const int pos0 = job.req.len - job.req.n;  // of the request's first row
     const int last_row = row0 + TR - 1 < rows ? row0 + TR - 1 : rows - 1;
-    const KeySpan<32> span(p, job.req.len, pos0 + row0 / p.G, pos0 + last_row / p.G);
+    auto position = [&](int row) { return pos0 + __builtin_amdgcn_readfirstlane(quotient(row, p.G, p.inv_G)); };
+    const KeySpan<32> span(p, job.req.len, position(row0), position(last_row));
     const PagedRun kr(p, p.k, job, span.end), vr(p, p.v, job, span.end);
     const int t1 = (int)((int64_t)span.steps * (job.part + 1) / job.parts);
     int t = (int)((int64_t)span.steps * job.part / job.parts) + wave;

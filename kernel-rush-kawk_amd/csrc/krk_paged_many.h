@@ -170,8 +170,9 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const ParkedJob&
     auto clamped = [&](int row) { return row < rows ? row : rows - 1; };
     // Positions of the first and last row of the tile and of this wave's rows.
     const int wave0 = early.row0 + 32 * wave;
-    const int wave_first = pos0 + clamped(wave0) / p.G, wave_last = pos0 + clamped(wave0 + 31) / p.G;
-    const int tile_first = pos0 + early.row0 / p.G, tile_last = pos0 + clamped(early.row0 + kTileRows - 1) / p.G;
+    auto position = [&](int row) { return pos0 + __builtin_amdgcn_readfirstlane(quotient(clamped(row), p.G, p.inv_G)); };
+    const int wave_first = position(wave0), wave_last = position(wave0 + 31);
+    const int tile_first = position(early.row0), tile_last = position(early.row0 + kTileRows - 1);
     const KeySpan<kTileStep> span(p, early.req.len, tile_first, tile_last);
     const int t0 = (int)((int64_t)span.steps * early.part / early.parts), t1 = (int)((int64_t)span.steps * (early.part + 1) / early.parts);
     const int my_row = wave0 + n32;
