@@ -18,7 +18,10 @@ projection calls of one decode step, on libkrk_gemm.so.
   down, then the normed lm_head; 4 · layers + 1 calls, 145 for Qwen3-4B.
   With a :class:`kernels.cache.DecodeCache` it runs the whole layer: q/k
   norm, rotary embedding, cache write and attention between qkv and o.
-  Without one the o projection reads a caller-filled ``attn_out`` buffer and
+  With a :class:`kernels.serve.PagedCache` it does so for requests of different
+  lengths, and with a :class:`kernels.serve.AdapterSet` each row's own adapter
+  stands behind the projections.
+  Without a cache the o projection reads a caller-filled ``attn_out`` buffer and
   the qkv output is not consumed.  The residual stream uses the reference's two
   buffers (qkv reads ``cur`` and writes ``xa``, gate/up reads ``xa`` and
   writes ``xb``, lm reads ``xb`` and writes ``xa``), and :meth:`capture`
@@ -39,6 +42,7 @@ from types import SimpleNamespace
 import torch
 
 from . import gemm as G
+from .serve import PagedCache
 
 
 def decode_matmuls(m, M: int, log=None, tune: bool = True, select_k: int | None = None) -> dict:
@@ -92,12 +96,23 @@ class GemmStep:
     adds the attention of the R rows of each sequence, sequence after sequence
     in x; each run or replay moves the cache on by R rows.  ``tree`` (int64
     ``[B, R]`` on the GPU, read at every run and replay) makes them a draft
-    tree's nodes; ``cache.accept`` then keeps the accepted path."""
+    tree's nodes; ``cache.accept`` then keeps the accepted path.
+
+    A :class:`kernels.serve.PagedCache` of steps of M rows takes the rows that its
+    ``schedule`` named, request after request, before each run or replay; what the
+    rows behind them give is of no meaning.
+
+    ``adapters`` (a :class:`kernels.serve.AdapterSet`) adds the rows' adapters:
+    ``index`` (int32 ``[M]`` on the GPU, read at every run and replay) names them, -1 for
+    none; with a paged cache it is ``cache.tables.owner``, by the requests'
+    ``cache.labels``.  Projections with adapters behind the norm run it as its own
+    kernel, and gate and up round once, behind the product."""
 
     def __init__(self, m, M: int, mm: dict | None = None, log=None, tune: bool = False,
-                 select_k: int | None = None, cache=None, tree: torch.Tensor | None = None):
+                 select_k: int | None = None, cache=None, tree: torch.Tensor | None = None, adapters=None):
         self.m, self.M = m, M
-        if cache is not None and M % cache.B:
+        self.paged = isinstance(cache, PagedCache)
+        if cache is not None and not self.paged and M % cache.B:
             raise ValueError(f"M={M} rows for a cache of {cache.B} sequences")
         if tree is not None and cache is None:
             raise ValueError("tree masks need a cache")
@@ -105,8 +120,15 @@ class GemmStep:
             cfg = m.cfg
             if (cache.heads, cache.kv_heads, cache.head_dim, len(cache.k)) != (cfg.heads, cfg.kv_heads, cfg.head_dim, len(m.layers)):
                 raise ValueError("the cache was built for another model")
-            cache.check(M // cache.B, tree)
-        self.cache, self.tree = cache, tree
+            if not self.paged:
+                cache.check(M // cache.B, tree)
+            elif tree is not None:
+                raise ValueError("a paged cache takes no draft trees")
+            else:
+                cache.check(M)
+        if adapters is not None and adapters.m is not m:
+            raise ValueError("the adapters were built for another model")
+        self.cache, self.tree, self.adapters = cache, tree, adapters
         self.mm = mm if mm is not None else decode_matmuls(m, M, log, tune=tune, select_k=select_k)
         if select_k is not None and "lm_select" not in self.mm:
             raise ValueError("select_k needs an mm dict with an 'lm_select' entry")
@@ -117,6 +139,11 @@ class GemmStep:
         self.xb = torch.empty((M, cfg.hidden), dtype=bf16, device=dev)
         self.zero = torch.zeros((M, cfg.hidden), dtype=bf16, device=dev)
         self.attn_out = torch.zeros((M, cfg.heads * cfg.head_dim), dtype=bf16, device=dev)
+        if adapters is not None:
+            self.index = cache.tables.owner if self.paged else torch.full((M,), -1, dtype=torch.int32, device=dev)
+            self._adapt = {t: adapters.operator(t, M) for t in adapters.targets}
+            # In place of the normed calls: adapters read the normed rows too.
+            self._plain = {t: G.SkinnyMatmul(M, sum(adapters.widths[t]), cfg.hidden, dev) for t in ("qkv", "gu") if t in self._adapt}
         self.graph: torch.cuda.CUDAGraph | None = None
         self.out: torch.Tensor | None = None
 
@@ -131,6 +158,12 @@ class GemmStep:
         cache = self.cache
         if cache is None:
             return self._run(x)
+        if self.paged:
+            cache.planned()
+            cache.begin()
+            out = self._run(x)
+            cache.commit()
+            return out
         rows = self.M // cache.B
         cache.begin(rows, self.tree)
         try:
@@ -145,23 +178,45 @@ class GemmStep:
         xa, xb = self.xa, self.xb
         cur, y = x, self.zero
         for i, layer in enumerate(m.layers):
-            qkv = mm["qkv"](cur, y, layer.in_norm, xa, layer.wqkv)
+            qkv = self._normed("qkv", i, cur, y, layer.in_norm, xa, layer.wqkv)
             if cache is not None:
                 cache.attend(i, qkv, self.attn_out)
-            o = mm["o"](self.attn_out, layer.wo)
-            act = mm["gu"](xa, o, layer.post_norm, xb, layer.wgu)
-            y = mm["d"](act, layer.wd)
+            o = self._add("o", i, self.attn_out, mm["o"](self.attn_out, layer.wo))
+            act = self._normed("gu", i, xa, o, layer.post_norm, xb, layer.wgu)
+            y = self._add("d", i, act, mm["d"](act, layer.wd))
             cur = xb
         last = mm["lm_select"] if self.select else mm["lm"]
         return last(cur, y, m.final_norm, xa, m.lm_head)
+
+    def _adapted(self, target: str) -> bool:
+        return self.adapters is not None and target in self._adapt
+
+    def _add(self, target: str, i: int, x: torch.Tensor, y: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``y``, in place (or into ``out``), with layer ``i``'s adapters of ``target`` over ``x``."""
+        if not self._adapted(target):
+            return y
+        s = self.adapters
+        return self._adapt[target].run(x, s.a[target][i], s.b[target][i], self.index, y, y if out is None else out, scale=s.scale)
+
+    def _normed(self, target: str, i: int, x: torch.Tensor, y: torch.Tensor, norm: torch.Tensor, xout: torch.Tensor,
+                w: torch.Tensor) -> torch.Tensor:
+        """The projection behind a residual add and norm, with its adapters."""
+        if not self._adapted(target):
+            return self.mm[target](x, y, norm, xout, w)
+        n = G.add_rms_norm(x, y, norm, self.m.cfg.eps, xout)
+        z = self._plain[target](n, w)
+        return self._add(target, i, n, z, torch.empty((self.M, z.shape[1] // 2), dtype=z.dtype, device=z.device) if target == "gu" else None)
 
     def capture(self, x: torch.Tensor) -> torch.cuda.CUDAGraph:
         """Record run(x) in one graph (after warm-up calls on a side stream);
         replay() then recomputes self.out from the current contents of x and
         attn_out, or continues the cache by the rows of x.  A cache is left as
-        it was, but for slots behind its lengths."""
+        it was, but for slots behind its lengths (a paged one is captured without
+        rows; schedule() its step behind the capture)."""
         cache, state = self.cache, None
-        if cache is not None:
+        if self.paged:
+            cache.idle()
+        elif cache is not None:
             rows = self.M // cache.B
             cache.check(rows, self.tree)
             state = cache._state()
@@ -169,7 +224,9 @@ class GemmStep:
             cache._restore(state)
 
         def step():
-            if cache is not None:
+            if self.paged:
+                cache.begin()
+            elif cache is not None:
                 cache.begin(rows, self.tree, reserve=False)
             return self._run(x)
 
@@ -197,10 +254,14 @@ class GemmStep:
     def replay(self) -> torch.Tensor:
         if self.graph is None:
             raise RuntimeError("capture() first")
-        if self.cache is not None:
+        if self.paged:
+            self.cache.planned()
+        elif self.cache is not None:
             self.cache.reserve(self.M // self.cache.B)
             self.cache._rows = 0
         self.graph.replay()
+        if self.paged:
+            self.cache.commit()
         return self.out
 
 

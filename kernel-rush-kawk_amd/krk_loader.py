@@ -24,8 +24,8 @@ _PKG = Path(__file__).resolve().parent / "kernels"
 
 def load(name: str = "krk"):
     """The package imported under ``name`` (once per process), with its
-    submodules ``gemm``, ``attention``, ``cache``, ``step``, ``tune`` and
-    ``budget`` loaded."""
+    submodules ``gemm``, ``attention``, ``cache``, ``paged``, ``adapters``, ``serve``,
+    ``step``, ``tune`` and ``budget`` loaded."""
     if name in sys.modules:
         return sys.modules[name]
     spec = importlib.util.spec_from_file_location(name, _PKG / "__init__.py", submodule_search_locations=[str(_PKG)])
@@ -33,7 +33,7 @@ def load(name: str = "krk"):
     sys.modules[name] = mod
     try:
         spec.loader.exec_module(mod)
-        for sub in ("gemm", "attention", "cache", "step", "tune", "budget"):
+        for sub in ("gemm", "attention", "cache", "paged", "adapters", "serve", "step", "tune", "budget"):
             importlib.import_module(f"{name}.{sub}")
     except BaseException:
         for key in [k for k in sys.modules if k == name or k.startswith(name + ".")]:
