@@ -128,7 +128,7 @@ int check_shape(const krk_paged_shape& s) {
 struct Plan {
     bool many;  // some request may have more than kFewPairs rows of a head
     int64_t blocks;
-    size_t ctr, part, ml, bytes;  // workspace: sizes of its parts and their sum
+    size_t ctr, part, ml, plan, bytes;  // workspace: sizes of its parts and their sum
 };
 
 Plan make_plan(const krk_paged_shape& s) {
@@ -151,11 +151,12 @@ Plan make_plan(const krk_paged_shape& s) {
     p.blocks = tiles + few + many;
     if (few + many) {
         const size_t rows = (size_t)(few * 32 + many * krk::kManyRows);
-        p.ctr = align_up(krk::kCounters * sizeof(uint32_t), 256);
+        p.ctr = krk::kCounterBytes;
         p.part = rows * s.head_dim * sizeof(float);
         p.ml = rows * sizeof(float2);
     }
-    p.bytes = p.ctr + p.part + p.ml;
+    if (s.B > krk::kLaneRequests) p.plan = 256 + (size_t)cdiv(p.blocks, s.kv_heads) * sizeof(krk::PlannedRange);
+    p.bytes = p.ctr + p.part + p.ml + p.plan;
     return p;
 }
 
@@ -167,6 +168,11 @@ int launch_attn(const krk::PagedParams& p, const Plan& plan, hipStream_t stream)
     constexpr size_t shm = MANY && many > few ? many : few;
     if (hipError_t e = ensure_lds_limit(fn, shm, done)) return hip_status(e, "paged_attn_kernel LDS size");
     void* args[] = {(void*)&p};
+    if (p.planned) {
+        const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::paged_plan_kernel), dim3(1), dim3(krk::kPlanThreads), args,
+                                             krk::plan_lds_bytes(p.B), stream);
+        if (int rc = hip_status(e, "paged_plan_kernel launch")) return rc;
+    }
     return hip_status(hipLaunchKernel(fn, dim3((unsigned)plan.blocks), dim3(krk::kPagedThreads), args, shm, stream), "paged_attn_kernel launch");
 }
 
@@ -361,6 +367,10 @@ int krk_paged_attn_bf16(const krk_paged_shape* shape, const krk_paged_attn_args*
     p.ctr = reinterpret_cast<uint32_t*>(w);
     p.part = reinterpret_cast<float*>(w + plan.ctr);
     p.ml = reinterpret_cast<float2*>(w + plan.ctr + plan.part);
+    if (plan.plan) {
+        p.planned = reinterpret_cast<int*>(w + plan.ctr + plan.part + plan.ml);
+        p.plan = reinterpret_cast<krk::PlannedRange*>(w + plan.ctr + plan.part + plan.ml + 256);
+    }
     p.scale = a.scale;
     p.c = scale_log2;
     p.B = s.B;

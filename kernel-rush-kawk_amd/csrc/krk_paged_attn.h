@@ -6,10 +6,10 @@
 // query head h * G + j % G.
 //
 // Jobs.  A job is a tile of a request's rows of one head against one range of the
-// keys they see.  A call's lengths are on the device, so each workgroup works out from
-// them which job its number stands for: a lane takes one request in 64 of them (in
-// order), and scans over the wave find the request.  Every wave does so for itself: no
-// barrier, no launch in front, nothing kept from call to call.  Keys are cut by
+// keys they see.  A call's lengths are on the device, so each wave works out from them
+// which job its workgroup's number stands for, a lane a request: no barrier, no launch
+// in front, nothing kept from call to call (1.6 us; more than 64 requests are planned by
+// a launch in front).  Keys are cut by
 // length: into ranges that cost about what one of kTarget workgroups would take of
 // all of the call's work, so a long request beside short ones does not work on alone.
 // The workgroup that finishes the last range of a tile joins them, in order.
@@ -29,6 +29,7 @@ struct PageView {
     int64_t page, slot, head;
 };
 
+struct PlannedRange;
 struct PagedParams {
     const uint16_t* q;
     int64_t q_row;
@@ -39,7 +40,9 @@ struct PagedParams {
     uint16_t* out;
     int64_t out_row;
     float* lse;
-    uint32_t* ctr;  // [kCounters] finished ranges of a tile
+    int* planned;   // ranges that a launch in front listed: how many, and which (more than
+    PlannedRange* plan;  // kLaneRequests requests)
+    uint32_t* ctr;  // finished ranges of a tile
     float* part;    // [..][D] unnormalised outputs of ranges' rows
     float2* ml;     // [..] their running maximum (of q.k) and sum
     float scale;    // of q.k
@@ -67,9 +70,12 @@ constexpr float kFewCost = 5.0f, kManyCost = 2.0f;
 constexpr int kRounds = 4;
 constexpr float kGrain = 25.0f;
 // Tiles of more than one range have less than twice as many ranges as there are of the
-// target's size.  A tile has two at least.
+// target's size.
 constexpr int kFewSplits = 2 * kRounds * kTarget + 64, kManySplits = 2 * kTarget + 64;
-constexpr int kCounters = (kFewSplits + kManySplits) / 2;
+// Counters of tiles, one for every 16 rows of results.  As many for every shape: they are
+// at the front of a workspace that shapes may share, and partial results behind them.
+constexpr size_t kCounterBytes = (size_t)(2 * kFewSplits + 8 * kManySplits) * sizeof(uint32_t);
+static_assert(kCounterBytes % 256 == 0, "what follows is aligned");
 
 // n / d by its reciprocal (off by one at most), then put right.
 __device__ __forceinline__ int quotient(int n, int d, float inv) {
@@ -124,148 +130,219 @@ __device__ __forceinline__ float wave_total(float v) {
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(row_sum(v))));
 }
 
+// How many steps a range has: all of a call's work over kTarget workgroups, and what
+// follows from the jobs that this gives.
+struct Ranges {
+    int few, many;
+    float inv_few, inv_many;
+    // share: of a workgroup, in us.
+    __device__ __forceinline__ explicit Ranges(float share) {
+        few = at_least(share * (1.0f / kFewCost), kFewLeast);
+        many = at_least(share * (1.0f / kManyCost), kManyLeast);
+        inv_few = __builtin_amdgcn_rcpf((float)few);
+        inv_many = __builtin_amdgcn_rcpf((float)many);
+    }
+    // A few jobs too many would run by themselves behind the others: either ranges that
+    // long that all run at once, or, where they are long, short ones.
+    __device__ __forceinline__ void cut_anew(float share, int jobs) {
+        float rounds = floorf(share * (1.0f / kGrain));
+        rounds = rounds > (float)kRounds ? (float)kRounds : rounds;
+        few = rounds >= 2.0f ? at_least(share / (kFewCost * rounds), kFewLeast) : at_least((float)few * (float)jobs * (1.0f / kTarget), kFewLeast);
+        inv_few = __builtin_amdgcn_rcpf((float)few);
+    }
+    static __device__ __forceinline__ int at_least(float steps, int least) { return (int)steps + 1 > least ? (int)steps + 1 : least; }
+    __device__ __forceinline__ int parts(const Tiling& t) const {
+        return t.steps > (t.many ? many : few) ? (int)((float)(t.steps - 1) * (t.many ? inv_many : inv_few)) + 1 : 1;
+    }
+};
+__device__ __forceinline__ float cost_of(const Tiling& t) { return (float)(t.tiles * t.steps) * (t.many ? kManyCost : kFewCost); }
+
+// The nth of `many` jobs of many rows and `few` of few, by its number in the call: blocks
+// of 1 << block of the one, which keep the matrix pipe busy, and of the other, which read,
+// in turn, so that a CU has one of each; then what is left of the many and of the few.
+struct Nth {
+    bool many;
+    int n;
+    __device__ __forceinline__ Nth(int id, int all_many, int all_few, int block) {
+        const int both = (all_many < all_few ? all_many : all_few) >> block;
+        many = !(id >> block & 1);
+        n = (id >> (block + 1) << block) + (id & ((1 << block) - 1));
+        if (id >= both << (block + 1)) {
+            n = id - (both << block);
+            many = n < all_many;
+            n = many ? n : id - all_many;
+        }
+    }
+};
+
 // A tile of a request's rows of one key/value head, against one range of its keys.
 struct Job {
     int b, h, tile;     // tile: rows of a tile; < 0: no job
     int row0;           // first row of the tile, of the head's row list
     int part, parts;    // range, of how many
-    int slot, ctr;      // of parts > 1: row of the tile's first range's results; its counter
+    int slot;           // of parts > 1: row of the tile's first range's results
     Request req;
+    // The tile's counter: it has 32 rows of results at least.
+    __device__ __forceinline__ int counter() const { return slot >> 4; }
+    // place: of a request's jobs.  Heads change fastest, then ranges, then tiles, those
+    // that see more keys first.
+    __device__ __forceinline__ void at(const PagedParams& p, const Tiling& t, int place, int slot0) {
+        const int over_heads = __builtin_amdgcn_readfirstlane(quotient(place, p.kv_heads, p.inv_kv));
+        h = place - over_heads * p.kv_heads;
+        const int over_parts = __builtin_amdgcn_readfirstlane(quotient(over_heads, parts, __builtin_amdgcn_rcpf((float)parts)));
+        part = over_heads - over_parts * parts;
+        const int nth = t.tiles - 1 - over_parts;
+        tile = 1 << t.shift;
+        row0 = nth << t.shift;
+        slot = slot0 + ((nth * p.kv_heads + h) * parts << t.shift);
+    }
 };
 
-// Requests of a lane that stay in registers (of calls of up to 256).
-constexpr int kHeld = 4;
-
+// Calls of up to 64 requests: each wave works its job out from the lengths, a lane a
+// request.
+constexpr int kLaneRequests = 64;
 __device__ __forceinline__ Job job_of(const PagedParams& p, int id) {
     const int lane = threadIdx.x & 63;
-    const int per = (p.B + 63) / 64;
-    const int b0 = lane * per;
-    int n = p.B - b0;
-    n = n < 0 ? 0 : n < per ? n : per;
-    Request held[kHeld];
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        held[i] = Request{0, 0, 0};
-        if (i < per) {  // the same for all lanes
-            held[i] = request(p, i < n ? b0 + i : p.B - 1);
-            if (i >= n) held[i].n = 0;
-        }
-    }
-    // f(i, request) of this lane's requests in order, those of no rows too.
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i)
-            if (i < per) f(i, held[i]);
-        for (int i = kHeld; i < n; ++i) f(i, request(p, b0 + i));
-    };
-    float cost = 0.0f;
-    int all_rows = 0;
-    each([&](int, const Request& r) {
-        const Tiling t = tiling(p, r);
-        all_rows += r.n;
-        cost += (float)(t.tiles * t.steps) * (t.many ? kManyCost : kFewCost);
-    });
-    const float share = wave_total(cost) * (float)p.kv_heads * (1.0f / kTarget);  // of a workgroup
-    // Steps of a range.
-    auto at_least = [](float steps, int least) { return (int)steps + 1 > least ? (int)steps + 1 : least; };
-    int few = at_least(share * (1.0f / kFewCost), kFewLeast);
-    const int many = at_least(share * (1.0f / kManyCost), kManyLeast);
-    float inv_few = __builtin_amdgcn_rcpf((float)few);
-    const float inv_many = __builtin_amdgcn_rcpf((float)many);
-    // Ranges, jobs, tiles of several ranges and rows of their results.
-    struct Cut {
-        int parts, jobs, ctrs, rows;
-    };
-    auto cut = [&](const Tiling& t) {
-        Cut c;
-        c.parts = t.steps > (t.many ? many : few) ? (int)((float)(t.steps - 1) * (t.many ? inv_many : inv_few)) + 1 : 1;
-        const int tiles = t.tiles * p.kv_heads;
-        c.ctrs = c.parts > 1 ? tiles : 0;
-        c.jobs = tiles * c.parts;
-        c.rows = c.parts > 1 ? c.jobs << t.shift : 0;
-        return c;
-    };
-    int jobs_many, jobs_few, ctrs, rows, upto_many, upto_few, all_many, all_few;
+    Request r = request(p, lane < p.B ? lane : p.B - 1);
+    if (lane >= p.B) r.n = 0;
+    const Tiling t = tiling(p, r);
+    const float share = wave_total(cost_of(t)) * (float)p.kv_heads * (1.0f / kTarget);
+    Ranges ranges(share);
+    int parts, jobs, upto_many, upto_few, all_many, all_few;
     auto count = [&]() {
-        jobs_many = jobs_few = ctrs = rows = 0;
-        each([&](int, const Request& r) {
-            const Tiling t = tiling(p, r);
-            const Cut c = cut(t);
-            jobs_many += t.many ? c.jobs : 0;
-            jobs_few += t.many ? 0 : c.jobs;
-            ctrs += c.ctrs;
-            rows += c.rows;
-        });
-        upto_many = wave_scan(jobs_many);
-        upto_few = wave_scan(jobs_few);
+        parts = ranges.parts(t);
+        jobs = t.tiles * p.kv_heads * parts;
+        upto_many = wave_scan(t.many ? jobs : 0);
+        upto_few = wave_scan(t.many ? 0 : jobs);
         all_many = __builtin_amdgcn_readlane(upto_many, 63);
         all_few = __builtin_amdgcn_readlane(upto_few, 63);
     };
     count();
     if (all_many + all_few > kTarget && all_few) {
-        // A few jobs too many would run by themselves behind the others: either ranges
-        // that long that all run at once, or, where they are long, short ones.
-        float rounds = floorf(share * (1.0f / kGrain));
-        rounds = rounds > (float)kRounds ? (float)kRounds : rounds;
-        few = rounds >= 2.0f ? at_least(share / (kFewCost * rounds), kFewLeast)
-                             : at_least((float)few * (float)(all_many + all_few) * (1.0f / kTarget), kFewLeast);
-        inv_few = __builtin_amdgcn_rcpf((float)few);
+        ranges.cut_anew(share, all_many + all_few);
         count();
     }
-    // Which kind, and which of its jobs: 256 of many rows, which keep the matrix pipe
-    // busy, and 256 of few, which read, in turn, so that a CU has one of each; then what
-    // is left of the many and of the few.
-    const int both = (all_many < all_few ? all_many : all_few) >> 8;
-    bool want_many = !(id >> 8 & 1);
-    int nth = (id >> 9 << 8) + (id & 255);
-    if (id >= both << 9) {
-        nth = id - (both << 8);
-        want_many = nth < all_many;
-        nth = want_many ? nth : id - all_many;
-    }
-    int left = nth - (want_many ? upto_many - jobs_many : upto_few - jobs_few);
-    const uint64_t who = __ballot(left >= 0 && left < (want_many ? jobs_many : jobs_few));
+    const Nth nth(id, all_many, all_few, 8);
+    const int left = nth.n - (t.many ? upto_many : upto_few) + jobs;
+    const uint64_t who = __ballot(t.many == nth.many && left >= 0 && left < jobs);
     Job j;
     j.tile = -1;
     // More rows than the call has, as starts do not ascend: the jobs' bounds would not hold.
-    if (!who || __builtin_amdgcn_readlane(wave_scan(all_rows), 63) > p.rows) return j;
+    if (!who || __builtin_amdgcn_readlane(wave_scan(r.n), 63) > p.rows) return j;
     const int src = __ffsll((unsigned long long)who) - 1;
-    int ctr = wave_scan(ctrs) - ctrs, slot = wave_scan(rows) - rows, at = -1, parts = 1, place = 0;
-    Request r = {0, 0, 0};
-    each([&](int i, const Request& x) {
-        const Tiling t = tiling(p, x);
-        const Cut c = cut(t);
-        if (at < 0) {
-            if (t.many == want_many && left < c.jobs) {
-                at = i;
-                r = x;
-                parts = c.parts;
-                place = left;
-            } else {
-                left -= t.many == want_many ? c.jobs : 0;
-                ctr += c.ctrs;
-                slot += c.rows;
-            }
-        }
-    });
-    j.b = __builtin_amdgcn_readlane(b0 + at, src);
+    const int rows = parts > 1 ? jobs << t.shift : 0;
+    const int slot0 = wave_scan(rows) - rows;
+    j.b = src;
     j.req.row = __builtin_amdgcn_readlane(r.row, src);
     j.req.n = __builtin_amdgcn_readlane(r.n, src);
     j.req.len = __builtin_amdgcn_readlane(r.len, src);
     j.parts = __builtin_amdgcn_readlane(parts, src);
-    place = __builtin_amdgcn_readlane(place, src);
-    const Tiling t = tiling(p, j.req);
-    // Heads change fastest, then ranges, then tiles, those that see more keys first.
-    const int over_heads = __builtin_amdgcn_readfirstlane(quotient(place, p.kv_heads, p.inv_kv));
-    j.h = place - over_heads * p.kv_heads;
-    const int over_parts = __builtin_amdgcn_readfirstlane(quotient(over_heads, j.parts, __builtin_amdgcn_rcpf((float)j.parts)));
-    j.part = over_heads - over_parts * j.parts;
-    const int tile = t.tiles - 1 - over_parts;
-    j.tile = 1 << t.shift;
-    j.row0 = tile << t.shift;
-    const int tile_head = tile * p.kv_heads + j.h;
-    j.ctr = __builtin_amdgcn_readlane(ctr, src) + tile_head;
-    j.slot = __builtin_amdgcn_readlane(slot, src) + (tile_head * j.parts << t.shift);
+    j.at(p, tiling(p, j.req), __builtin_amdgcn_readlane(left, src), __builtin_amdgcn_readlane(slot0, src));
+    return j;
+}
+
+// More requests: a launch in front, of one workgroup, lists the tiles' ranges in the order
+// of the jobs; a job is a head of one of them.  (Each wave for itself, with four requests
+// a lane: 4.0 us a job instead of 1.6 at 256 requests.)
+struct PlannedRange {
+    int b, row0, parts_part, slot;  // parts << 16 | part; row of results of the tile's ranges of head 0
+};
+constexpr int kPlanThreads = 1024;
+__host__ __device__ constexpr size_t plan_lds_bytes(int B) { return (size_t)(3 * B + 2) * sizeof(int); }
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedParams p) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ int scratch[kPageWaves];
+    __shared__ float costs[kPageWaves];
+    int* first_many = reinterpret_cast<int*>(lds);  // [B + 1] ranges of earlier requests, by kind
+    int* first_few = first_many + p.B + 1;
+    int* first_row = first_few + p.B + 1;           // [B] rows of results of earlier requests
+    const int per = (p.B + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = (int)threadIdx.x * per, b1 = b0 + per < p.B ? b0 + per : p.B;
+    float cost = 0.0f;
+    int all_rows = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Request r = request(p, b);
+        all_rows += r.n;
+        cost += cost_of(tiling(p, r));
+    }
+    cost = wave_total(cost);
+    if ((threadIdx.x & 63) == 0) costs[threadIdx.x >> 6] = cost;
+    int total;
+    block_scan(all_rows, scratch, &total);
+    float share = 0.0f;
+    for (int w = 0; w < kPageWaves; ++w) share += costs[w];
+    share *= (float)p.kv_heads * (1.0f / kTarget);
+    Ranges ranges(share);
+    int many, few, rows, all_many, all_few;
+    auto count = [&]() {
+        many = few = rows = 0;
+        for (int b = b0; b < b1; ++b) {
+            const Tiling t = tiling(p, request(p, b));
+            const int parts = ranges.parts(t), n = t.tiles * parts;
+            many += t.many ? n : 0;
+            few += t.many ? 0 : n;
+            rows += parts > 1 ? n * p.kv_heads << t.shift : 0;
+        }
+        many = block_scan(many, scratch, &all_many);
+        few = block_scan(few, scratch, &all_few);
+    };
+    count();
+    if ((all_many + all_few) * p.kv_heads > kTarget && all_few) {
+        ranges.cut_anew(share, (all_many + all_few) * p.kv_heads);
+        count();
+    }
+    int unused;
+    rows = block_scan(rows, scratch, &unused);
+    for (int b = b0; b < b1; ++b) {
+        const Tiling t = tiling(p, request(p, b));
+        const int parts = ranges.parts(t), n = t.tiles * parts;
+        first_many[b] = many;
+        first_few[b] = few;
+        first_row[b] = rows;
+        many += t.many ? n : 0;
+        few += t.many ? 0 : n;
+        rows += parts > 1 ? n * p.kv_heads << t.shift : 0;
+    }
+    __syncthreads();
+    // More rows than the call has, as starts do not ascend: no job.
+    const int n = total > p.rows ? 0 : all_many + all_few;
+    if (threadIdx.x == 0) *p.planned = n;
+    int block = 8;  // blocks of 256 jobs
+    while (block > 0 && (p.kv_heads << block) > 256) --block;
+    for (int e = threadIdx.x; e < n; e += kPlanThreads) {
+        const Nth nth(e, all_many, all_few, block);
+        const int* first = nth.many ? first_many : first_few;
+        const int b = owner_of(first, p.B, nth.n);
+        const Tiling t = tiling(p, request(p, b));
+        const int parts = ranges.parts(t), place = nth.n - first[b];
+        const int tile = quotient(place, parts, __builtin_amdgcn_rcpf((float)parts)), part = place - tile * parts;
+        PlannedRange x;
+        x.b = b;
+        x.row0 = (t.tiles - 1 - tile) << t.shift;
+        x.parts_part = parts << 16 | part;
+        x.slot = first_row[b] + ((t.tiles - 1 - tile) * p.kv_heads * parts << t.shift);
+        p.plan[e] = x;
+    }
+}
+
+__device__ __forceinline__ Job planned_job(const PagedParams& p, int id) {
+    Job j;
+    j.tile = -1;
+    const int e = __builtin_amdgcn_readfirstlane(quotient(id, p.kv_heads, p.inv_kv));
+    if (e >= *p.planned) return j;
+    const PlannedRange x = p.plan[e];
+    j.b = __builtin_amdgcn_readfirstlane(x.b);
+    j.row0 = __builtin_amdgcn_readfirstlane(x.row0);
+    const int pp = __builtin_amdgcn_readfirstlane(x.parts_part);
+    j.parts = pp >> 16;
+    j.part = pp & 0xffff;
+    const Request r = request(p, j.b);
+    j.req = {__builtin_amdgcn_readfirstlane(r.row), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.len)};
+    j.h = id - e * p.kv_heads;
+    const int shift = tiling(p, j.req).shift;
+    j.tile = 1 << shift;
+    j.slot = __builtin_amdgcn_readfirstlane(x.slot) + (j.h * j.parts << shift);
     return j;
 }
 
@@ -661,9 +738,9 @@ __device__ __forceinline__ bool last_range(const PagedParams& p, const Job& job,
     drain_memory();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(p.ctr + job.ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(p.ctr + job.counter(), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *last = before == (uint32_t)job.parts - 1;
-        if (*last) __hip_atomic_store(p.ctr + job.ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (*last) __hip_atomic_store(p.ctr + job.counter(), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     const bool yes = *last;

@@ -136,13 +136,13 @@ struct PageStream {
 struct ParkedJob {
     int v = 0;
     __device__ __forceinline__ explicit ParkedJob(const Job& j) {
-        put(0, j.b), put(1, j.h), put(2, j.tile), put(3, j.row0), put(4, j.part), put(5, j.parts), put(6, j.slot), put(7, j.ctr);
-        put(8, j.req.row), put(9, j.req.n), put(10, j.req.len);
+        put(0, j.b), put(1, j.h), put(2, j.tile), put(3, j.row0), put(4, j.part), put(5, j.parts), put(6, j.slot);
+        put(7, j.req.row), put(8, j.req.n), put(9, j.req.len);
     }
     __device__ __forceinline__ Job job() const {
         Job j;
-        j.b = get(0), j.h = get(1), j.tile = get(2), j.row0 = get(3), j.part = get(4), j.parts = get(5), j.slot = get(6), j.ctr = get(7);
-        j.req = {get(8), get(9), get(10)};
+        j.b = get(0), j.h = get(1), j.tile = get(2), j.row0 = get(3), j.part = get(4), j.parts = get(5), j.slot = get(6);
+        j.req = {get(7), get(8), get(9)};
         return j;
     }
     __device__ __forceinline__ void put(unsigned i, int x) { v = (threadIdx.x & 63) == i ? x : v; }
@@ -471,7 +471,7 @@ __device__ __forceinline__ void many_rows(const PagedParams& p, const ParkedJob&
 template <int D, bool MANY>
 __global__ void __launch_bounds__(kPagedThreads, 2) paged_attn_kernel(PagedParams p) {
     extern __shared__ __align__(16) unsigned char lds[];
-    const Job first = job_of(p, (int)blockIdx.x);
+    const Job first = p.planned ? planned_job(p, (int)blockIdx.x) : job_of(p, (int)blockIdx.x);
     if (first.tile < 0) return;
     const ParkedJob parked(first);
     // Each kind of job with arguments of its own: what they have in common would else

@@ -284,3 +284,51 @@ def test_python_calls_need_the_gpu():
     ad = kernels.LowRankAdapters(9, 256, 1024, 16, "cpu")
     with pytest.raises(ValueError, match="GPU tensor"):
         ad(q, torch.zeros((2, 16, 1024), dtype=BF), torch.zeros((2, 256, 16), dtype=BF), i, torch.zeros((9, 256), dtype=BF))
+
+
+# ------------------------------------------------- a model's cache, its host side
+@pytest.fixture(scope="module")
+def model():
+    from kernels import step
+
+    return step.synthetic_model("cpu", layers=1, hidden=64, intermediate=64, heads=2, kv_heads=1, head_dim=64, vocab=64)
+
+
+def test_schedules(model):
+    c = kernels.PagedCache(model, 3, 30, 8, 8, width=5)
+    with pytest.raises(RuntimeError, match="schedule"):
+        c.planned()
+    assert c.schedule([17, 0, 9]) == [0, 17, 17]
+    c.planned()
+    assert c.new.tolist() == [17, 0, 9] and c.keep.tolist() == [0, 0, 0] and c.lens == [0, 0, 0]
+    c.commit()
+    assert c.lens == [17, 0, 9]
+    for new, msg in (([1, 0], "each of 3"), ([1, -1, 0], "each of 3"), ([10, 10, 11], "31 rows"), ([24, 0, 0], "pass its 5 pages"),
+                     ([8, 14, 8], "9 of 8 pages")):
+        with pytest.raises(ValueError, match=msg):
+            c.schedule(new)
+        assert c.lens == [17, 0, 9] and c.new.tolist() == [17, 0, 9]
+    c.rollback([2, 0, 9])
+    with pytest.raises(RuntimeError, match="schedule"):
+        c.planned()
+    with pytest.raises(ValueError, match="rollback"):
+        c.rollback([16, 0, 0])
+    c.schedule([1, 24, 0])  # 2 + 3 pages
+    assert c.keep.tolist() == [15, 0, 0]
+    c.commit()
+    c.reset(1)
+    assert c.lens == [16, 0, 0]
+    c.reset()
+    assert c.lens == [0, 0, 0]
+    c.check(30)
+    with pytest.raises(ValueError, match="M=29"):
+        c.check(29)
+
+
+def test_adapter_sets(model):
+    s = kernels.AdapterSet(model, 2, 8)
+    assert [tuple(s.a[t][0].shape) for t in s.targets] == [(2, 24, 64), (2, 8, 128), (2, 16, 64), (2, 8, 64)]
+    assert [tuple(s.b[t][0].shape) for t in s.targets] == [(2, 256, 8), (2, 64, 8), (2, 128, 8), (2, 64, 8)]
+    for kw in (dict(targets=()), dict(targets=("lm",)), dict(targets=("o", "o")), dict(rank=9), dict(adapters=0)):
+        with pytest.raises(ValueError):
+            kernels.AdapterSet(model, **{**dict(adapters=1, rank=8), **kw})

@@ -272,6 +272,24 @@ def test_steps(device, case, layout):
     check_step(device, 500 + case, *STEPS[case], layout=layout)
 
 
+#: More requests than a wave has lanes: planned by a launch in front.
+CROWDS = [
+    ([1] * 65, [(53 * i) % 97 + 1 for i in range(65)], 8, 2, 128, 16),
+    ([(0, 1, 1, 7, 1)[i % 5] for i in range(300)], [(37 * i) % 150 + 7 for i in range(300)], 4, 1, 128, 8),
+    ([130 if i == 40 else 40 if i == 41 else i % 2 for i in range(120)], [900 if i in (40, 99) else (29 * i) % 300 + 41 for i in range(120)],
+     8, 2, 64, 32),
+    ([1] * 1030, [i % 40 + 1 for i in range(1030)], 2, 2, 64, 8),
+    ([300 if i == 3 else 1 for i in range(70)], [2500 if i == 3 else 1500 if i == 60 else 30 + i for i in range(70)], 32, 8, 128, 16),
+    ([0] * 80, [5] * 80, 8, 2, 128, 16),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CROWDS)))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 2)])
+def test_many_requests(device, case, window, sinks):
+    check_step(device, 550 + case, *CROWDS[case], window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (32, 0), (33, 40), (100, 4), (5000, 9)])
 @pytest.mark.parametrize("P", [8, 64])
 def test_window_and_sinks(device, window, sinks, P):
@@ -314,16 +332,22 @@ def test_page_numbers_outside_the_pool_read_another_page(device):
 
 
 @pytest.mark.parametrize("starts", [[0, 5, 2, 9], [-4, 3, 700, 2], [9, 9, 9, 9], [3, 1, 0, -8]])
-def test_starts_that_do_not_ascend(device, starts):
-    """In bounds, whatever they hold; rows behind the call's are untouched."""
+@pytest.mark.parametrize("more", [0, 80])
+def test_starts_that_do_not_ascend(device, starts, more):
+    """In bounds, whatever they hold; rows behind the call's are untouched, and the
+    workspace serves the next call."""
     g = gen(6)
     k, v = rnd(g, 20, 8, 2, 128).to(device), rnd(g, 20, 8, 2, 128).to(device)
     big = torch.full((30, 1024), 3.0, dtype=BF, device=device)
-    table = torch.randint(0, 20, (3, 6), generator=g).to(I32).to(device)
-    op = K.PagedAttention(3, 9, 8, 2, 128, 8, 6, device)
-    op.run(rnd(g, 9, 1024).to(device), k, v, table, i32(device, starts), i32(device, [48, 20, 33]), big[10:19])
+    table = torch.randint(0, 20, (3 + more, 6), generator=g).to(I32).to(device)
+    op = K.PagedAttention(3 + more, 9, 8, 2, 128, 8, 6, device)
+    q, keys = rnd(g, 9, 1024).to(device), i32(device, [48, 20, 33] + [30] * more)
+    op.run(q, k, v, table, i32(device, starts + [9, 0] * (more // 2)), keys, big[10:19])
     torch.cuda.synchronize()
     assert torch.all(big[:10] == 3.0) and torch.all(big[19:] == 3.0) and big[10:19].isfinite().all()
+    good = i32(device, [0, 3, 5, 9] + [9] * more)
+    other = K.PagedAttention(3 + more, 9, 8, 2, 128, 8, 6, device)
+    assert torch.equal(op(q, k, v, table, good, keys), other(q, k, v, table, good, keys))
 
 
 def test_pool_offsets_beyond_32_bits(device):
@@ -402,6 +426,20 @@ def test_objects_on_two_streams_and_a_shared_workspace(device):
     if need:
         with pytest.raises(ValueError, match="workspace"):
             K.PagedAttention(3, op.rows, 8, 2, 128, 16, op.width, device, workspace=ws[:need - 1])
+
+
+def test_shapes_that_share_a_workspace(device):
+    """Of other sizes, head sizes and planning, one after the other in one workspace."""
+    made = [check_step(device, 720 + i, *c) for i, c in enumerate([
+        ([1, 1], [3000, 900], 8, 2, 128, 16), ([200, 1, 1], [3000, 2000, 64], 8, 2, 64, 8), ([1] * 70, [700] * 70, 4, 1, 128, 16),
+        ([30], [5000], 8, 8, 128, 64)])]
+    need = max(K.paged_workspace_bytes(o.B, o.rows, o.heads, o.kv_heads, o.head_dim, o.page_size, o.width) for o, _, _ in made)
+    ws = torch.zeros(need, dtype=torch.uint8, device=device)
+    shared = [K.PagedAttention(o.B, o.rows, o.heads, o.kv_heads, o.head_dim, o.page_size, o.width, device, workspace=ws) for o, _, _ in made]
+    for i in (0, 1, 2, 3, 2, 0, 3, 1, 0, 2):
+        _, args, out = made[i]
+        n = int(args[4][-1])
+        assert torch.equal(shared[i](*args)[:n], out[:n]), i
 
 
 def test_python_refusals(device):
