@@ -18,6 +18,8 @@
 // those of the contiguous caches' kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "krk_attn_common.h"
 #include "krk_epilogue.h"
 #include "krk_page_step.h"
@@ -590,10 +592,18 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
     // it: the products run on zeros in their place, and the rows that see them
     // get them behind the last step.
     bool any_odd = false;
-    for (; t < t1; t += kPagedWaves) {
+    // The last step without the loads for a next one, in code of its own: where loads may
+    // have been left out the compiler waits as if they had, for V before it takes the
+    // scores (8 drafts of 16 rows: 34.3 -> 32.5 us).
+    auto step = [&](int t, auto more) {
+        constexpr bool MORE = decltype(more)::value;
         const int kb = span.key(t);
         const int next = t + kPagedWaves;
-        const unsigned kp2 = k_page(next + kPagedWaves), vp2 = v_page(next + kPagedWaves);
+        unsigned kp2 = 0, vp2 = 0;
+        if constexpr (MORE) {
+            kp2 = k_page(next + kPagedWaves);
+            vp2 = v_page(next + kPagedWaves);
+        }
         f32x4 s[MT][2];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -603,7 +613,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) s[i][u] = mfma16(kf.f[u][ks], qf[i][ks], s[i][u]);
             }
-        if (next < t1) load_k(span.key(next), kp);
+        if constexpr (MORE) load_k(span.key(next), kp);
         // What each row does not see gets no weight.
         if (!span.whole(kb, p.sinks)) {
 #pragma unroll
@@ -655,10 +665,12 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
 #pragma unroll
             for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, low[i], acc[i][j]));
         }
-        if (next < t1) load_v(span.key(next), vp);
+        if constexpr (MORE) load_v(span.key(next), vp);
         kp = kp2;
         vp = vp2;
-    }
+    };
+    for (; t + kPagedWaves < t1; t += kPagedWaves) step(t, std::true_type{});
+    if (t < t1) step(t, std::false_type{});
     if (any_odd) {  // rare, so key by key
 #pragma unroll 1
         for (t = t_first; t < t1; t += kPagedWaves) {
