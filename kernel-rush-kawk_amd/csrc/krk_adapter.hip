@@ -54,7 +54,12 @@ Plan make_plan(const krk_adapter_shape& s) {
     const int tile = p.many ? 64 : 16, most_sets = tile < s.rows ? tile : s.rows;
     p.tiles = (int)cdiv(s.rows, tile);
     p.groups = (int)cdiv((int64_t)s.slices * s.rank, 16 * krk::kAdapterTiles);
-    const int64_t want = cdiv(2 * kCuCount, (int64_t)p.tiles * p.groups);
+    // Few rows: a range each for two workgroups a CU, or more.  Many rows: at most three
+    // workgroups for two CUs, since a tile of two requests has a second one that starts
+    // where room is left (4096 rows of 9728, a call: 56.5 us in 8 ranges or 7, 53.9 in 6;
+    // 1000 rows and narrower calls the same).
+    const int64_t blocks = (int64_t)p.tiles * p.groups, few = cdiv(2 * kCuCount, blocks), many = 3 * kCuCount / 2 / blocks;
+    const int64_t want = !p.many ? few : many > 0 ? many : 1;
     const int64_t most = p.many ? cdiv(s.K, 4 * krk::kAdapterManyStep) : cdiv(s.K, krk::kAdapterWaves * krk::kAdapterFewStep);
     p.splits = (int)(want < most ? want : most);
     p.splits = p.splits < krk::kAdapterSplits ? p.splits : krk::kAdapterSplits;
@@ -74,7 +79,8 @@ int launch_shrink(krk::AdapterParams p, const Plan& plan, hipStream_t st) {
     p.slots = plan.shrink_slots;
     void* kargs[] = {(void*)&p};
     const void* fn = plan.many ? reinterpret_cast<const void*>(&krk::adapter_shrink64_kernel) : reinterpret_cast<const void*>(&krk::adapter_shrink_kernel);
-    const hipError_t e = hipLaunchKernel(fn, dim3(plan.splits, plan.tiles * p.slots, plan.groups), dim3(krk::kAdapterThreads), kargs, 0, st);
+    const dim3 grid = plan.many ? dim3(plan.splits * plan.tiles, p.slots, plan.groups) : dim3(plan.splits, plan.tiles * p.slots, plan.groups);
+    const hipError_t e = hipLaunchKernel(fn, grid, dim3(krk::kAdapterThreads), kargs, 0, st);
     return hip_status(e, "adapter_shrink_kernel launch");
 }
 

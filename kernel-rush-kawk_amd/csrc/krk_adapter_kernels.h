@@ -50,19 +50,18 @@ struct AdapterParams {
 // adapters each of `slots` blocks takes every slots-th, so that rows of many adapters do
 // not wait for one another.  All tiles' first slots come first: workgroups go to the
 // shader engines in a fixed order, and with idle ones in every other place half of the
-// CUs stayed idle (4096 rows of 9728: 40 us, now 27).
+// CUs stayed idle (4096 rows of 9728: 40 us and 28).
 template <int MT>
 struct RowSets {
     static constexpr int TR = 16 * MT;
     int row0, id;     // id: of row0 + lane % TR, -1 for none
     int skip, slots;
     uint64_t todo;    // bit i: row0 + i
-    __device__ __forceinline__ RowSets(const AdapterParams& p, int block) {
+    __device__ __forceinline__ RowSets(const AdapterParams& p, int tile, int slot) {
         const int i = (threadIdx.x & 63) % TR;
-        const int tiles = (p.rows + TR - 1) / TR;
         slots = p.slots;
-        skip = block / tiles;
-        row0 = TR * (block - skip * tiles);
+        skip = slot;
+        row0 = TR * tile;
         const bool in = row0 + i < p.rows;
         id = p.index[in ? row0 + i : p.rows - 1];
         id = id >= 0 && id < p.adapters ? id : -1;
@@ -98,7 +97,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink_kernel(Adap
     const int n0 = 16 * kAdapterTiles * blockIdx.z;
     const int steps = (p.K + kAdapterFewStep - 1) / kAdapterFewStep;
     const int c0 = (int)((int64_t)steps * blockIdx.x / p.splits), c1 = (int)((int64_t)steps * (blockIdx.x + 1) / p.splits);
-    RowSets<1> sets(p, blockIdx.y);
+    const int tiles = (p.rows + 15) / 16;
+    RowSets<1> sets(p, blockIdx.y % tiles, blockIdx.y / tiles);
     const int row = sets.row0 + n16;
     const uint16_t* x = p.x + (int64_t)(row < p.rows ? row : p.rows - 1) * p.ldx + 8 * q4;
     const u32x4 zero = {0, 0, 0, 0};
@@ -161,9 +161,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink_kernel(Adap
 // in a ring of two steps; each wave takes 16 of the rows.  (Straight into operands a
 // load takes 64 bytes each of 16 rows: rows whose length is a multiple of 1 KB then
 // meet in a few sets of the L1, and 4096 rows of 9728 took 43 us.)  Chunks of 16 bytes
-// of a row are permuted with the row's low bits, against bank conflicts.  Ranges of K
-// change fastest: with 8 of them each XCD (workgroups go to them round robin) keeps to
-// its own part of every A.
+// of a row are permuted with the row's low bits, against bank conflicts.  The tiles of a
+// range of K lie side by side on one XCD or two, which keep to that part of every A.
 __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink64_kernel(AdapterParams p) {
     constexpr int ROWS = 64, CH = kAdapterManyStep / 8;  // chunks of a row and step
     constexpr int DMAS = ROWS / 4 / kAdapterWaves;       // of 4 rows, of x and of A, per wave and step
@@ -174,8 +173,10 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink64_kernel(Ad
     const int n16 = lane & 15, q4 = lane >> 4;
     const int n0 = 16 * kAdapterTiles * blockIdx.z;
     const int steps = (p.K + kAdapterManyStep - 1) / kAdapterManyStep;
-    const int c0 = (int)((int64_t)steps * blockIdx.x / p.splits), c1 = (int)((int64_t)steps * (blockIdx.x + 1) / p.splits);
-    RowSets<4> sets(p, blockIdx.y);
+    const int tiles = (p.rows + ROWS - 1) / ROWS;
+    const int block = xcd_block(blockIdx.x, tiles * p.splits), range = block / tiles;
+    const int c0 = (int)((int64_t)steps * range / p.splits), c1 = (int)((int64_t)steps * (range + 1) / p.splits);
+    RowSets<4> sets(p, block - range * tiles, blockIdx.y);
     int id;
     uint64_t rows;
     while (sets.next(&id, &rows)) {
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink64_kernel(Ad
 #pragma unroll
             for (int t = 0; t < kAdapterTiles; ++t) {
                 const int n = n0 + 16 * t + 4 * q4;
-                if (n < p.HN) *reinterpret_cast<f32x4*>(p.h + ((int64_t)blockIdx.x * p.rows + row) * p.HN + n) = acc[t];
+                if (n < p.HN) *reinterpret_cast<f32x4*>(p.h + ((int64_t)range * p.rows + row) * p.HN + n) = acc[t];
             }
         }
     }
@@ -305,7 +306,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_expand_kernel(Adap
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
-    RowSets<MT> sets(p, blockIdx.y);
+    const int tiles = (p.rows + TR - 1) / TR;
+    RowSets<MT> sets(p, blockIdx.y % tiles, blockIdx.y / tiles);
     int id;
     uint64_t rows;
     bool more = sets.next(&id, &rows);
