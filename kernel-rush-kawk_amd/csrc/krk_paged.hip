@@ -149,13 +149,11 @@ Plan make_plan(const krk_paged_shape& s) {
     const int64_t few = splits(krk::kFewStep * krk::kFewLeast, krk::kFewSplits);
     const int64_t many = p.many ? splits(krk::kManyStep * krk::kManyLeast, krk::kManySplits) : 0;
     p.blocks = tiles + few + many;
-    if (few + many) {
-        const size_t rows = (size_t)(few * 32 + many * krk::kManyRows);
-        p.ctr = krk::kCounterBytes;
-        p.part = rows * s.head_dim * sizeof(float);
-        p.ml = rows * sizeof(float2);
-    }
+    const size_t rows = (size_t)(few * 32 + many * krk::kManyRows);
+    p.part = rows * s.head_dim * sizeof(float);
+    p.ml = rows * sizeof(float2);
     if (s.B > krk::kLaneRequests) p.plan = 256 + (size_t)cdiv(p.blocks, s.kv_heads) * sizeof(krk::PlannedRange);
+    if (rows || p.plan) p.ctr = krk::kCounterBytes;  // also where this shape counts nothing: they stay zero
     p.bytes = p.ctr + p.part + p.ml + p.plan;
     return p;
 }

@@ -442,6 +442,20 @@ def test_shapes_that_share_a_workspace(device):
         assert torch.equal(shared[i](*args)[:n], out[:n]), i
 
 
+@pytest.mark.parametrize("B,P,width", [(70, 8, 16), (300, 64, 2), (70, 16, 1)])
+def test_a_workspace_shared_with_requests_of_one_range(device, B, P, width):
+    """Many requests of a few keys, which are listed in the workspace and never cut, leave the counters at its front zero."""
+    cut, args, out = check_step(device, 730, [1, 1], [3000, 900], 8, 2, 128, 16)
+    short, sargs, sout = check_step(device, 731, [1] * B, [width * P] * B, 8, 2, 128, P, width=width)
+    need = [K.paged_workspace_bytes(o.B, o.rows, o.heads, o.kv_heads, o.head_dim, o.page_size, o.width) for o in (cut, short)]
+    ws = torch.zeros(max(need), dtype=torch.uint8, device=device)
+    shared = [K.PagedAttention(o.B, o.rows, o.heads, o.kv_heads, o.head_dim, o.page_size, o.width, device, workspace=ws) for o in (cut, short)]
+    for i in range(3):
+        assert torch.equal(shared[1](*sargs)[:B], sout[:B]), i
+        assert int(ws[:256].sum()) == 0
+        assert torch.equal(shared[0](*args)[:2], out[:2]), i
+
+
 def test_python_refusals(device):
     op = K.PagedAttention(2, 4, 8, 2, 128, 16, 3, device)
     q = torch.zeros((4, 1024), dtype=BF, device=device)
