@@ -152,7 +152,9 @@ __global__ void __launch_bounds__(kPageThreads) page_step_kernel(PageStepParams 
         want += fits && managed ? ((cut + n + page - 1) >> p.shift) - held[b] : 0;
     }
     int take = block_scan(want, scratch, &all_wanted);
-    const int top = count + all_back < p.pages ? count + all_back : p.pages;
+    // Lengths that no step left may give back more pages than there are (B * width, so
+    // the sum with count could pass 2^31): those behind the stack's end are lost.
+    const int top = all_back < p.pages - count ? count + all_back : p.pages;
     row = first_row;
     for (int b = b0; b < b1; ++b) {
         int old;
@@ -174,10 +176,9 @@ __global__ void __launch_bounds__(kPageThreads) page_step_kernel(PageStepParams 
     }
     __syncthreads();
     if (managed) {
-        for (int i = threadIdx.x; i < all_back; i += kPageThreads) {
+        for (int i = threadIdx.x; i < top - count; i += kPageThreads) {
             const int b = owner_of(given, p.B, i);
-            const int spot = top - 1 - i;
-            if (spot >= count) p.free_pages[spot] = p.table[(int64_t)b * p.table_row + held[b] + i - given[b]];
+            p.free_pages[top - 1 - i] = p.table[(int64_t)b * p.table_row + held[b] + i - given[b]];
         }
         __syncthreads();
         // What the requests in order take, up to the first that no longer fits.

@@ -99,6 +99,16 @@ def test_states_that_no_step_leaves(device):
     assert op.lens.tolist() == [1, 16] and op.slots.tolist()[:2] == [0, -1] and int(op.count) == 3
 
 
+def test_lengths_of_more_pages_than_there_are(device):
+    """Pages given back that were never taken, with the count close to 2^31 together: the stack holds what it can."""
+    B, width = 4096, 500000
+    op = K.PageTables(B, 8, 1 << 27, 8, width, device)
+    op.lens.fill_(8 * width)
+    op.step(i32(device, [1] + [0] * (B - 1)), keep=torch.zeros(B, dtype=I32, device=device))
+    torch.cuda.synchronize()
+    assert int(op.count) == (1 << 27) - 1 and op.lens.tolist() == [1] + [0] * (B - 1) and op.slots.tolist() == [0] + [-1] * 7
+
+
 def test_step_captured_and_on_other_streams(device):
     B, rows = 40, 90
     op, ref = K.PageTables(B, rows, 200, 8, 30, device), P64.Tables(B, rows, 200, 8, 30)
