@@ -50,7 +50,9 @@ typedef struct krk_adapter_shape {
 /* An index outside 0 .. adapters - 1 is no adapter: out is y (or silu(gate) * up of
  * it).  Products x A^T are summed in fp32 and enter the second product as two bf16
  * parts (off by 2^-16); the sum with y, and silu, are taken in fp32 with one rounding
- * at the end.  Rows do not reach into each other's results, whatever they hold. */
+ * at the end.  Rows do not reach into each other's results, whatever they hold.
+ * An infinite value of B gives NaN (or an infinity, as the two parts have it) to the
+ * rows of its adapter. */
 typedef struct krk_adapter_args {
     const void* x;            /* [rows, K], row stride ldx (multiple of 8) */
     int64_t ldx;

@@ -2,80 +2,14 @@
 // checks, how the work is cut, and stream-ordered launches.  Nothing here
 // allocates, synchronises or touches device memory from the host, so every
 // call is graph-capturable.
-#include <hip/hip_runtime.h>
-#include <stdarg.h>
-#include <stdint.h>
-#include <stdio.h>
-
-#include <atomic>
-#include <utility>
-
 #include "krk_attn.h"
 #include "krk_attn_split.h"
 #include "krk_attn_tile.h"
 #include "krk_evict.h"
+#include "krk_host.h"
 #include "krk_rope.h"
 
 namespace {
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof g_err, fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-constexpr int kCuCount = 256;  // MI355X: 8 XCDs x 32 CUs
-constexpr int64_t kMaxStride = (int64_t)1 << 40;
-
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-
-int hip_status(hipError_t e, const char* what) {
-    if (e == hipSuccess) return KRK_ATTN_OK;
-    return fail(KRK_ATTN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
-// Raise a kernel's dynamic-LDS limit on the current device, once per device
-// and kernel.
-hipError_t ensure_lds_limit(const void* fn, size_t bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
-    if (bit && (done.load(std::memory_order_acquire) & bit)) return hipSuccess;
-    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == hipSuccess && bit) done.fetch_or(bit, std::memory_order_acq_rel);
-    return e;
-}
-
-// ------------------------------------------------------------------ checks
-struct Span {
-    uintptr_t a, b;
-};
-bool overlaps(const Span& x, const Span& y) { return x.a < y.b && y.a < x.b; }
-Span span(const void* p, uint64_t elems, size_t size) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-    return p ? Span{a, a + elems * size} : Span{0, 0};
-}
-
-// Whether no two elements of a written operand share memory: sorted by stride,
-// each is at least the extent of those inside it.  (Strides of extents of one
-// are 0.)
-bool nested(const int64_t (&stride)[3], const int64_t (&n)[3], int64_t inner) {
-    int at[3] = {0, 1, 2};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[at[j]] < stride[at[i]]) std::swap(at[i], at[j]);
-    for (int i : at) {
-        if (n[i] > 1 && stride[i] < inner) return false;
-        inner += (n[i] - 1) * stride[i];
-    }
-    return true;
-}
 
 // A cache of `seqs` sequences, `slots` keys, `heads` heads of `dim`.  Strides
 // of extents of one are of no matter and set to 0.
@@ -99,45 +33,9 @@ int check_cache(const char* name, krk_cache& c, int64_t seqs, int64_t slots, int
     return KRK_ATTN_OK;
 }
 
-// Whether two written caches of one shape share memory.  Views whose spans meet
-// (k and v side by side in one tensor) have to have the same strides; they are
-// apart if no step from a row of one to a row of the other is shorter than a row.
-// A step's part along the largest stride is one of the two multiples next to it,
-// as what is left has to lie within the extent inside that stride.
-bool apart(int64_t d, const int64_t (&stride)[3], const int64_t (&n)[3], int dim, int level = 0) {
-    if (level == 3) return d <= -dim || d >= dim;
-    const int64_t s = stride[level];
-    if (s == 0) return apart(d, stride, n, dim, level + 1);
-    int64_t q = d / s;
-    if (q * s > d) --q;
-    for (int64_t i = q; i <= q + 1; ++i)
-        if (i > -n[level] && i < n[level] && !apart(d - i * s, stride, n, dim, level + 1)) return false;
-    return true;
-}
 bool share_memory(const krk_cache& x, const Span& xs, const krk_cache& y, const Span& ys, int64_t seqs, int64_t slots, int64_t heads,
                   int dim) {
-    if (!overlaps(xs, ys)) return false;
-    if (x.seq != y.seq || x.slot != y.slot || x.head != y.head) return true;
-    const intptr_t bytes = reinterpret_cast<intptr_t>(y.p) - reinterpret_cast<intptr_t>(x.p);
-    int64_t stride[3] = {x.seq, x.slot, x.head}, n[3] = {seqs, slots, heads};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[j] > stride[i]) {
-                std::swap(stride[i], stride[j]);
-                std::swap(n[i], n[j]);
-            }
-    return !apart(bytes / 2, stride, n, dim);
-}
-
-// [rows, cols] operand; one row's stride is of no matter and set to its length.
-int check_rows(const char* name, const void* p, int64_t& row, int64_t rows, int64_t cols, Span* out) {
-    if (rows == 1) row = cols;
-    if (!p) return fail(KRK_ATTN_ERR_INVALID, "%s: null pointer", name);
-    if (row < cols || row > kMaxStride) return fail(KRK_ATTN_ERR_INVALID, "%s: row stride %lld must be >= %lld", name, (long long)row, (long long)cols);
-    if (row % 8) return fail(KRK_ATTN_ERR_ALIGN, "%s: the row stride must be a multiple of 8 elements", name);
-    if (reinterpret_cast<uintptr_t>(p) % 16) return fail(KRK_ATTN_ERR_ALIGN, "%s must be 16-byte aligned", name);
-    *out = span(p, (uint64_t)((rows - 1) * row + cols), 2);
-    return KRK_ATTN_OK;
+    return share_memory(x.p, xs, {x.seq, x.slot, x.head}, y.p, ys, {y.seq, y.slot, y.head}, {seqs, slots, heads}, dim);
 }
 
 int check_scores(const char* name, const void* p, int64_t& seq, int64_t& head, int64_t seqs, int64_t heads, int64_t slots,

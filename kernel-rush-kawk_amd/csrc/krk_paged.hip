@@ -42,20 +42,6 @@ int check_table(const void* table, int64_t& row, int B, int width, Span* out) {
     return check_words("table", table, (uint64_t)((B - 1) * row + width), out);
 }
 
-// Whether no two elements of a written operand share memory: sorted by stride, each
-// is at least the extent of those inside it.  (Strides of extents of one are 0.)
-bool nested(const int64_t (&stride)[3], const int64_t (&n)[3], int64_t inner) {
-    int at[3] = {0, 1, 2};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[at[j]] < stride[at[i]]) std::swap(at[i], at[j]);
-    for (int i : at) {
-        if (n[i] > 1 && stride[i] < inner) return false;
-        inner += (n[i] - 1) * stride[i];
-    }
-    return true;
-}
-
 // A pool of keys or values.  Strides of extents of one are of no matter and set to 0.
 int check_pages(const char* name, krk_pages& c, int64_t pages, int64_t slots, int64_t heads, int dim, bool written, Span* out) {
     if (!c.p) return fail(kErrInvalid, "%s: null pointer", name);
@@ -76,34 +62,9 @@ int check_pages(const char* name, krk_pages& c, int64_t pages, int64_t slots, in
     return 0;
 }
 
-// Whether two written pools of one shape share memory.  Views whose spans meet (k and
-// v side by side in one tensor) have to have the same strides; they are apart if no
-// step from a row of one to a row of the other is shorter than a row.  A step's part
-// along the largest stride is one of the two multiples next to it, as what is left
-// has to lie within the extent inside that stride.
-bool apart(int64_t d, const int64_t (&stride)[3], const int64_t (&n)[3], int dim, int level = 0) {
-    if (level == 3) return d <= -dim || d >= dim;
-    const int64_t s = stride[level];
-    if (s == 0) return apart(d, stride, n, dim, level + 1);
-    int64_t q = d / s;
-    if (q * s > d) --q;
-    for (int64_t i = q; i <= q + 1; ++i)
-        if (i > -n[level] && i < n[level] && !apart(d - i * s, stride, n, dim, level + 1)) return false;
-    return true;
-}
 bool share_memory(const krk_pages& x, const Span& xs, const krk_pages& y, const Span& ys, int64_t pages, int64_t slots, int64_t heads,
                   int dim) {
-    if (!overlaps(xs, ys)) return false;
-    if (x.page != y.page || x.slot != y.slot || x.head != y.head) return true;
-    const intptr_t bytes = reinterpret_cast<intptr_t>(y.p) - reinterpret_cast<intptr_t>(x.p);
-    int64_t stride[3] = {x.page, x.slot, x.head}, n[3] = {pages, slots, heads};
-    for (int i = 0; i < 3; ++i)
-        for (int j = i + 1; j < 3; ++j)
-            if (stride[j] > stride[i]) {
-                std::swap(stride[i], stride[j]);
-                std::swap(n[i], n[j]);
-            }
-    return !apart(bytes / 2, stride, n, dim);
+    return share_memory(x.p, xs, {x.page, x.slot, x.head}, y.p, ys, {y.page, y.slot, y.head}, {pages, slots, heads}, dim);
 }
 
 int check_heads(int rows, int heads, int kv_heads, int head_dim) {

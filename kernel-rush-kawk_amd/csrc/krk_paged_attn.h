@@ -152,7 +152,10 @@ struct Ranges {
         few = rounds >= 2.0f ? at_least(share / (kFewCost * rounds), kFewLeast) : at_least((float)few * (float)jobs * (1.0f / kTarget), kFewLeast);
         inv_few = __builtin_amdgcn_rcpf((float)few);
     }
-    static __device__ __forceinline__ int at_least(float steps, int least) { return (int)steps + 1 > least ? (int)steps + 1 : least; }
+    static __device__ __forceinline__ int at_least(float steps, int least) {
+        const int n = (int)fminf(steps, 1e9f) + 1;
+        return n > least ? n : least;
+    }
     __device__ __forceinline__ int parts(const Tiling& t) const {
         return t.steps > (t.many ? many : few) ? (int)((float)(t.steps - 1) * (t.many ? inv_many : inv_few)) + 1 : 1;
     }

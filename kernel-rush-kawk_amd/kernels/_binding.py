@@ -165,6 +165,6 @@ class Owner:
 
 
 def refuse_capture(device) -> None:
-    """Memory of an object is filled when it is built."""
+    """Memory of an object is filled, and waited for, when it is built."""
     if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("an object's memory is filled when it is built: build it before the capture")

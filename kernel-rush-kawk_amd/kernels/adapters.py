@@ -3,8 +3,8 @@
 :class:`LowRankAdapters` adds ``scale[i] * (x A_i^T) B_i^T`` to a projection's output,
 with i each row's own adapter, or none (the reference has no adapters).  Calls launch
 on torch's current stream, never synchronise, and may be captured in a graph; an
-object's calls are ordered on one stream, and a graph that holds them needs the object
-as long as it is replayed.  All compute runs in libkrk_adapter.so; there is no fallback.
+object's calls are ordered on one stream; it is built before a graph is captured, and a
+graph that holds its calls needs it as long as it is replayed.  All compute runs in libkrk_adapter.so; there is no fallback.
 """
 
 from __future__ import annotations
@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from ._adapter_lib import LIB, PACK, SLICES, Shape
-from ._binding import Owner, blocks, index_of, ints, plain, rows as _rows
+from ._binding import Owner, blocks, index_of, ints, plain, refuse_capture, rows as _rows
 
 __all__ = ["LowRankAdapters"]
 
@@ -40,6 +40,7 @@ class LowRankAdapters(Owner):
         LIB.check(LIB.load().krk_adapter_check(_byref(self._shape)))
         self.rows, self.N, self.K, self.rank, self.silu, self.widths = rows, N, K, rank, bool(silu), tuple(widths)
         self.out_cols = N // 2 if silu else N
+        refuse_capture(device)
         self.workspace = torch.empty(int(LIB.load().krk_adapter_workspace_bytes(_byref(self._shape))), dtype=torch.uint8, device=device)
         super().__init__(device, (self.workspace,))
 

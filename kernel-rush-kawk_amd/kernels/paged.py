@@ -183,9 +183,9 @@ class PagedAttention(Owner):
         self.scale = float(head_dim ** -0.5 if scale is None else scale)
         nbytes = int(LIB.load().krk_paged_workspace_bytes(_byref(self._shape)))
         self._q_shape = (rows, heads * head_dim)
+        refuse_capture(device)
         if workspace is None:
             if nbytes:
-                refuse_capture(device)
                 workspace = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         elif workspace.dtype is not torch.uint8 or workspace.numel() < nbytes or not workspace.is_contiguous():
             raise ValueError(f"workspace must be {nbytes} contiguous bytes (uint8) or more, got {workspace.dtype} {tuple(workspace.shape)}")

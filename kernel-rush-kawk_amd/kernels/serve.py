@@ -14,6 +14,7 @@ import torch
 
 from . import attention as A
 from . import paged as P
+from ._binding import refuse_capture
 from .adapters import LowRankAdapters
 
 _BF16, _I32 = torch.bfloat16, torch.int32
@@ -40,6 +41,7 @@ class PagedCache:
     def __init__(self, m, B: int, rows: int, pages: int, page_size: int = 64, *, width: int | None = None, window: int = 0,
                  sinks: int = 0, max_positions: int | None = None):
         cfg, dev = m.cfg, m.device
+        refuse_capture(dev)
         width = pages if width is None else width
         self.m, self.B, self.rows, self.pages, self.page_size, self.width = m, B, rows, pages, page_size, width
         self.heads, self.kv_heads, self.head_dim = cfg.heads, cfg.kv_heads, cfg.head_dim
@@ -116,7 +118,7 @@ class PagedCache:
         verified draft."""
         if len(rows) != self.B or any(not 0 <= n <= have for n, have in zip(rows, self.lens)):
             raise ValueError(f"rollback needs 0 .. keys rows for each of {self.B} requests, got {list(rows)}")
-        self.lens = [have - n for have, n in zip(self.lens, rows)]
+        self.lens = [have - int(n) for have, n in zip(self.lens, rows)]
         self._plan = None
 
     def reset(self, b: int | None = None) -> None:
@@ -151,6 +153,7 @@ class AdapterSet:
         if adapters < 1:
             raise ValueError(f"adapters={adapters} must be >= 1")
         cfg, dev = m.cfg, m.device
+        refuse_capture(dev)
         D = cfg.head_dim
         q, kv, I = cfg.heads * D, cfg.kv_heads * D, cfg.intermediate
         widths = {"qkv": (q, kv, kv), "o": (cfg.hidden,), "gu": (I, I), "d": (cfg.hidden,)}

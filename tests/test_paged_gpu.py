@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import kernels as K
+from kernels.step import synthetic_model
 from oracle import attn_ref as A64
 from oracle import paged_ref as P64
 from test_attn_gpu import close, gen, rnd, say
@@ -481,9 +482,13 @@ def test_python_refusals(device):
     for kw in (dict(new=keys.long()), dict(new=keys[:1]), dict(new=keys, keep=keys.cpu()), dict(new=keys, labels=starts)):
         with pytest.raises(ValueError):
             t.step(**kw)
+    model = synthetic_model(device, layers=1, hidden=64, intermediate=64, heads=8, kv_heads=2, vocab=64)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         q.zero_()
-        for build in (lambda: K.PageTables(2, 4, 5, 16, 3, device),):
+        for build in (lambda: K.PageTables(2, 4, 5, 16, 3, device), lambda: K.PagedAttention(2, 4, 8, 2, 128, 16, 3, device),
+                      lambda: K.PagedAttention(2, 4, 8, 2, 128, 16, 3, device, workspace=op.workspace),
+                      lambda: K.LowRankAdapters(4, 64, 128, 8, device), lambda: K.PagedCache(model, 2, 4, 8, 16),
+                      lambda: K.AdapterSet(model, 2, 8)):
             with pytest.raises(RuntimeError, match="before the capture"):
                 build()
