@@ -39,6 +39,11 @@ struct Plan {
 };
 
 constexpr int kFewRows = 256;
+// Tiles of 16 that a workgroup of the second product takes of many rows: 32 rows read B
+// half as often as 16 (4096 rows of 2560 columns, a call: 51 us, in 16 or 64 rows 53);
+// with gate and up in registers 16 leave room for more workgroups (2048 rows: 57 us, 63).
+template <bool SILU>
+constexpr int kManyTiles = SILU ? 1 : 2;
 // Workgroups that the slots of a tile's adapters may come to: those without one cost 9 ns
 // each (64 rows of 4 runs, 38 blocks of columns: a workgroup for every row took 25 us).
 constexpr int kSlotBlocks = 1024;
@@ -66,7 +71,7 @@ Plan make_plan(const krk_adapter_shape& s) {
     p.shrink_slots = slots((int64_t)p.tiles * p.groups * p.splits, most_sets);
     for (int i = 0; i < s.slices; ++i) p.col_blocks += (int)cdiv(s.widths[i], krk::kAdapterWaves * krk::kAdapterCols);
     if (s.silu) p.col_blocks = (int)cdiv(s.N / 2, krk::kAdapterWaves * krk::kAdapterCols);
-    const int expand_tiles = p.many ? (int)cdiv(s.rows, 32) : p.tiles;
+    const int expand_tiles = p.many ? (int)cdiv(s.rows, 16 * (s.silu ? kManyTiles<true> : kManyTiles<false>)) : p.tiles;
     p.expand_slots = slots((int64_t)expand_tiles * p.col_blocks, most_sets);
     const size_t values = (size_t)s.rows * s.slices * s.rank;
     p.h = align_up(p.splits * values * sizeof(float), 256);
@@ -90,7 +95,7 @@ int launch_expand(krk::AdapterParams p, const Plan& plan, hipStream_t st) {
     void* kargs[] = {(void*)&p};
     const void* fn = reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, SILU, JOINED>);
     static std::atomic<uint64_t> done{0};
-    constexpr size_t rows = JOINED ? 0 : 16 * MT * (SILU ? 2 : 1);
+    constexpr size_t rows = 16 * MT * (SILU ? 2 : 1);
     if (rows)
         if (hipError_t x = ensure_lds_limit(fn, rows * krk::adapter_row_bytes(128), done)) return hip_status(x, "adapter_expand_kernel LDS size");
     const hipError_t e = hipLaunchKernel(fn, dim3(plan.col_blocks, (unsigned)cdiv(p.rows, 16 * MT) * p.slots), dim3(krk::kAdapterThreads), kargs,
@@ -107,8 +112,7 @@ int launch(const krk::AdapterParams& p, const Plan& plan, hipStream_t st) {
     const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_join_kernel), dim3((unsigned)cdiv((int64_t)p.rows * (p.HN / 4), 256)),
                                          dim3(256), kargs, 0, st);
     if (int rc = hip_status(e, "adapter_join_kernel launch")) return rc;
-    // 32 rows: with 64 few workgroups are left (4096 rows of 2560 columns: 31 us against 23).
-    return launch_expand<2, SILU, true>(p, plan, st);
+    return launch_expand<kManyTiles<SILU>, SILU, true>(p, plan, st);
 }
 
 // A factor of each adapter: [adapters, rows, cols].

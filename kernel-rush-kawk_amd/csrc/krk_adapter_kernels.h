@@ -297,8 +297,10 @@ __host__ __device__ constexpr int adapter_row_bytes(int rank) { return 4 * rank 
 // 64 of the columns.  Of a tile of 16 columns lane group q gets four; tiles are
 // interleaved so that those of two are 8 neighbours, 16 bytes beside the next group's:
 // row i of tile t is column 32 (t >> 1) + 8 (i >> 2) + 4 (t & 1) + (i & 3).  Blocks of
-// columns change fastest, so that rows are read and written whole.  An adapter's B (of the first 32 of its rank) and y are on their way
-// before h is put together (or, JOINED, read as adapter_join_kernel left it).
+// columns change fastest, so that rows are read and written whole.  An adapter's B (of
+// the first 32 of its rank) and y are on their way before h is put together (or, JOINED,
+// copied as adapter_join_kernel left it).  h comes through LDS, once for the four waves
+// (each wave's own loads, in two steps: 4096 rows of 2560 columns 22.6 us, now 19).
 template <int MT, bool SILU, bool JOINED>
 __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_expand_kernel(AdapterParams p) {
     constexpr int PARTS = SILU ? 2 : 1, TR = 16 * MT;
@@ -361,8 +363,18 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_expand_kernel(Adap
     };
     if (n > 0) load();
 
-    const int pitch = JOINED ? 4 * p.HN : adapter_row_bytes(p.rank);
-    if constexpr (!JOINED) {
+    const int pitch = adapter_row_bytes(p.rank);
+    if constexpr (JOINED) {
+        const int r4 = p.rank / 4;  // 16 bytes each of a row's h, both parts
+        for (int e = threadIdx.x; e < PARTS * TR * r4; e += kAdapterThreads) {
+            const int u = PARTS > 1 && e >= TR * r4;
+            const int i = (e - u * TR * r4) / r4, j = e - u * TR * r4 - i * r4;
+            const int row = sets.row0 + i < p.rows ? sets.row0 + i : p.rows - 1;
+            *reinterpret_cast<u32x4*>(lds + (u * TR + i) * pitch + 16 * j) =
+                load_cached16(p.joined + (int64_t)row * 2 * p.HN + 2 * part[PARTS > 1 ? u : 0] + 8 * j);
+        }
+        __syncthreads();
+    } else {
         const int r4 = p.rank / 4;
         for (int e = threadIdx.x; e < PARTS * TR * r4; e += kAdapterThreads) {
             const int u = PARTS > 1 && e >= TR * r4;
@@ -392,13 +404,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_expand_kernel(Adap
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         if (!has(i)) continue;
-                        const unsigned char* h;
-                        if constexpr (JOINED) {
-                            const int row = sets.row0 + 16 * i + n16;
-                            h = reinterpret_cast<const unsigned char*>(p.joined) + (int64_t)(row < p.rows ? row : p.rows - 1) * pitch + 4 * part[u];
-                        } else {
-                            h = lds + (u * TR + 16 * i + n16) * pitch;
-                        }
+                        const unsigned char* h = lds + (u * TR + 16 * i + n16) * pitch;
                         u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
                         if (g < r8) {
                             hi = *reinterpret_cast<const u32x4*>(h + 16 * g);
