@@ -87,7 +87,8 @@ struct RowSets {
 };
 
 // h of 16 rows, 64 rows of A and one range of K.  The waves take 128 of K in turn, all
-// of their loads in flight at once, and meet in LDS.
+// of their loads in flight at once, and meet in LDS.  Bound by latency: 32 rows of 2560
+// over 16 adapters 6 us, 4.6 with one row.
 __global__ void __launch_bounds__(kAdapterThreads, 2) adapter_shrink_kernel(AdapterParams p) {
     constexpr int U = kAdapterFewStep / 32;
     __shared__ f32x4 lds[kAdapterWaves][kAdapterTiles][64];
