@@ -1,7 +1,7 @@
 // Page tables, slots and positions of a step from the requests' lengths (gfx950).
 //
 // Integers only, a few bytes a request and row: bound by latency (64 requests of one row
-// 5.3 us, 256 of 8500 rows 10.7; a small launch takes 2).  One workgroup
+// 5.4 us, 256 of 8500 rows 9.4; a small launch takes 2).  One workgroup
 // does the whole step: the requests' sums (rows, pages given back, pages taken)
 // are three scans over LDS, then the pages move (a thread a page), then the rows
 // are mapped (a thread a row), each finding its request by bisection of the sums.
@@ -69,7 +69,7 @@ __device__ __forceinline__ int owner_of(const int* first, int n, int x) {
 
 // N rows of the step, r, r + apart, ...: starts and keys as the step leaves them.  Side by
 // side, as each is a chain of reads (requests' sums, table, label): 8500 rows of 256
-// requests one after the other 9 us, four at a time 6.
+// requests in one workgroup took 9 us one after the other, four at a time 6.
 template <int N>
 __device__ __forceinline__ void map_rows(const PageStepParams& p, const int* starts, const int* keys, int r, int apart) {
     const int total = starts[p.B];

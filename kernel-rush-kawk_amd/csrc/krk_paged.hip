@@ -11,9 +11,9 @@
 namespace {
 
 constexpr int kMaxRequests = 4096, kMaxRows = 1 << 18;
-// Rows that the one workgroup of a page step maps itself; more have a launch of
-// their own.
-constexpr int kStepRows = 16384;
+// Rows that the one workgroup of a page step maps itself, four a thread at once; more
+// have a launch of their own (8500 rows of 256 requests 9.4 us, 10.8 without).
+constexpr int kStepRows = 4 * krk::kPageThreads;
 
 // log2 of a page's slots, or a negative code.
 int page_shift(int page_size) {
