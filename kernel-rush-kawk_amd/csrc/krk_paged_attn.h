@@ -12,7 +12,8 @@
 // a launch in front).  Keys are cut by
 // length: into ranges that cost about what one of kTarget workgroups would take of
 // all of the call's work, so a long request beside short ones does not work on alone.
-// The workgroup that finishes the last range of a tile joins them, in order.
+// The workgroup that finishes the last range of a tile joins them, in order (many ranges
+// of many rows: group by group, and the groups then).
 //
 // Products, key order and the treatment of infinities and NaNs in masked places are
 // those of the contiguous caches' kernels.
@@ -66,6 +67,10 @@ constexpr int kManyRows = 128;  // rows of a job of many
 // one of two workgroups of a CU (head size 128; only their proportion is of matter).
 constexpr int kFewStep = 32 * kPagedWaves, kManyStep = 64;
 constexpr int kFewLeast = 1, kManyLeast = 4;
+// A tile of many steps has longer ranges at least, by one step for every kManyMore: each
+// range's 64 KB is joined by one workgroup (one request of 32 rows over 5200 keys: 58 us
+// in ranges of 4 steps, 48 of 6, 49 of 8; over 1000 keys of 20 rows 25, 27, 30).
+constexpr int kManyMore = 32;
 constexpr float kFewCost = 5.0f, kManyCost = 2.0f;
 // Jobs that do not all run at once: where a share of the work is long, ranges of few
 // rows are cut finer, into up to kRounds a workgroup of at least kGrain us each.
@@ -157,7 +162,11 @@ struct Ranges {
         return n > least ? n : least;
     }
     __device__ __forceinline__ int parts(const Tiling& t) const {
-        return t.steps > (t.many ? many : few) ? (int)((float)(t.steps - 1) * (t.many ? inv_many : inv_few)) + 1 : 1;
+        const int least = kManyLeast + t.steps / kManyMore;
+        const bool longer = t.many && least > many;
+        const int len = longer ? least : t.many ? many : few;
+        const float inv = longer ? __builtin_amdgcn_rcpf((float)least) : t.many ? inv_many : inv_few;
+        return t.steps > len ? (int)((float)(t.steps - 1) * inv) + 1 : 1;
     }
 };
 __device__ __forceinline__ float cost_of(const Tiling& t) { return (float)(t.tiles * t.steps) * (t.many ? kManyCost : kFewCost); }
@@ -187,8 +196,8 @@ struct Job {
     int part, parts;    // range, of how many
     int slot;           // of parts > 1: row of the tile's first range's results
     Request req;
-    // The tile's counter: it has 32 rows of results at least.
-    __device__ __forceinline__ int counter() const { return slot >> 4; }
+    // The counter of range `part`: each has 16 rows of results at least.
+    __device__ __forceinline__ int counter(int part) const { return (slot + part * tile) >> 4; }
     // place: of a request's jobs.  Heads change fastest, then ranges, then tiles, those
     // that see more keys first.
     __device__ __forceinline__ void at(const PagedParams& p, const Tiling& t, int place, int slot0) {
@@ -444,19 +453,25 @@ struct Merged {
     }
 };
 
-// Joins all ranges of a tile with the whole workgroup: every four outputs of a row are
-// one thread's, or (few rows) several threads', each with every groups-th range,
-// which then meet in LDS in order: the result does not depend on which range finished
-// first.  A thread has loads of up to kJoinUnits of its outputs and kJoinParts ranges in
+// Which ranges of a tile are joined: part, part + apart, ... (`parts` of them); into the
+// tile's results, or (`again`) into the first one's place, to be joined with others.
+struct Joined {
+    int part, apart, parts;
+    bool again;
+};
+// Joins them with the whole workgroup: every four outputs of a row are one thread's, or
+// (few rows) several threads', each with every groups-th range, which then meet in LDS
+// in order: the result does not depend on which range finished first.  A thread has loads of up to kJoinUnits of its outputs and kJoinParts ranges in
 // flight at a time, as each is a round trip beyond this XCD's L2.
-constexpr int kJoinUnits = 4, kJoinParts = 4;
+constexpr int kJoinUnits = 4, kJoinParts = 4, kJoinAlone = 8;
 template <int D>
-__device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, unsigned char* lds) {
+__device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, const Joined& of, unsigned char* lds) {
     const int left = j.req.n * p.G - j.row0;
     const int units = (left < j.tile ? left : j.tile) * (D / 4);
+    auto place = [&](int nth, int e) { return j.slot + (int64_t)(of.part + nth * of.apart) * j.tile + e / (D / 4); };
     // Outputs first, first + kPagedThreads, ... (of `units`), over ranges from, from + step, ...
     auto join = [&](Merged (&y)[kJoinUnits], int first, int from, int step) {
-        for (int s0 = from; s0 < j.parts; s0 += kJoinParts * step) {
+        for (int s0 = from; s0 < of.parts; s0 += kJoinParts * step) {
             float2 ml[kJoinUnits][kJoinParts];
             f32x4 x[kJoinUnits][kJoinParts];
 #pragma unroll
@@ -466,7 +481,7 @@ __device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, un
 #pragma unroll
                 for (int s = 0; s < kJoinParts; ++s) {
                     const int at = s0 + s * step;
-                    const int64_t g = j.slot + (int64_t)(at < j.parts ? at : s0) * j.tile + e / (D / 4);
+                    const int64_t g = place(at < of.parts ? at : s0, e);
                     ml[u][s] = get_agent(p.ml + g);
                     x[u][s] = get_agent(p.part + g * D + 4 * (e % (D / 4)));
                 }
@@ -476,12 +491,18 @@ __device__ __forceinline__ void join_tile(const PagedParams& p, const Job& j, un
                 if (u && first + u * kPagedThreads >= units) break;
 #pragma unroll
                 for (int s = 0; s < kJoinParts; ++s)
-                    if (s0 + s * step < j.parts) y[u].add(p.c, ml[u][s].x, ml[u][s].y, x[u][s]);
+                    if (s0 + s * step < of.parts) y[u].add(p.c, ml[u][s].x, ml[u][s].y, x[u][s]);
             }
         }
     };
     auto finish = [&](const Merged& y, int e) {
-        finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+        if (of.again) {  // read by this thread alone, and its row's maximum and sum by this wave alone
+            const int64_t g = place(0, e);
+            put_agent(p.part + g * D + 4 * (e % (D / 4)), y.o);
+            if (e % (D / 4) == 0) put_agent(p.ml + g, make_float2(y.M, y.L));
+        } else {
+            finish_row(p, j, j.row0 + e / (D / 4), D, 4 * (e % (D / 4)), y.o, y.M, y.L);
+        }
     };
     int groups = 1;
     while (2 * groups * units <= kPagedThreads && groups < 8) groups *= 2;
@@ -746,22 +767,45 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
     }
 }
 
-// Whether this workgroup's was the last range of its tile.  (Through the front of lds,
+// Whether this workgroup was the last of `all` at a counter.  (Through the front of lds,
 // which nobody uses any more: the tile kernel's 80 KB are all that two workgroups of a
 // CU can have.)
-__device__ __forceinline__ bool last_range(const PagedParams& p, const Job& job, unsigned char* lds) {
+__device__ __forceinline__ bool last_of(const PagedParams& p, int counter, int all, unsigned char* lds) {
     int* last = reinterpret_cast<int*>(lds);
     drain_memory();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(p.ctr + job.counter(), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *last = before == (uint32_t)job.parts - 1;
-        if (*last) __hip_atomic_store(p.ctr + job.counter(), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(p.ctr + counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = before == (uint32_t)all - 1;
+        if (*last) __hip_atomic_store(p.ctr + counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     const bool yes = *last;
     __syncthreads();
     return yes;
+}
+
+// The ranges of a tile joined by the workgroups that finish last.  Many ranges of many
+// rows would keep the last one busy by itself: about sqrt(parts) of them at a time are
+// joined by the last of each such group, then those by the last group's (one request of
+// 32 rows over 5200 keys, 21 ranges: 66 us, in two goes 58; 12 rows, 14 ranges: 22.5 and
+// 19.7).
+template <int D>
+__device__ __forceinline__ void join_ranges(const PagedParams& p, const Job& job, unsigned char* lds) {
+    int per = job.parts;
+    if (job.parts > kJoinAlone && (job.req.n * p.G - job.row0) * (D / 4) > kPagedThreads / 2)
+        for (per = 3; per * per < job.parts; ++per) {}
+    const int group = job.part / per, groups = (job.parts + per - 1) / per;
+    const int left = job.parts - group * per;
+    Joined of = {group * per, 1, left < per ? left : per, groups > 1};
+    int counter = job.counter(of.part);
+    for (;;) {
+        if (!last_of(p, counter, of.parts, lds)) return;
+        join_tile<D>(p, job, of, lds);
+        if (!of.again) return;
+        of = {0, per, groups, false};
+        counter = job.counter(1);  // no group begins there
+    }
 }
 
 }  // namespace krk

@@ -486,8 +486,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_attn_kernel(PagedParam
     }
     const Job job = parked.job();
     if (job.parts == 1) return;
-    const PagedParams late = kernel_params();
-    if (last_range(late, job, lds)) join_tile<D>(late, job, lds);
+    join_ranges<D>(kernel_params(), job, lds);
 }
 
 }  // namespace krk

@@ -301,6 +301,15 @@ def test_many_requests(device, case, window, sinks):
     check_step(device, 550 + case, *CROWDS[case], window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("new,keys,heads,kv,D,P", [
+    ([20], [5244], 4, 1, 128, 16), ([32], [9000], 32, 8, 128, 64), ([17, 1], [3300, 40], 8, 2, 64, 16), ([12], [5000], 8, 2, 128, 16),
+    ([70, 9], [2900, 4000], 4, 1, 128, 8), ([24] + [1] * 70, [7000] + [9] * 70, 4, 1, 128, 16),
+])
+def test_many_ranges(device, new, keys, heads, kv, D, P):
+    """Few tiles over many keys: ranges that are joined in groups, and the groups then."""
+    check_step(device, 760 + sum(new), new, keys, heads, kv, D, P, odd=len(new) == 2)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (32, 0), (33, 40), (100, 4), (5000, 9)])
 @pytest.mark.parametrize("P", [8, 64])
 def test_window_and_sinks(device, window, sinks, P):
