@@ -67,7 +67,8 @@ Plan make_plan(const krk_adapter_shape& s) {
     const int64_t want = !p.many ? few : many > 0 ? many : 1;
     const int64_t most = p.many ? cdiv(s.K, 4 * krk::kAdapterManyStep) : cdiv(s.K, krk::kAdapterWaves * krk::kAdapterFewStep);
     p.splits = (int)(want < most ? want : most);
-    p.splits = p.splits < krk::kAdapterSplits ? p.splits : krk::kAdapterSplits;
+    const int limit = p.many ? krk::kAdapterManySplits : krk::kAdapterFewSplits;
+    p.splits = p.splits < limit ? p.splits : limit;
     p.shrink_slots = slots((int64_t)p.tiles * p.groups * p.splits, most_sets);
     for (int i = 0; i < s.slices; ++i) p.col_blocks += (int)cdiv(s.widths[i], krk::kAdapterWaves * krk::kAdapterCols);
     if (s.silu) p.col_blocks = (int)cdiv(s.N / 2, krk::kAdapterWaves * krk::kAdapterCols);
@@ -109,7 +110,9 @@ int launch(const krk::AdapterParams& p, const Plan& plan, hipStream_t st) {
     if (!plan.many) return launch_expand<1, SILU, false>(p, plan, st);
     krk::AdapterParams q = p;
     void* kargs[] = {(void*)&q};
-    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&krk::adapter_join_kernel), dim3((unsigned)cdiv((int64_t)p.rows * (p.HN / 4), 256)),
+    const void* fn = p.splits <= krk::kAdapterFewSplits ? reinterpret_cast<const void*>(&krk::adapter_join_kernel<krk::kAdapterFewSplits>)
+                                                        : reinterpret_cast<const void*>(&krk::adapter_join_kernel<krk::kAdapterManySplits>);
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)cdiv((int64_t)p.rows * (p.HN / 4), 256)),
                                          dim3(256), kargs, 0, st);
     if (int rc = hip_status(e, "adapter_join_kernel launch")) return rc;
     return launch_expand<kManyTiles<SILU>, SILU, true>(p, plan, st);

@@ -68,6 +68,7 @@ CASES = [
     (257, [512, 128, 128], 384, 16, 6, "runs"),
     (300, [328], 1000, 32, 9, "random"),
     (1031, [264], 640, 48, 4, "runs"),
+    (300, [264], 9728, 16, 4, "runs"),
 ]
 
 
