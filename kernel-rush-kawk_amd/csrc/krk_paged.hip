@@ -85,39 +85,8 @@ int check_shape(const krk_paged_shape& s) {
     return 0;
 }
 
-// -------------------------------------------------------------------- plan
-struct Plan {
-    bool many;  // some request may have more than kFewPairs rows of a head
-    int64_t blocks;
-    size_t ctr, part, ml, plan, bytes;  // workspace: sizes of its parts and their sum
-};
-
-Plan make_plan(const krk_paged_shape& s) {
-    Plan p{};
-    const int64_t RG = (int64_t)s.rows * (s.heads / s.kv_heads);
-    p.many = RG > krk::kFewPairs;
-    // A request with rows has up to two tiles where they are few, of 16 rows or more but
-    // for the last; else tiles of 128.
-    const int64_t live = s.B < s.rows ? s.B : s.rows;
-    const int64_t tiles = s.kv_heads * (RG / krk::kManyRows + (live < RG / 16 ? 2 * live : live + RG / 16));
-    // Their key ranges: as many as the longest request could have, and those of tiles
-    // that have several are limited.
-    const int64_t keys = (int64_t)s.width * s.page_size;
-    auto splits = [&](int64_t least, int64_t most) {
-        const int64_t parts = cdiv(keys, least);
-        return parts < 2 ? 0 : tiles * parts < most ? tiles * parts : most;
-    };
-    const int64_t few = splits(krk::kFewStep * krk::kFewLeast, krk::kFewSplits);
-    const int64_t many = p.many ? splits(krk::kManyStep * krk::kManyLeast, krk::kManySplits) : 0;
-    p.blocks = tiles + few + many;
-    const size_t rows = (size_t)(few * 32 + many * krk::kManyRows);
-    p.part = rows * s.head_dim * sizeof(float);
-    p.ml = rows * sizeof(float2);
-    if (s.B > krk::kLaneRequests) p.plan = 256 + (size_t)cdiv(p.blocks, s.kv_heads) * sizeof(krk::PlannedRange);
-    if (rows || p.plan) p.ctr = krk::kCounterBytes;  // also where this shape counts nothing: they stay zero
-    p.bytes = p.ctr + p.part + p.ml + p.plan;
-    return p;
-}
+using krk::Plan;
+using krk::make_plan;
 
 template <int D, bool MANY>
 int launch_attn(const krk::PagedParams& p, const Plan& plan, hipStream_t stream) {
