@@ -134,7 +134,9 @@ typedef struct krk_paged_rope_args {
 int krk_paged_rope_bf16(const krk_paged_rope_args* args, void* stream);
 
 /* What a call of krk_paged_attn_bf16 computes, fixed for an object that makes many of
- * them: it decides the grid and the workspace. */
+ * them: it decides the grid and the workspace.  A request's tiles of rows have a
+ * workgroup each per key/value head, fewer than 2^24 in all (only shapes of thousands
+ * of requests and of key/value heads can have more; krk_paged_check says so). */
 typedef struct krk_paged_shape {
     int B, rows;         /* requests; rows of the call (rows * heads < 2^25) */
     int heads, kv_heads; /* heads a multiple of kv_heads */

@@ -286,7 +286,7 @@ __device__ __forceinline__ f32x4 sum_h(const AdapterParams& p, int row, int j) {
 template <int SPLITS>
 __global__ void __launch_bounds__(256) adapter_join_kernel(AdapterParams p) {
     const int q = p.HN / 4;
-    const int e = (int)(blockIdx.x * 256 + threadIdx.x);  // rows * q < 2^25
+    const int e = (int)(blockIdx.x * 256 + threadIdx.x);  // rows * q <= 2^25
     const int row = e / q, j = 4 * (e - row * q);
     if (row >= p.rows) return;
     const SplitH h(sum_h<SPLITS>(p, row, j));

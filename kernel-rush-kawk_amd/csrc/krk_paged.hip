@@ -10,6 +10,9 @@
 
 namespace {
 
+using krk::make_plan;
+using krk::Plan;
+
 constexpr int kMaxRequests = 4096, kMaxRows = 1 << 18;
 // Rows that the one workgroup of a page step maps itself, four a thread at once; more
 // have a launch of their own (8500 rows of 256 requests 9.4 us, 10.8 without).
@@ -70,7 +73,8 @@ bool share_memory(const krk_pages& x, const Span& xs, const krk_pages& y, const 
 int check_heads(int rows, int heads, int kv_heads, int head_dim) {
     if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail(kErrInvalid, "heads=%d must be a multiple of kv_heads=%d, both >= 1", heads, kv_heads);
     if (head_dim != 64 && head_dim != 128) return fail(kErrUnsupported, "head_dim=%d: this build has 64 and 128", head_dim);
-    // Grids of up to 128 threads a row and head stay below 2^32 threads.
+    // The rotary embedding's grid: head_dim / 8 threads for each of up to 3 * heads heads
+    // of a row, below 2^32 threads.
     if ((int64_t)rows * heads >= (int64_t)1 << 25) return fail(kErrInvalid, "rows * heads = %lld must be below 2^25", (long long)((int64_t)rows * heads));
     return 0;
 }
@@ -82,11 +86,11 @@ int check_shape(const krk_paged_shape& s) {
     if (s.window < 0 || s.sinks < 0 || s.window >= 1 << 28 || s.sinks >= 1 << 28)
         return fail(kErrInvalid, "window=%d and sinks=%d must be 0 .. 2^28 - 1", s.window, s.sinks);
     if (s.sinks && !s.window) return fail(kErrInvalid, "sinks need a window");
+    if (const int64_t blocks = make_plan(s).blocks; blocks * krk::kPagedThreads >= (int64_t)1 << 32)
+        return fail(kErrInvalid, "%d rows of %d requests over %d heads take %lld workgroups: needs fewer than 2^32 threads in all", s.rows, s.B, s.kv_heads,
+                    (long long)blocks);
     return 0;
 }
-
-using krk::Plan;
-using krk::make_plan;
 
 template <int D, bool MANY>
 int launch_attn(const krk::PagedParams& p, const Plan& plan, hipStream_t stream) {

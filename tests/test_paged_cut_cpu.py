@@ -13,6 +13,7 @@ from pathlib import Path
 
 import pytest
 
+import kernels
 from kernels import _paged_lib as PL
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -58,6 +59,21 @@ def test_tiles_times_steps_beyond_31_bits(replay, rows, heads, kv, keys, D):
     r = replay([rows], [keys], heads, kv, D, 64)
     assert r["many_parts"] == 1  # far more tiles than workgroups
     replay([rows - 70] + [1] * 70, [keys] + [9] * 70, heads, kv, D, 64)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(B=4096, rows=4096, heads=8191, kv_heads=8191, width=1), dict(B=4096, rows=4096, heads=8191, kv_heads=8191, width=100),
+    dict(B=1, rows=1, heads=(1 << 25) - 1, kv_heads=(1 << 25) - 1, width=1),
+])
+def test_grids_beyond_32_bits_refused(kw):
+    """A workgroup of 256 threads for every tile of a key/value head, and fewer than 2^32 threads in all."""
+    lib, s = PL.LIB.load(), PL.Shape(head_dim=64, page_size=8, **kw)
+    assert lib.krk_paged_check(ctypes.byref(s)) == -1 and "2^32 threads" in lib.krk_paged_last_error().decode()
+    assert lib.krk_paged_workspace_bytes(ctypes.byref(s)) == 0
+    with pytest.raises(ValueError, match="threads"):
+        kernels.PagedAttention(**kw, head_dim=64, page_size=8, device="cpu")
+    s.heads = s.kv_heads = s.heads // 4
+    assert lib.krk_paged_check(ctypes.byref(s)) == 0
 
 
 def spread(rng, lo, hi):
