@@ -34,8 +34,8 @@ class PagedCache:
     those that :meth:`rollback` or :meth:`reset` took off, give their pages back when
     it begins.
 
-    ``labels`` (int32 ``[B]`` on the GPU) is each request's adapter, -1 for none; by row it
-    is ``tables.owner``.  ``window``, ``sinks``: sliding-window attention in every layer.
+    ``labels`` (int32 ``[B]`` on the GPU) is each request's adapter, -1 for none, as
+    :meth:`reset` leaves it; by row it is ``tables.owner``.  ``window``, ``sinks``: sliding-window attention in every layer.
     """
 
     def __init__(self, m, B: int, rows: int, pages: int, page_size: int = 64, *, width: int | None = None, window: int = 0,
@@ -122,9 +122,11 @@ class PagedCache:
         self._plan = None
 
     def reset(self, b: int | None = None) -> None:
-        """Forget request ``b`` (None: all): its pages are free for the next step."""
+        """Forget request ``b`` (None: all): its pages are free for the next step, and the
+        next request in its place has no adapter until its label is written."""
         for i in range(self.B) if b is None else [b]:
             self.lens[i] = 0
+        self.labels[slice(None) if b is None else b] = -1
         self._plan = None
 
     def idle(self) -> None:
