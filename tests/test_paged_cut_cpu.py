@@ -15,6 +15,7 @@ import pytest
 
 import kernels
 from kernels import _paged_lib as PL
+from test_paged_forms_gpu import FORMS
 
 ROOT = Path(__file__).resolve().parent.parent
 FIELDS = ("blocks", "rows", "counters", "jobs", "used", "pairs", "rounds", "few_parts", "many_parts", "wrong")
@@ -74,6 +75,13 @@ def test_grids_beyond_32_bits_refused(kw):
         kernels.PagedAttention(**kw, head_dim=64, page_size=8, device="cpu")
     s.heads = s.kv_heads = s.heads // 4
     assert lib.krk_paged_check(ctypes.byref(s)) == 0
+
+
+@pytest.mark.parametrize("name", list(FORMS))
+def test_forms_that_the_gpu_tests_reach(replay, name):
+    new, keys, heads, kv, D, P, window, sinks, want = FORMS[name]
+    r = replay(new, keys, heads, kv, D, P, rows=sum(new) + 3, width=-(-max(keys) // P) + 1, window=window, sinks=sinks)
+    assert all(r[k] >= n for k, n in want.items()), r
 
 
 def spread(rng, lo, hi):
