@@ -163,9 +163,10 @@ typedef struct krk_paged_shape {
  * starts have to ascend; where they do not, rows may be left as they were.
  *
  * Sums, maxima and weights are held in 32 bits.  The weights enter the products with
- * v as two bf16 parts (off by 2^-16), or, where a request has more than
- * KRK_PAGED_FEW_ROWS pairs of a row and a query head per key/value head, rounded to one:
- * an output is then off by up to 2^-8 of sum p |v| besides its own rounding.
+ * v as bf16 parts: of a request with up to 16 pairs of a row and a query head per
+ * key/value head as three (2^-24), with up to KRK_PAGED_FEW_ROWS as two (2^-16), with
+ * more rounded to one: an output is then off by up to 2^-8 of sum p |v| besides its own
+ * rounding.
  */
 #define KRK_PAGED_FEW_ROWS 64
 typedef struct krk_paged_attn_args {

@@ -384,13 +384,18 @@ constexpr size_t few_lds_bytes() {
 // requests of 300 to 16000 keys 383 us, 5.8 TB/s; one of 1000 keys 7.8 us, latency), so
 // a wave's loads run ahead: K's registers are loaded again as soon as the scores are
 // taken, V's as soon as the products are, and the page numbers of the step behind
-// those are on their way meanwhile.  Weights go into the second product as two bf16
-// parts (p = hi + lo, 16 bits of mantissa).
+// those are on their way meanwhile.  Weights go into the second product as bf16 parts,
+// three of up to 16 rows: all 24 bits of them, nearly under the time of the reads (one
+// request of 1000 keys 8.0 us, with two parts 7.9; 64 of 300 to 16000 keys 392 and 389;
+// with two, 1.4 outputs in 1000 of the one request were not the bf16 nearest to the exact
+// value, now 0.2).  Two of 32 rows, 16 bits: a third would cost 8 drafts of 16 rows 7%
+// (32.4 -> 34.6 us) for 0.7 outputs in 1000.
 template <int D, int MT>
 __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, unsigned char* lds) {
     constexpr int TR = 16 * MT;
     constexpr int KS = D / 32;
     constexpr int VD = D / 16;
+    constexpr int PARTS = MT == 1 ? 3 : 2;  // of a weight
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
@@ -491,7 +496,7 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
                     s[i][e >> 2][e & 3] = row_sees(pos[i], lo[i], p.sinks, key) ? s[i][e >> 2][e & 3] : kNegInf;
                 }
         }
-        bf16x8 hi[MT], low[MT];
+        bf16x8 weight[MT][PARTS];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             float mx = s[i][0][0];
@@ -508,15 +513,18 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
                 sum += w[e];
             }
             l[i] = l[i] * alpha + sum;
-            u32x4 ph, pl;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                ph[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
-                const uint32_t x = ph[e];
-                pl[e] = pack_bf16(w[2 * e] - bf16_to_f32(x & 0xffffu), w[2 * e + 1] - __uint_as_float(x & 0xffff0000u));
+            for (int n = 0; n < PARTS; ++n) {
+                u32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = pack_bf16(w[2 * e], w[2 * e + 1]);
+                    const uint32_t y = x[e];
+                    w[2 * e] -= bf16_to_f32(y & 0xffffu);  // what is left, exactly
+                    w[2 * e + 1] -= __uint_as_float(y & 0xffff0000u);
+                }
+                weight[i][n] = __builtin_bit_cast(bf16x8, x);
             }
-            hi[i] = __builtin_bit_cast(bf16x8, ph);
-            low[i] = __builtin_bit_cast(bf16x8, pl);
             if (__any(alpha != 1.0f)) {
 #pragma unroll
                 for (int j = 0; j < VD; ++j) acc[i][j] *= alpha;
@@ -530,7 +538,9 @@ __device__ __forceinline__ void few_rows(const PagedParams& p, const Job& job, u
         for (int j = 0; j < VD; ++j) {
             const bf16x8 a = vf.operand(j);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i][j] = mfma16(a, hi[i], mfma16(a, low[i], acc[i][j]));
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int n = PARTS - 1; n >= 0; --n) acc[i][j] = mfma16(a, weight[i][n], acc[i][j]);
         }
         if constexpr (MORE) load_v(span.key(next), vp);
         kp = kp2;

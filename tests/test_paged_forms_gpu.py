@@ -8,6 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import kernels as K
 from kernels import cache as C
 from kernels import serve as V
 from kernels import step as S
@@ -123,3 +124,29 @@ def test_zero_factors_in_front(device, model, targets):  # noqa: F811
     step.index.fill_(1)
     got = step.run(x)
     assert float((got.double() - plain.double()).norm() / plain.double().norm()) < 0.04
+
+
+@pytest.mark.parametrize("D,P,B,heads", [(128, 16, 33, 8), (64, 8, 70, 4)])
+def test_weights_of_single_tokens_keep_32_bits(device, D, P, B, heads):
+    """Two keys of weights 1 and w, and values that cancel but for what a bf16 leaves of w u:
+    out = (w u + v0) / (1 + w), v0 = -bf16(w u).
+
+    Scores are one exact product.  w is off by its exponent x's two roundings (|x| <= 2:
+    2 ln 2 2^-23) and exp2's unit (2^-23): 2.4 * 2^-23.  Three products and their sums, the
+    join of the waves and 1 / L: at most 8 half steps of fp32 of |w u| <= 2 |w u| / (1 + w)."""
+    g = torch.Generator().manual_seed(B)
+    x = -torch.rand((B, heads), generator=g) * 1.5 - 0.2  # scores: q x at key 1, 0 at key 0
+    table = torch.randperm(B, generator=g).to(I32).view(B, 1)
+    k, v, q = (torch.zeros(shape, dtype=BF) for shape in ((B, P, heads, D), (B, P, heads, D), (B, heads * D)))
+    k[:, 1, :, 5] = x.to(BF)[torch.argsort(table[:, 0])]  # by page
+    q.view(B, heads, D)[:, :, 5] = 1.0
+    w = k[table[:, 0].long(), 1, :, 5].double().exp()[:, :, None]
+    u = torch.randn((B, heads, D), generator=g).to(BF)
+    v0 = (-w * u.double()).to(BF)
+    v[table[:, 0].long(), 0], v[table[:, 0].long(), 1] = v0, u
+    op = K.PagedAttention(B, B, heads, heads, D, P, 1, device, scale=1.0)
+    starts, keys = torch.arange(B + 1, dtype=I32), torch.full((B,), 2, dtype=I32)
+    out = op(*(t.to(device) for t in (q, k, v, table, starts, keys))).view(B, heads, D)
+    ref, size = (w * u.double() + v0.double()) / (1 + w), w * u.double().abs() / (1 + w)
+    assert (ref.abs() < 2.0 ** -7 * size + 1e-30).all()
+    close(out, ref, STEP * ref.abs() * 1.01 + size * (2.4 * 2.0 ** -23 + 2 * 8 * 2.0 ** -24), "out")
