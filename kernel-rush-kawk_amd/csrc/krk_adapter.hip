@@ -97,8 +97,7 @@ int launch_expand(krk::AdapterParams p, const Plan& plan, hipStream_t st) {
     const void* fn = reinterpret_cast<const void*>(&krk::adapter_expand_kernel<MT, SILU, JOINED>);
     static std::atomic<uint64_t> done{0};
     constexpr size_t rows = 16 * MT * (SILU ? 2 : 1);
-    if (rows)
-        if (hipError_t x = ensure_lds_limit(fn, rows * krk::adapter_row_bytes(128), done)) return hip_status(x, "adapter_expand_kernel LDS size");
+    if (hipError_t x = ensure_lds_limit(fn, rows * krk::adapter_row_bytes(128), done)) return hip_status(x, "adapter_expand_kernel LDS size");
     const hipError_t e = hipLaunchKernel(fn, dim3(plan.col_blocks, (unsigned)cdiv(p.rows, 16 * MT) * p.slots), dim3(krk::kAdapterThreads), kargs,
                                          rows * krk::adapter_row_bytes(p.rank), st);
     return hip_status(e, "adapter_expand_kernel launch");
