@@ -381,7 +381,7 @@ constexpr size_t few_lds_bytes() {
 // Jobs of few rows: 16 * MT rows of a head against one range of keys, the four waves 32
 // keys at a time in turn.  Waves keep their own running maximum, sum and O and meet in
 // LDS once, at the end.  Bound by reading K and V once a tile (4 * D bytes a key; 64
-// requests of 300 to 16000 keys 383 us, 5.8 TB/s; one of 1000 keys 7.8 us, latency), so
+// requests of 300 to 16000 keys 383 to 392 us, 5.7 TB/s; one of 1000 keys 8 us, latency), so
 // a wave's loads run ahead: K's registers are loaded again as soon as the scores are
 // taken, V's as soon as the products are, and the page numbers of the step behind
 // those are on their way meanwhile.  Weights go into the second product as bf16 parts,

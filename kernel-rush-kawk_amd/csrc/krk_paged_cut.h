@@ -40,14 +40,15 @@ struct PagedParams {
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 
-// Workgroups that the work is cut for: one a CU, though two run at once (ranges half as
-// long: 4 drafts of 8 rows 21 -> 30 us, 100 rows over 16000 keys 86 -> 118, 32 requests of
-// 4000 keys 88 -> 98).
+// Workgroups that the work is cut for: one a CU, though two run at once (for 512, ranges
+// half as long: 4 drafts of 8 rows 19 -> 26 us, 100 rows over 16000 keys 84 -> 102, 500 over
+// 4000 73 -> 77, 32 requests of 4000 keys 88 -> 95; two chunks beside 48 requests 278 -> 271).
 constexpr int kTarget = 256;
 constexpr int kFewPairs = 64;   // rows of a head that tiles of few rows (16 or 32) take
 constexpr int kManyRows = 128;  // rows of a job of many
 // Keys of a step of a workgroup, least steps of a range, and what a step costs, in us of
-// one of two workgroups of a CU (head size 128; only their proportion is of matter).
+// one of two workgroups of a CU (of head size 128, and close enough for 64: many rows at 1.2
+// or 3.0 change its mixed calls by 1 to 4%; only the proportion is of matter).
 constexpr int kFewStep = 32 * kPagedWaves, kManyStep = 64;
 constexpr int kFewLeast = 1, kManyLeast = 4;
 // A tile of many steps has longer ranges at least, by one step for every kManyMore: each

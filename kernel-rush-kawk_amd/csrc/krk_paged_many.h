@@ -1,8 +1,8 @@
 // Attention over pages for requests of many rows (chunks of prompts): 128 rows of a
 // head a workgroup, K and V through LDS.
 //
-// Bound by the matrix pipe, LDS and the vector pipe alike (2048 rows over 16384 keys 489
-// us, 1055 TFLOP/s; the matrix pipe is busy half of the time), as the contiguous caches'
+// Bound by the matrix pipe, LDS and the vector pipe alike (2048 rows over 16384 keys
+// 490 to 520 us, 990 to 1050 TFLOP/s; the matrix pipe is busy half of the time), as the contiguous caches'
 // tile kernel is, whose fragments and orders of issue these are: four waves, each with 32
 // rows of its own, all reading the same 64-key steps from LDS; S^T = K Q^T and O^T = V^T
 // P^T on v_mfma_f32_32x32x16_bf16, weights staying in their lane; rings of three steps of

@@ -27,6 +27,8 @@ class PagedCache:
     steps of up to ``rows`` rows: ``pages`` pages of ``page_size`` slots, shared by all
     requests and numbered alike in all layers.
 
+    A step's projections and logits run over all ``rows``, whatever its plan brings.
+
     A step is planned by :meth:`schedule`, on the host, which refuses what does not fit;
     :meth:`begin` then moves pages, tables and lengths on, on the device, so a captured
     step serves every plan.  The host's own count of each request's keys
